@@ -7,6 +7,7 @@ import os
 from typing import Dict, Optional
 
 import numpy as np
+import torch
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "lib", "libdmn_hip.so")
@@ -18,6 +19,7 @@ if os.environ.get("DMN_LIB_VARIANT"):
 DMN_MAX_MULTS = 8
 TABLE_COLS = 12
 F32, BF16 = 0, 1
+DTYPE_CODES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}   # DMN_DT_* of include/dmn.h
 
 
 class DmnUnetCfg(C.Structure):
@@ -28,6 +30,10 @@ class DmnUnetCfg(C.Structure):
 
 class DmnTensorDesc(C.Structure):
     _fields_ = [("name", C.c_char_p), ("data", C.POINTER(C.c_float)), ("ndim", C.c_int), ("shape", C.c_int64 * 4)]
+
+
+class DmnGradTensor(C.Structure):
+    _fields_ = [("src", C.c_void_p), ("dst", C.c_void_p), ("numel", C.c_int64), ("src_dtype", C.c_int), ("dst_dtype", C.c_int)]
 
 
 _vp, _i, _f, _u64, _i64, _sz = C.c_void_p, C.c_int, C.c_float, C.c_uint64, C.c_int64, C.c_size_t
@@ -75,6 +81,11 @@ SIGNATURES = {
     "dmn_train_workspace_bytes": (_i, [_vp, _i, _i, _i, C.POINTER(_sz)]),
     "dmn_train_loss_and_grads": (_i, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _vp, _vp, _vp, _sz, _vp]),
     "dmn_adamw_step": (_i, [_vp, _vp, _vp, _vp, _i64, _f, _f, _f, _f, _f, _i, _f, _f, _vp, _vp]),
+    "dmn_layer_norm_forward": (_i, [_vp, _i64, _vp, _vp, _vp, _vp, _i64, _i, _i, _i, _f, _vp]),
+    "dmn_layer_norm_workspace_bytes": (_sz, [_i64, _i, _i]),
+    "dmn_layer_norm_backward": (_i, [_vp, _i64, _vp, _i64, _vp, _vp, _vp, _vp, _vp, _i64, _i, _i, _i, _vp, _sz, _vp]),
+    "dmn_clip_grads_workspace_bytes": (_sz, [_i]),
+    "dmn_clip_grads": (_i, [_vp, _i, _i, _f, _f, _vp, _vp, _sz, _vp]),
     "dmn_fill_normal": (_i, [_vp, _i, _i, _u64, C.c_uint32, _i64, _f, _vp]),
     "dmn_unet_set_sample_chains": (_i, [_vp, _i, _i]),
     "dmn_ddpm_loop_chains": (_i, [_vp, _i]),
@@ -139,8 +150,20 @@ def ptr(t) -> Optional[int]:
 
 
 def current_stream_handle(device=None) -> int:
-    import torch
     return torch.cuda.current_stream(device).cuda_stream
+
+
+def launch(device, fn, *args):
+    """Calls an entry point whose last argument is the stream: torch's current stream of `device`, with that device current."""
+    index = device.index if device.index is not None else torch.cuda.current_device()
+    stream = torch._C._cuda_getCurrentRawStream(index)
+    if torch.cuda.current_device() == index:
+        rc = fn(*args, stream)
+    else:
+        with torch.cuda.device(index):
+            rc = fn(*args, stream)
+    if rc != 0:
+        check(rc)
 
 
 def make_tensor_descs(params: Dict[str, np.ndarray]):

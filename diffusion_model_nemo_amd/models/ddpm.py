@@ -272,8 +272,8 @@ class DDPM(AbstractDiffusionModel):
         """models/ddpm.py:43-57: t ~ U{0..T-1}, eps ~ N(0, I), x_t = q_sample(x_0, t, eps), loss(net(x_t, t), eps).
         Forward AND backward run in the HIP kernels during this call; the returned scalar carries an autograd node
         whose backward hands the finished gradients to every parameter's `.grad` (scaled by the incoming gradient),
-        so `loss.backward()` followed by any torch optimiser behaves like the reference. `train_batch` is the
-        all-device alternative (all-reduce + clip + AdamW without leaving the GPU)."""
+        so `loss.backward()` followed by any torch optimiser behaves like the reference (`configure_gradient_clipping`
+        clips in between). `train_batch` is the all-device alternative (all-reduce + clip + AdamW without leaving the GPU)."""
         samples = batch["pixel_values"]
         B = samples.shape[0]
         dev = samples.device
@@ -288,6 +288,20 @@ class DDPM(AbstractDiffusionModel):
         params = [p for p in self.diffusion_model.parameters()]
         names = [n for n, _ in self.diffusion_model.named_parameters()]
         return _NativeLoss.apply(value, tr, names, *params)
+
+    def configure_gradient_clipping(self, optimizer, gradient_clip_val: Optional[float] = None,
+                                    gradient_clip_algorithm: Optional[str] = None):
+        """What a trainer's loop calls between `loss.backward()` and `optimizer.step()` (Lightning's hook of this name):
+        clips the `.grad`s of the optimizer's parameters to the global 2-norm `gradient_clip_val` (default: the config's
+        `trainer.gradient_clip_val`; None or 0: no clipping) with `training.clip_grad_norm_`. Returns the norm as a device
+        scalar, or None where nothing is clipped."""
+        from ..training import clip_grad_norm_
+        if gradient_clip_algorithm not in (None, 'norm'):
+            raise NotImplementedError(f"gradient_clip_algorithm '{gradient_clip_algorithm}': only 'norm' is built")
+        value = self._optim_settings()["clip"] if gradient_clip_val is None else float(gradient_clip_val)
+        if value == 0.0:
+            return None
+        return clip_grad_norm_([p for group in optimizer.param_groups for p in group["params"]], value)
 
     def train_batch(self, batch, lr: Optional[float] = None, t=None, noise=None):
         """One complete optimisation step on the device: loss + gradients, ONE all-reduce of the flat gradient

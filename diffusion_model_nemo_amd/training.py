@@ -10,8 +10,9 @@ exchange. There is no torch autograd implementation behind this: a missing libra
 """
 import ctypes as C
 import math
-from typing import Dict, Optional
+from typing import Dict, Iterable, Optional, Sequence, Union
 
+import numpy as np
 import torch
 
 from . import _native as N
@@ -225,6 +226,102 @@ class UnetTrainer:
                 self.flat_size, lr, betas[0], betas[1], eps, weight_decay, self.step_count, max_grad_norm, grad_scale,
                 self._scratch.data_ptr(), N.current_stream_handle(self.device)))
         self.unet._weights_version = None   # the sampling handle repacks from the updated parameters
+
+
+def _dense(t: torch.Tensor) -> bool:
+    """Whether `t` covers its memory without gaps or overlaps, in whatever order of its axes."""
+    if t.is_contiguous():
+        return True
+    expect = 1
+    for stride, size in sorted((st, sz) for st, sz in zip(t.stride(), t.shape) if sz != 1):
+        if stride != expect:
+            return False
+        expect *= size
+    return True
+
+
+@torch.no_grad()
+def clip_grad_norm_(parameters: Union[torch.Tensor, Iterable[torch.Tensor]], max_norm: float, norm_type: float = 2.0,
+                    error_if_nonfinite: bool = False, *, grad_scale: float = 1.0,
+                    out: Optional[Sequence[torch.Tensor]] = None) -> torch.Tensor:
+    """Clips the gradients of `parameters` to a global norm, as torch.nn.utils.clip_grad_norm_: with norm = the 2-norm (or,
+    for norm_type inf, the largest magnitude) of ALL their `.grad`s together, every gradient is multiplied by
+    min(1, max_norm / (norm + 1e-6)) in place. Returns the norm as a float32 device scalar; nothing waits for the device
+    unless `error_if_nonfinite` asks for it (then a NaN or infinite norm raises before any gradient is touched).
+
+    `grad_scale` multiplies the gradients first (1 / world_size behind a summing all-reduce, or an inverse loss scale); the
+    norm is that of the scaled ones. `out`: tensors that receive the result in the parameters' place (entry i for parameter
+    i, same shape, contiguous, float32 / bfloat16 / float16), the gradients stay as they are. Gradients may be float32,
+    bfloat16 and float16 side by side and are read and scaled in two launches for up to 192 of them; they must be on one
+    device. A gradient that shares memory with another one is refused: it would be scaled more than once.
+
+    This is the clip for gradients in tensors of their own (the autograd route of `DDPM.training_step`); `UnetTrainer` clips
+    its flat buffer inside `optimizer_step`."""
+    params = [parameters] if isinstance(parameters, torch.Tensor) else list(parameters)
+    norm_type, max_norm, grad_scale = float(norm_type), float(max_norm), float(grad_scale)
+    if norm_type not in (2.0, math.inf):
+        raise NotImplementedError(f"norm_type {norm_type}: only 2 and inf are built")
+    if not max_norm >= 0.0:
+        raise ValueError(f"max_norm must be >= 0, got {max_norm}")
+    if not math.isfinite(grad_scale):
+        raise ValueError(f"grad_scale must be finite, got {grad_scale}")
+    grads = [p.grad for p in params]
+    if out is not None:
+        if len(out) != len(params):
+            raise ValueError(f"out holds {len(out)} tensors for {len(params)} parameters")
+        out = [o for o, g in zip(out, grads) if g is not None]
+    grads = [g for g in grads if g is not None]
+    if not grads:
+        return torch.zeros(())
+    dev = grads[0].device
+    if dev.type != "cuda":
+        raise RuntimeError("clip_grad_norm_ runs only on MI355X device tensors (no CPU implementation)")
+    copied = []   # (gradient, its dense copy): scattered gradients are clipped in a copy and written back
+    for i, g in enumerate(grads):
+        if g.device != dev:
+            raise RuntimeError(f"gradients on {dev} and {g.device}: all must be on one device")
+        if g.layout != torch.strided or g.dtype not in N.DTYPE_CODES:
+            raise ValueError(f"gradients must be dense float32, bfloat16 or float16 tensors, got {g.dtype} ({g.layout})")
+        if not g.is_contiguous() and (out is not None or not _dense(g)):
+            if out is None and any(st == 0 and sz > 1 for st, sz in zip(g.stride(), g.shape)):
+                raise ValueError("a gradient is an expanded tensor: several of its elements are one place in memory")
+            grads[i] = g.contiguous()
+            copied.append((g, grads[i]))
+    table = np.empty((len(grads), 4), dtype=np.int64)   # DmnGradTensor: src, dst, numel, types
+    table[:, 0] = [g.data_ptr() for g in grads]
+    table[:, 2] = [g.numel() for g in grads]
+    table[:, 3] = [N.DTYPE_CODES[g.dtype] for g in grads]
+    if out is None:
+        table[:, 1] = table[:, 0]
+        table[:, 3] *= (1 << 32) + 1
+    else:
+        for o, g in zip(out, grads):
+            if o.device != dev or o.shape != g.shape or o.dtype not in N.DTYPE_CODES or not o.is_contiguous():
+                raise ValueError("out must hold contiguous float32 / bfloat16 / float16 tensors of the gradients' shapes, on "
+                                 "their device")
+        table[:, 1] = [o.data_ptr() for o in out]
+        table[:, 3] += np.array([N.DTYPE_CODES[o.dtype] for o in out], dtype=np.int64) << 32
+    lib = N.lib()
+    nbytes = lib.dmn_clip_grads_workspace_bytes(len(grads))
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+    norm = torch.empty((), dtype=torch.float32, device=dev)
+
+    def call(rows):
+        N.launch(dev, lib.dmn_clip_grads, rows.ctypes.data, len(rows), int(norm_type != 2.0), max_norm, grad_scale,
+                 norm.data_ptr(), ws.data_ptr(), nbytes)
+
+    if error_if_nonfinite:
+        only = table.copy()
+        only[:, 1] = 0
+        call(only)
+        if not bool(torch.isfinite(norm)):
+            raise RuntimeError(f"the total norm of the gradients is non-finite ({float(norm)}); they were not clipped")
+    call(table)
+    if out is None:
+        for g, c in copied:
+            g.copy_(c)
+    torch.autograd.graph.increment_version(grads if out is None else out)
+    return norm
 
 
 def cosine_annealing_lr(step: int, max_steps: int, base_lr: float, min_lr: float, warmup_steps: int = 0) -> float:

@@ -266,6 +266,46 @@ int dmn_adamw_step(float* params, const float* grads, float* exp_avg, float* exp
                    float beta2, float eps, float weight_decay, int step, float max_norm, float grad_scale, float* scratch,
                    void* stream);
 
+/* ---- operators of a trained block ---------------------------------------------------------------------------------
+ * The layers and the gradient clipping that a block of linear layers beside the network needs: what
+ * Residual(PreNorm(fn)) (utils.py:68-93), nn.Linear + GELU (modules/unet.py:55-61) and the trainer's gradient_clip_val are
+ * to the network itself, on tensors of the caller. Tensors are DEVICE memory, rows of contiguous elements `ld` elements
+ * apart; addresses need the alignment of the element type only. Nothing is allocated, nothing waits for the device, and a
+ * call can be recorded into a graph; the device that owns the tensors must be the current one. Two calls that may overlap
+ * in time need workspaces of their own. Sums and statistics are float32 or wider; results are rounded once to the output's
+ * type. The order of every sum is fixed by the sizes: two calls on the same data give the same bits. */
+#define DMN_DT_F32 0
+#define DMN_DT_BF16 1
+#define DMN_DT_F16 2
+
+/* y[r] = (x[r] - mean) * rstd * weight + bias over rows of `width` elements. weight, bias: [width] of affine_dtype (dtype or
+ * DMN_DT_F32), or NULL (1 and 0). y: [rows][width]. stats: optional [rows][2] float32, receives mean and rstd of every row for
+ * the backward. rows may be 0. */
+int dmn_layer_norm_forward(const void* x, int64_t ldx, const void* weight, const void* bias, void* y, float* stats, int64_t rows,
+                           int width, int dtype, int affine_dtype, float eps, void* stream);
+/* dx, dweight, dbias (each optional) from dy, the forward's x, weight and stats. dx: [rows][width] of dtype; dweight, dbias:
+ * [width] of affine_dtype, overwritten (zero for no rows). workspace: needed for dweight / dbias, 16-byte aligned. */
+size_t dmn_layer_norm_workspace_bytes(int64_t rows, int width, int dtype);
+int dmn_layer_norm_backward(const void* dy, int64_t lddy, const void* x, int64_t ldx, const void* weight, const float* stats,
+                            void* dx, void* dweight, void* dbias, int64_t rows, int width, int dtype, int affine_dtype,
+                            void* workspace, size_t workspace_bytes, void* stream);
+
+/* One gradient tensor: numel contiguous elements of src_dtype; dst receives the scaled ones as dst_dtype (dst == src with the
+ * same type: in place; NULL in every tensor: only the norm is computed). */
+typedef struct {
+    const void* src;
+    void* dst;
+    int64_t numel;
+    int src_dtype, dst_dtype;
+} DmnGradTensor;
+/* torch.nn.utils.clip_grad_norm_ over n_tensors tensors (HOST array, read during the call): *norm (device) = grad_scale times
+ * the 2-norm (inf_norm 0) or the largest magnitude (1) of all elements, then dst = src * grad_scale * min(1, max_norm /
+ * (norm + 1e-6)). A NaN or infinity among the gradients reaches the norm, and NaN or zero the gradients, as in torch. A
+ * written range that overlaps another tensor of the call is refused. No elements at all: norm 0. */
+size_t dmn_clip_grads_workspace_bytes(int n_tensors);
+int dmn_clip_grads(const DmnGradTensor* tensors, int n_tensors, int inf_norm, float max_norm, float grad_scale, float* norm,
+                   void* workspace, size_t workspace_bytes, void* stream);
+
 /* N(0,1) * scale into x[B][per] with the library's generator (prior draws; tests). */
 int dmn_fill_normal(float* x, int B, int per, uint64_t seed, uint32_t step, int64_t img_offset, float scale, void* stream);
 

@@ -1,0 +1,420 @@
+"""Layer norm, linear layer and gradient clipping against their formulas in float64, element by element.
+
+Tolerances are bounds, derived per element: half a step of the output's type (eps / 2 of the value) plus the float32 work in
+front of it. A float32 sum of n terms in any order is off by at most (n - 1) u sum |terms| with u = 2^-24; the kernels' sums are
+trees over short runs, so `DEPTH` additions stand for the longest chain a term passes through."""
+import math
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+U = 2.0 ** -24
+BF, HF, F32 = torch.bfloat16, torch.float16, torch.float32
+TYPES = [F32, BF, HF]
+
+
+def half_step(t):
+    """Half a rounding step relative to the value; float16 results below 2^-14 step by 2^-24, bfloat16 and float32 ones below
+    2^-126 by far less than any tolerance here."""
+    return torch.finfo(t).eps / 2
+
+
+def floor_of(t):
+    return 2.0 ** -25 if t == HF else 2.0 ** -149
+
+
+def randn(shape, seed, dtype=F32, scale=1.0, shift=0.0):
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    return (torch.randn(shape, generator=g, device="cuda") * scale + shift).to(dtype)
+
+
+def close(got, want, tol, what):
+    assert got.shape == want.shape, (what, got.shape, want.shape)
+    bad = ~((got.double() - want).abs() <= tol)
+    assert not bool(bad.any()), (what, int(bad.sum()), float(((got.double() - want).abs() / tol).nan_to_num(9e9).max()))
+
+
+# ---- layer norm --------------------------------------------------------------------------------------------------------
+
+def ln_formula(x, w, b, eps, dy=None):
+    x = x.double()
+    n = x.shape[-1]
+    w = torch.ones(n, dtype=torch.float64, device=x.device) if w is None else w.double()
+    b = torch.zeros(n, dtype=torch.float64, device=x.device) if b is None else b.double()
+    mean = x.mean(-1, keepdim=True)
+    rstd = 1 / ((x - mean).square().mean(-1, keepdim=True) + eps).sqrt()
+    xh = (x - mean) * rstd
+    out = {"y": xh * w + b, "xh": xh, "rstd": rstd, "w": w, "b": b}
+    if dy is not None:
+        dy = dy.double()
+        g = dy * w
+        out["dx"] = rstd * (g - g.mean(-1, keepdim=True) - xh * (g * xh).mean(-1, keepdim=True))
+        red = tuple(range(x.dim() - 1))
+        out["dw"], out["db"] = (dy * xh).sum(red), dy.sum(red)
+    return out
+
+
+def ln_bounds(f, x, dy, t, pt):
+    """DEPTH: a thread adds at most 32 elements of a row, then 10 levels of lanes and waves; mean and rstd add a few more."""
+    depth = 64 * U
+    big = x.double().abs().amax(-1, keepdim=True) * f["rstd"]          # what an error of the mean is multiplied by
+    slack = depth * (big + f["xh"].abs() + 1)                          # error of xhat
+    out = {"y": half_step(t) * f["y"].abs() + slack * f["w"].abs() + 4 * U * f["b"].abs() + floor_of(t)}
+    if dy is not None:
+        dy = dy.double().abs()
+        g = dy * f["w"].abs()
+        part = (g * (f["xh"].abs() + slack)).mean(-1, keepdim=True)
+        out["dx"] = (half_step(t) * f["dx"].abs() + floor_of(t)
+                     + f["rstd"] * (depth * (g + g.mean(-1, keepdim=True) + f["xh"].abs() * part + g * f["xh"].abs())
+                                    + slack * part + f["xh"].abs() * (g * slack).mean(-1, keepdim=True)))
+        red = tuple(range(dy.dim() - 1))
+        rows = dy.numel() // dy.shape[-1]
+        chain = (min(rows, 160) + 64) * U                              # rows of one slot, then the partial rows
+        out["dw"] = half_step(pt) * f["dw"].abs() + (dy * (chain * f["xh"].abs() + slack)).sum(red) + floor_of(pt)
+        out["db"] = half_step(pt) * f["db"].abs() + chain * dy.sum(red) + floor_of(pt)
+    return out
+
+
+def check_ln(x, w, b, dy, eps=1e-5):
+    from diffusion_model_nemo_amd.modules import layer_norm
+    t, pt = x.dtype, (w if w is not None else b).dtype if (w is not None or b is not None) else x.dtype
+    f = ln_formula(x, w, b, eps, dy)
+    tol = ln_bounds(f, x, dy, t, pt)
+    with torch.no_grad():
+        y0 = layer_norm(x, w, b, eps)
+    leaves = [v.detach().requires_grad_(True) for v in (x, w, b) if v is not None]
+    it = iter(leaves)
+    args = [next(it) if v is not None else None for v in (x, w, b)]
+    y = layer_norm(*args, eps)
+    assert torch.equal(y, y0) and y.dtype == t and y.is_contiguous()
+    close(y, f["y"], tol["y"], "y")
+    grads = iter(torch.autograd.grad(y, leaves, dy))
+    for name, v in (("dx", x), ("dw", w), ("db", b)):
+        if v is not None:
+            got = next(grads)
+            assert got.dtype == v.dtype
+            close(got, f[name], tol[name], name)
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("width", [1, 2, 7, 8, 63, 64, 65, 100, 128, 250, 256, 511, 512, 1000, 1024, 1111, 2048, 2049, 4096, 4099,
+                                   8192, 8200, 16384, 16387, 33001])
+def test_layer_norm_widths(dtype, width):
+    rows = 37 if width < 5000 else 5
+    x = randn((rows, width), 1, dtype, 1.5, 0.3)
+    check_ln(x, randn((width,), 2, dtype, 0.1, 1.0), randn((width,), 3, dtype, 0.1), randn((rows, width), 4, dtype))
+
+
+@pytest.mark.parametrize("rows", [1, 2, 31, 1025, 5003])
+@pytest.mark.parametrize("width", [24, 130, 768, 4096])
+def test_layer_norm_rows_with_float32_parameters(rows, width):
+    x = randn((rows, width), 5, BF, 2.0, -1.0)
+    check_ln(x, randn((width,), 6, F32, 0.1, 1.0), randn((width,), 7, F32, 0.1), randn((rows, width), 8, BF))
+
+
+def test_layer_norm_without_parameters_and_with_one_of_them():
+    x, dy = randn((9, 200), 1, HF), randn((9, 200), 2, HF)
+    check_ln(x, None, None, dy)
+    check_ln(x, randn((200,), 3, F32, 0.1, 1.0), None, dy)
+    check_ln(x, None, randn((200,), 3, HF), dy)
+
+
+def test_layer_norm_offset_constant_and_extreme_rows():
+    x = randn((8, 1000), 1, F32, 1.0, 1000.0)
+    x[1] = 5.0                       # no variance: xhat = 0
+    x[2] *= 1e-20
+    x[3] = randn((1000,), 2) * 1e15
+    check_ln(x, randn((1000,), 3), randn((1000,), 4), randn((8, 1000), 5))
+
+
+def test_layer_norm_nonfinite_rows_stay_in_their_rows():
+    from diffusion_model_nemo_amd.modules import layer_norm
+    x = randn((6, 130), 1, BF)
+    clean = layer_norm(x)
+    x[1, 3], x[2, 7], x[4, 129] = float("nan"), float("inf"), float("-inf")
+    y = layer_norm(x)
+    for r in range(6):
+        if r in (1, 2, 4):
+            assert bool(torch.isnan(y[r, 3 if r == 1 else 0])), r
+        else:
+            assert torch.equal(y[r], clean[r])
+
+
+def test_layer_norm_strides_shapes_and_expanded_gradients():
+    from diffusion_model_nemo_amd.modules import layer_norm
+    w, b = randn((96,), 1, F32, 0.1, 1.0), randn((96,), 2, F32)
+    big = randn((40, 200), 3, BF)
+    check_ln(big[:, 5:101], w, b, randn((40, 200), 4, BF)[:, 50:146])       # rows 200 apart, no 16-byte boundary
+    check_ln(randn((96, 40), 5, BF).t(), w, b, randn((40, 96), 6, BF))      # transposed: copied
+    check_ln(randn((2, 3, 5, 96), 7, BF), w, b, randn((2, 3, 5, 96), 8, BF))
+    check_ln(randn((96,), 9, BF).expand(7, 96), w, b, randn((7, 96), 10, BF))
+    check_ln(randn((1, 96), 9, BF).expand(7, 96).t()[:, :1].t(), w, b, randn((1, 96), 10, BF))
+    x = randn((4, 96), 11, BF).requires_grad_(True)
+    (g,) = torch.autograd.grad(layer_norm(x, w, b).sum(), x)                # the gradient of a sum is one expanded element
+    f = ln_formula(x.detach(), w, b, 1e-5, torch.ones(4, 96, device="cuda"))
+    close(g, f["dx"], ln_bounds(f, x.detach(), torch.ones(4, 96, device="cuda"), BF, F32)["dx"], "dx")
+
+
+def test_layer_norm_empty_batch():
+    from diffusion_model_nemo_amd.modules import layer_norm
+    x, w, b = (v.requires_grad_(True) for v in (randn((0, 33), 1), randn((33,), 2), randn((33,), 3)))
+    y = layer_norm(x, w, b)
+    dx, dw, db = torch.autograd.grad(y, (x, w, b), torch.empty(0, 33, device="cuda"))
+    assert y.shape == dx.shape == (0, 33) and not dw.any() and not db.any()
+
+
+def test_layer_norm_gradient_agrees_with_differences():
+    from diffusion_model_nemo_amd.modules import layer_norm
+    x, w, b, dy = randn((3, 17), 1), randn((17,), 2), randn((17,), 3), randn((3, 17), 4)
+    leaves = [v.clone().requires_grad_(True) for v in (x, w, b)]
+    grads = torch.autograd.grad(layer_norm(*leaves), leaves, dy)
+    h = 2.0 ** -7
+    for which, (leaf, grad) in enumerate(zip((x, w, b), grads)):
+        v = randn(leaf.shape, 20 + which)
+        ends = []
+        for s in (h, -h):
+            args = [x, w, b]
+            args[which] = leaf + s * v
+            ends.append((layer_norm(*args).double() * dy.double()).sum())
+        slope = float((ends[0] - ends[1]) / (2 * h))
+        want = float((grad.double() * v.double()).sum())
+        # rounding of the two values over the step, and the third derivative's h^2 / 6 (of order one here, times 17 * 3 terms)
+        assert abs(slope - want) <= 64 * U * float(dy.abs().sum()) * 8 / h + h * h * float((dy.abs().sum())) * 8, (which, slope, want)
+
+
+def test_layer_norm_same_bits_again_on_another_stream_and_in_a_graph():
+    from diffusion_model_nemo_amd.modules import layer_norm
+    x, w, b = (v.requires_grad_(True) for v in (randn((300, 520), 1, BF), randn((520,), 2, F32), randn((520,), 3, F32)))
+    dy = randn((300, 520), 4, BF)
+
+    def step():
+        y = layer_norm(x, w, b)
+        return (y.detach(),) + torch.autograd.grad(y, (x, w, b), dy)
+
+    want = step()
+    assert all(torch.equal(p, q) for p, q in zip(step(), want))
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        other = step()
+    side.synchronize()
+    assert all(torch.equal(p, q) for p, q in zip(other, want))
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = step()
+    for turn in range(3):
+        with torch.no_grad():
+            x.copy_(randn((300, 520), 10 + turn, BF))
+        graph.replay()
+        eager = step()
+        torch.cuda.synchronize()
+        assert all(torch.equal(p, q) for p, q in zip(got, eager)), turn
+
+
+# ---- gradient clipping -----------------------------------------------------------------------------------------------------
+
+def params_with(grads):
+    out = []
+    for g in grads:
+        p = torch.nn.Parameter(torch.empty(g.shape, dtype=g.dtype, device=g.device))
+        p.grad = g
+        out.append(p)
+    return out
+
+
+def clip_formula(grads, max_norm, kind, scale=1.0):
+    flat = [g.double().flatten() * scale for g in grads]
+    flat = [f for f in flat if f.numel()]
+    if kind == math.inf:
+        norm = torch.stack([f.abs().max() for f in flat]).max()
+    else:
+        norm = torch.stack([f.square().sum() for f in flat]).sum().sqrt()
+    c = (max_norm / (norm + 1e-6)).clamp(max=1.0)
+    return norm, [g.double() * scale * c for g in grads]
+
+
+SHAPES = [(1,), (3,), (64, 32, 3, 3), (17, 5), (), (0, 4), (8191,), (8193,), (257, 129), (2, 1), (33000,)]
+
+
+@pytest.mark.parametrize("kind", [2.0, math.inf], ids=["two", "inf"])
+@pytest.mark.parametrize("clipped", [False, True], ids=["within", "clipped"])
+@pytest.mark.parametrize("dtypes", [(F32,), (BF,), (HF,), (F32, BF, HF)], ids=["fp32", "bf16", "fp16", "mixed"])
+def test_clip_many_tensors(dtypes, clipped, kind):
+    from diffusion_model_nemo_amd.training import clip_grad_norm_
+    grads = [randn(s, 30 + i, dtypes[i % len(dtypes)], 0.1 * (1 + i % 3)) for i, s in enumerate(SHAPES * 40)]   # 440: several launches
+    norm0, _ = clip_formula(grads, 1.0, kind)
+    limit = float(norm0) * (0.37 if clipped else 3.0)
+    norm, want = clip_formula(grads, limit, kind)
+    params = params_with([g.clone() for g in grads])
+    got = clip_grad_norm_(params, limit, norm_type=kind)
+    # the squares are added in float64; what is left are the norm's own rounding, the limit's and the factor's
+    assert got.shape == () and got.dtype == F32 and abs(float(got) - float(norm)) <= 2 * U * float(norm)
+    for p, g, w in zip(params, grads, want):
+        if not clipped:
+            assert torch.equal(p.grad, g)
+        else:
+            close(p.grad, w, (half_step(g.dtype) + 3 * U) * w.abs() + floor_of(g.dtype), "grad")
+
+
+@pytest.mark.parametrize("to", TYPES, ids=str)
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+def test_clip_into_other_tensors_with_a_scale(dtype, to):
+    from diffusion_model_nemo_amd.training import clip_grad_norm_
+    grads = [randn(s, 50 + i, dtype, 0.2) for i, s in enumerate(SHAPES)]
+    norm, want = clip_formula(grads, 0.9, 2.0, 0.125)
+    before = [g.clone() for g in grads]
+    out = [torch.full(g.shape, float("nan"), dtype=to, device="cuda") for g in grads]
+    got = clip_grad_norm_(params_with(grads), 0.9, grad_scale=0.125, out=out)
+    assert abs(float(got) - float(norm)) <= 2 * U * float(norm)
+    for g, b, o, w in zip(grads, before, out, want):
+        assert torch.equal(g, b)
+        close(o, w, (half_step(to) + 3 * U) * w.abs() + floor_of(to), "out")
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+def test_clip_tightly_packed_views_leave_their_neighbours_alone(dtype):
+    from diffusion_model_nemo_amd.training import clip_grad_norm_
+    flat = randn((60000,), 1, dtype)
+    keep = flat.clone()
+    cuts, at = [], 1
+    for n in (1, 2, 3, 5, 7, 8, 9, 31, 33, 8192, 8193, 16385, 20001):
+        cuts.append((at, at + n))
+        at += n + (n % 2)
+    params = params_with([flat[a:b] for a, b in cuts])
+    norm, want = clip_formula([keep[a:b] for a, b in cuts], 1.0, 2.0)
+    clip_grad_norm_(params, 1.0)
+    mask = torch.ones(60000, dtype=torch.bool, device="cuda")
+    for (a, b), w in zip(cuts, want):
+        close(flat[a:b], w, (half_step(dtype) + 3 * U) * w.abs() + floor_of(dtype), (a, b))
+        mask[a:b] = False
+    assert torch.equal(flat[mask], keep[mask])
+
+
+def test_clip_extreme_values_and_nonfinite_gradients():
+    from diffusion_model_nemo_amd.training import clip_grad_norm_
+    big = params_with([torch.full((1000,), 1e30, device="cuda"), torch.full((10,), 1e-30, device="cuda")])
+    assert abs(float(clip_grad_norm_(big, math.inf)) / (1e30 * math.sqrt(1000)) - 1) < 1e-6     # squares overflow float32
+    small = params_with([torch.full((100,), 1e-30, device="cuda")])
+    assert abs(float(clip_grad_norm_(small, 1.0)) / 1e-29 - 1) < 1e-6                             # ... and underflow it
+    for bad, kind in ((float("nan"), 2.0), (float("nan"), math.inf), (float("inf"), 2.0), (float("-inf"), math.inf)):
+        for at in (0, 4999, 9999):
+            g = randn((10000,), 3)
+            g[at] = bad
+            params = params_with([randn((5,), 4), g])
+            first = params[0].grad.clone()
+            with pytest.raises(RuntimeError, match="non-finite"):
+                clip_grad_norm_(params, 1.0, norm_type=kind, error_if_nonfinite=True)
+            assert torch.equal(params[0].grad, first)
+            n = clip_grad_norm_(params, 1.0, norm_type=kind)
+            assert math.isnan(float(n)) if math.isnan(bad) else float(n) == math.inf
+            # as in torch: a NaN norm makes every gradient NaN, an infinite one makes finite gradients zero
+            assert bool(torch.isnan(params[0].grad).all()) if math.isnan(bad) else not bool(params[0].grad.any())
+            assert bool(torch.isnan(params[1].grad[at]))
+
+
+def test_clip_scattered_and_reordered_gradients():
+    from diffusion_model_nemo_amd.training import clip_grad_norm_
+    base = randn((40, 60), 1)
+    keep = base.clone()
+    perm = randn((4, 6, 5, 7), 2).to(memory_format=torch.channels_last)
+    pk = perm.clone()
+    norm, want = clip_formula([keep[:, 3:50], pk, keep[:, 55:].t()], 1.0, 2.0)
+    got = clip_grad_norm_(params_with([base[:, 3:50], perm, base[:, 55:].t()]), 1.0)
+    assert abs(float(got) - float(norm)) <= 2 * U * float(norm)
+    for g, w in zip((base[:, 3:50], perm, base[:, 55:].t()), want):
+        close(g, w, (half_step(F32) + 3 * U) * w.abs() + 1e-40, "grad")
+    assert torch.equal(base[:, :3], keep[:, :3]) and torch.equal(base[:, 50:55], keep[:, 50:55])
+
+
+def test_clip_skips_parameters_without_gradients_and_handles_none_at_all():
+    from diffusion_model_nemo_amd.training import clip_grad_norm_
+    p = params_with([randn((10,), 1), randn((20,), 2)])
+    p[0].grad = None
+    want = float(p[1].grad.double().norm())
+    assert abs(float(clip_grad_norm_(p, 1e9)) - want) <= 2 * U * want
+    out = [torch.full((10,), 7.0, device="cuda"), torch.zeros(20, device="cuda")]
+    clip_grad_norm_(p, 1e9, out=out)
+    assert torch.equal(out[1], p[1].grad) and bool((out[0] == 7).all())
+    assert float(clip_grad_norm_([], 1.0)) == 0.0
+    assert float(clip_grad_norm_(params_with([torch.zeros((0, 3), device="cuda")]), 1.0)) == 0.0
+    single = params_with([randn((64,), 3)])[0]
+    assert abs(float(clip_grad_norm_(single, 1e9)) - float(single.grad.double().norm())) <= 1e-5
+
+
+def test_clip_refuses_overlaps_and_bad_arguments():
+    from diffusion_model_nemo_amd._native import DmnError
+    from diffusion_model_nemo_amd.training import clip_grad_norm_
+    g = randn((100,), 1)
+    keep = g.clone()
+    for grads in ([g, g], [g[:60], g[59:]], [g[10:20], g]):
+        with pytest.raises(DmnError, match="overlaps"):
+            clip_grad_norm_(params_with(grads), 1.0)
+    out = torch.zeros(100, device="cuda")
+    with pytest.raises(DmnError, match="overlaps"):
+        clip_grad_norm_(params_with([g, g]), 1.0, out=[out, out])
+    with pytest.raises(DmnError, match="overlaps"):
+        clip_grad_norm_(params_with([g[:50]]), 1.0, out=[g[1:51]])
+    with pytest.raises(ValueError):
+        clip_grad_norm_(params_with([torch.ones(1, device="cuda").expand(5)]), 1.0)
+    with pytest.raises(ValueError):
+        clip_grad_norm_(params_with([g]), -1.0)
+    with pytest.raises(ValueError):
+        clip_grad_norm_(params_with([g]), 1.0, out=[])
+    with pytest.raises(ValueError):
+        clip_grad_norm_(params_with([g]), 1.0, out=[torch.zeros(99, device="cuda")])
+    with pytest.raises(ValueError):
+        clip_grad_norm_(params_with([g.double()]), 1.0)
+    with pytest.raises(NotImplementedError):
+        clip_grad_norm_(params_with([g]), 1.0, norm_type=1.0)
+    assert torch.equal(g, keep)
+    # the same gradient may be READ twice
+    a, b = torch.zeros(100, device="cuda"), torch.zeros(100, device="cuda")
+    n = clip_grad_norm_(params_with([g, g]), 1e9, out=[a, b])
+    assert torch.equal(a, g) and torch.equal(b, g) and abs(float(n) - math.sqrt(2) * float(g.double().norm())) < 1e-4
+
+
+def test_clip_in_a_graph_and_repeated():
+    from diffusion_model_nemo_amd.training import clip_grad_norm_
+    grads = [randn((n,), n, BF) for n in (5, 4096, 20000, 33)]
+    out = [torch.zeros_like(g, dtype=F32) for g in grads]
+    params = params_with(grads)
+    clip_grad_norm_(params, 1.0, out=out)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        norm = clip_grad_norm_(params, 1.0, out=out)
+    for turn in range(3):
+        for i, g in enumerate(grads):
+            g.copy_(randn(g.shape, 100 * turn + i, BF))
+        graph.replay()
+        got = [norm.clone()] + [o.clone() for o in out]
+        eager = [torch.zeros_like(o) for o in out]
+        n2 = clip_grad_norm_(params, 1.0, out=eager)
+        torch.cuda.synchronize()
+        assert torch.equal(n2, got[0]) and all(torch.equal(p, q) for p, q in zip(eager, got[1:]))
+
+
+def test_clip_on_the_autograd_route_of_the_denoising_network():
+    from diffusion_model_nemo_amd.models import DDPM
+    cfg = {"image_size": 32, "timesteps": 10, "channels": 3,
+           "diffusion_model": {"_target_": "diffusion_model_nemo.modules.Unet", "input_dim": 32, "dim": 32,
+                               "use_convnext": False, "dropout": 0.0, "compute_dtype": "fp32"},
+           "sampler": {"_target_": "diffusion_model_nemo.modules.GaussianDiffusion", "timesteps": 10, "schedule_name": "linear"},
+           "loss": {"_target_": "diffusion_model_nemo.loss.DiffusionLoss", "loss_type": "l2", "reduction": "mean"},
+           "optim": {"name": "adamw"}}
+    torch.manual_seed(0)
+    m = DDPM(cfg, trainer={"gradient_clip_val": 0.05}).cuda()
+    opt = torch.optim.SGD(m.parameters(), lr=1e-3)
+    loss = m.training_step({"pixel_values": randn((2, 3, 32, 32), 1)}, t=torch.tensor([1, 7], device="cuda"), noise=randn((2, 3, 32, 32), 2))
+    loss.backward()
+    grads = [p.grad.clone() for p in m.parameters()]
+    norm, want = clip_formula(grads, 0.05, 2.0)
+    assert float(norm) > 0.05
+    got = m.configure_gradient_clipping(opt)
+    assert abs(float(got) - float(norm)) <= 2 * U * float(norm)
+    for p, w in zip(m.parameters(), want):
+        close(p.grad, w, 4 * U * w.abs() + 1e-40, "grad")
+    assert m.configure_gradient_clipping(opt, gradient_clip_val=0.0) is None
+    with pytest.raises(NotImplementedError):
+        m.configure_gradient_clipping(opt, gradient_clip_algorithm="value")
