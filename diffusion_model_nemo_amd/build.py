@@ -14,7 +14,7 @@ CSRC = os.path.join(HERE, "csrc")
 LIB_DIR = os.path.join(HERE, "lib")
 LIB_PATH = os.path.join(LIB_DIR, "libdmn_hip.so")
 SOURCES = ["dmn_conv.hip", "dmn_elem.hip", "dmn_attn.hip", "dmn_linattn.hip", "dmn_sampler.hip", "dmn_unet.cpp", "dmn_api.cpp",
-           "dmn_train_gemm.hip", "dmn_train_ops.hip", "dmn_train.cpp", "dmn_peaks.hip", "dmn_layernorm.hip", "dmn_clip.hip"]
+           "dmn_train_gemm.hip", "dmn_train_ops.hip", "dmn_train.cpp", "dmn_peaks.hip", "dmn_layernorm.hip", "dmn_clip.hip", "dmn_linear.hip"]
 ARCH = "gfx950"
 BLOCK_FLAGS = ["-fhonor-nans", "-ffp-contract=fast"]
 
@@ -54,7 +54,7 @@ def build(force: bool = False, verbose: bool = False) -> str:
              "dmn_train_gemm.hip": ["-munsafe-fp-atomics"], "dmn_train_ops.hip": ["-munsafe-fp-atomics"],
              # operators on a caller's tensors: a NaN or infinity in them has to come out as one (the clip's norm, a maximum);
              # multiply-add pairs may be fused (no reference bits to keep)
-             "dmn_layernorm.hip": BLOCK_FLAGS, "dmn_clip.hip": BLOCK_FLAGS}
+             "dmn_layernorm.hip": BLOCK_FLAGS, "dmn_clip.hip": BLOCK_FLAGS, "dmn_linear.hip": BLOCK_FLAGS}
     jobs = []
     objs = []
     for src in SOURCES:

@@ -134,3 +134,104 @@ class LayerNorm(nn.Module):
         if x.shape[-1] != self.dim:
             raise ValueError(f"expected a last axis of {self.dim}, got {tuple(x.shape)}")
         return layer_norm(x, self.weight, self.bias, self.eps)
+
+
+# ---- linear layer ------------------------------------------------------------------------------------------------------
+
+ACTIVATIONS = {None: 0, "relu": 1, "silu": 2, "gelu": 3}
+
+
+def _workspace(nbytes: int, device) -> Optional[torch.Tensor]:
+    return torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
+
+
+def _linear_forward(x, ldx, weight, bias, residual, ldr, code, want_z):
+    out, width = weight.shape
+    rows = x.numel() // width
+    y = torch.empty(x.shape[:-1] + (out,), dtype=x.dtype, device=x.device)
+    z = torch.empty((rows, out), dtype=x.dtype, device=x.device) if want_z else None
+    lib, dt = N.lib(), N.DTYPE_CODES[x.dtype]
+    nbytes = lib.dmn_linear_forward_workspace_bytes(rows, width, out, dt)
+    ws = _workspace(nbytes, x.device)
+    N.launch(x.device, lib.dmn_linear_forward, x.data_ptr(), ldx, weight.data_ptr(), N.ptr(bias), N.ptr(residual), ldr, y.data_ptr(),
+             N.ptr(z), rows, width, out, code, dt, N.ptr(ws), nbytes)
+    return y, z
+
+
+class _LinearFunction(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, bias, residual, code):
+        x, ldx = _rows(x)
+        ldr = 0
+        if residual is not None:
+            residual, ldr = _rows(residual)
+        # the value in front of the activation is all the backward needs of the forward's results
+        y, z = _linear_forward(x, ldx, weight, bias, residual, ldr, code, code != 0 and any(ctx.needs_input_grad[:3]))
+        ctx.save_for_backward(x, weight, z)
+        ctx.ldx, ctx.code = ldx, code
+        return y
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy):
+        x, weight, z = ctx.saved_tensors
+        need_x, need_w, need_b, need_r = ctx.needs_input_grad[:4]
+        dx = dw = db = None
+        if need_x or need_w or need_b:
+            rows_dy, lddy = _rows(dy)
+            out, width = weight.shape
+            rows = x.numel() // width
+            dx = torch.empty(x.shape, dtype=x.dtype, device=x.device) if need_x else None
+            dw = torch.empty((out, width), dtype=x.dtype, device=x.device) if need_w else None
+            db = torch.empty(out, dtype=x.dtype, device=x.device) if need_b else None
+            lib, dt = N.lib(), N.DTYPE_CODES[x.dtype]
+            nbytes = lib.dmn_linear_backward_workspace_bytes(rows, width, out, ctx.code, dt)
+            ws = _workspace(nbytes, x.device)
+            N.launch(x.device, lib.dmn_linear_backward, rows_dy.data_ptr(), lddy, x.data_ptr(), ctx.ldx, weight.data_ptr(), N.ptr(z),
+                     N.ptr(dx), N.ptr(dw), N.ptr(db), rows, width, out, ctx.code, dt, N.ptr(ws), nbytes)
+        return dx, dw, db, dy if need_r else None, None
+
+
+def linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] = None, activation: Optional[str] = None,
+           residual: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """act(x weight^T + bias) + residual in one pass: `x` [..., in], `weight` [out, in], `bias` [out], `residual` [..., out],
+    all of one type (float32, bfloat16 or float16); `activation` None, 'relu', 'silu' or 'gelu' (the exact one). The sum in
+    front of the activation, the activation and the residual are formed in float32 and rounded once. For the backward with
+    an activation the value in front of it is kept, rounded to the type; rows with any stride are read in place for 2-D
+    tensors, other layouts are copied first."""
+    _check_tensor(x, "linear")
+    if weight.dim() != 2 or weight.shape[0] == 0 or weight.shape[1] == 0:
+        raise ValueError(f"weight must be [out, in], got {tuple(weight.shape)}")
+    out, width = weight.shape
+    if x.dim() == 0 or x.shape[-1] != width:
+        raise ValueError(f"expected a last axis of {width}, got {tuple(x.shape)}")
+    if activation not in ACTIVATIONS:
+        raise ValueError(f"activation must be one of {list(ACTIVATIONS)}, got {activation!r}")
+    _check_param(weight, "weight", (out, width), x, (x.dtype,))
+    _check_param(bias, "bias", (out,), x, (x.dtype,))
+    _check_param(residual, "residual", x.shape[:-1] + (out,), x, (x.dtype,))
+    weight = weight.contiguous()
+    bias = bias if bias is None else bias.contiguous()
+    code = ACTIVATIONS[activation]
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, bias, residual)):
+        return _LinearFunction.apply(x, weight, bias, residual, code)
+    x, ldx = _rows(x)
+    ldr = 0
+    if residual is not None:
+        residual, ldr = _rows(residual)
+    return _linear_forward(x, ldx, weight, bias, residual, ldr, code, False)[0]
+
+
+class Linear(nn.Linear):
+    """torch.nn.Linear (its parameters, initialisation and state_dict) with an activation and a residual in its epilogue:
+    `Linear(in, out, activation='gelu')(x)`, `Linear(in, out)(x, residual=x0)`."""
+
+    def __init__(self, in_features: int, out_features: int, bias: bool = True, activation: Optional[str] = None, device=None,
+                 dtype=None):
+        if activation not in ACTIVATIONS:
+            raise ValueError(f"activation must be one of {list(ACTIVATIONS)}, got {activation!r}")
+        super().__init__(in_features, out_features, bias, device=device, dtype=dtype)
+        self.activation = activation
+
+    def forward(self, x: torch.Tensor, residual: Optional[torch.Tensor] = None) -> torch.Tensor:
+        return linear(x, self.weight, self.bias, self.activation, residual)

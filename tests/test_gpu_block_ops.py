@@ -213,6 +213,258 @@ def test_layer_norm_same_bits_again_on_another_stream_and_in_a_graph():
         assert all(torch.equal(p, q) for p, q in zip(got, eager)), turn
 
 
+# ---- linear layer ------------------------------------------------------------------------------------------------------
+
+def act_formula(z, kind):
+    if kind == "relu":
+        return z.clamp(min=0), (z > 0).double()
+    if kind == "silu":
+        s = torch.sigmoid(z)
+        return z * s, s * (1 + z * (1 - s))
+    if kind == "gelu":
+        cdf = 0.5 * torch.erfc(-z / math.sqrt(2))
+        return z * cdf, cdf + z * torch.exp(-z * z / 2) / math.sqrt(2 * math.pi)
+    return z, torch.ones_like(z)
+
+
+def product(a, b):
+    """a b and |a| |b| in float64 (operands laid out plainly)."""
+    a, b = a.double().contiguous(), b.double().contiguous()
+    return a @ b, a.abs() @ b.abs()
+
+
+def check_linear(x, w, b, r, kind, dy=None):
+    """Bounds: a float32 sum of k products is off by at most (k + splits) u sum |products| in any order; the matrix cores add
+    k one after the other within a split, so k u is the bound that holds for every split. The activations' slopes are at most
+    1.13 and their curvature at most 1.2; `1.2e-6` is the relative error of the float32 / 16-bit tail fits with the hardware
+    exponential and reciprocal (an argument of exp up to 14 in size is off by 14 u, each function by an ulp)."""
+    from diffusion_model_nemo_amd.modules import linear
+    t = x.dtype
+    x2, k, n = x.reshape(-1, x.shape[-1]), x.shape[-1], w.shape[0]
+    z, za = product(x2, w.t())
+    ez = (k + 64) * U * za
+    if b is not None:
+        z = z + b.double()
+        ez = ez + 4 * U * (z.abs() + b.double().abs())
+    a, slope = act_formula(z, kind)
+    want = a + (0 if r is None else r.reshape(-1, n).double())
+    tol = half_step(t) * want.abs() + 1.13 * ez + 2.4e-6 * a.abs() + 4 * U * (a.abs() + want.abs()) + floor_of(t)
+    with torch.no_grad():
+        y0 = linear(x, w, b, kind, r)
+    assert y0.dtype == t and y0.is_contiguous() and y0.shape == x.shape[:-1] + (n,)
+    close(y0.reshape(-1, n), want, tol, "y")
+    if dy is None:
+        return
+    names = [("x", x), ("w", w), ("b", b), ("r", r)]
+    leaves = {m: v.detach().requires_grad_(True) for m, v in names if v is not None}
+    y = linear(leaves["x"], leaves["w"], leaves.get("b"), kind, leaves.get("r"))
+    assert torch.equal(y, y0)
+    got = dict(zip(leaves, torch.autograd.grad(y, list(leaves.values()), dy)))
+    d2 = dy.reshape(-1, n).double()
+    dz = d2 * slope
+    # z is kept rounded (half a step of z times the slope's own slope), the sums are off by ez, dz is rounded for the products
+    edz = torch.zeros_like(dz)
+    if kind is not None:
+        edz = d2.abs() * (1.2 * (half_step(t) * z.abs() + ez + floor_of(t)) + 4e-6 + 4 * U)
+        if kind == "relu":   # the slope jumps at 0: only values whose sign is in doubt can change, and they by all of dy
+            edz = torch.where(z.abs() <= ez + floor_of(t), d2.abs(), torch.zeros_like(dz))
+    edz_op = edz + (half_step(t) * (dz.abs() + edz) + floor_of(t) if kind is not None else 0)
+    rows = d2.shape[0]
+    for name, (want, size), err, depth in (
+            ("x", product(dz, w), edz_op @ w.double().abs(), n),
+            ("w", product(dz.t(), x2), edz_op.t().contiguous() @ x2.double().abs(), rows)):
+        size = size + err
+        g = got[name].reshape(want.shape)
+        assert got[name].dtype == t
+        close(g, want, half_step(t) * want.abs() + err + (depth + 64) * U * size + floor_of(t), "d" + name)
+    if b is not None:
+        want = dz.sum(0)
+        close(got["b"], want, half_step(t) * want.abs() + edz.sum(0) + (rows + 64) * U * (dz.abs() + edz).sum(0) + floor_of(t), "db")
+    if r is not None:
+        assert torch.equal(got["r"], dy)
+
+
+def linear_case(m, k, n, dtype, kind, bias, res, train=True, seed=0):
+    x, w = randn((m, k), seed + 1, dtype), randn((n, k), seed + 2, dtype, k ** -0.5)
+    b = randn((n,), seed + 3, dtype, 0.3) if bias else None
+    r = randn((m, n), seed + 4, dtype) if res else None
+    check_linear(x, w, b, r, kind, randn((m, n), seed + 5, dtype) if train else None)
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("m,k,n", [(1, 1, 1), (1, 8, 8), (2, 3, 5), (1, 64, 64), (16, 32, 16), (17, 40, 24), (64, 64, 64), (65, 72, 80),
+                                   (63, 65, 61), (128, 128, 128), (129, 136, 144), (130, 127, 131), (200, 512, 96), (31, 1000, 153),
+                                   (5, 2056, 33), (300, 24, 520), (1000, 8, 7), (257, 260, 4)])
+def test_linear_sizes(dtype, m, k, n):
+    linear_case(m, k, n, dtype, "gelu", True, True)
+    linear_case(m, k, n, dtype, None, True, False, seed=10)
+
+
+@pytest.mark.parametrize("kind", [None, "relu", "silu", "gelu"])
+@pytest.mark.parametrize("bias,res", [(False, False), (True, False), (False, True), (True, True)])
+def test_linear_epilogues(kind, bias, res):
+    for dtype in TYPES:
+        linear_case(70, 96, 104, dtype, kind, bias, res)
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("m", [1, 2, 3, 4, 7, 8, 15, 16, 17, 31, 32, 33, 48, 63, 64, 65])
+def test_linear_few_rows(dtype, m):
+    linear_case(m, 1024, 272, dtype, "silu", True, True, train=False)
+    linear_case(m, 999, 77, dtype, "gelu", True, False, train=False, seed=20)
+
+
+@pytest.mark.parametrize("m,k,n", [(2048, 2048, 2048), (1555, 1032, 2056), (4001, 520, 264), (64, 8192, 128), (256, 4096, 256)])
+def test_linear_large_and_split_products(m, k, n):
+    linear_case(m, k, n, BF, "gelu", True, True)
+    linear_case(m, k, n, HF, None, True, False, seed=30)
+
+
+def test_linear_float32_large():
+    linear_case(1555, 1032, 520, F32, "silu", True, True)
+    linear_case(4096, 64, 256, F32, "gelu", True, False)
+    linear_case(100, 3, 4096, F32, None, False, False)
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+def test_linear_strides_and_shapes(dtype):
+    w, b = randn((80, 72), 1, dtype, 0.1), randn((80,), 2, dtype)
+    big, rbig = randn((50, 200), 3, dtype), randn((50, 120), 4, dtype)
+    dy = randn((50, 200), 5, dtype)
+    check_linear(big[:, 8:80], w, b, rbig[:, 40:], "gelu", dy[:, 16:96])     # rows apart, on 16-byte boundaries
+    check_linear(big[:, 3:75], w, b, rbig[:, 39:119], "gelu", dy[:, 5:85])   # ... and off them
+    check_linear(randn((72, 50), 6, dtype).t(), w, b, None, None, randn((80, 50), 7, dtype).t())
+    check_linear(randn((2, 5, 3, 72), 8, dtype), w, b, randn((2, 5, 3, 80), 9, dtype), "silu", randn((2, 5, 3, 80), 10, dtype))
+    check_linear(randn((72,), 11, dtype), w, b, None, "relu", randn((80,), 12, dtype))
+    check_linear(randn((72,), 11, dtype).expand(9, 72), w.t().contiguous().t(), b, None, None, randn((1,), 12, dtype).expand(9, 80))
+
+
+def test_linear_activation_tails_and_nonfinite_rows():
+    from diffusion_model_nemo_amd.modules import linear
+    one = torch.ones(1, 1, device="cuda")
+    z = torch.cat([torch.linspace(-14, 14, 4001), torch.tensor([0.0, -0.0, 50.0, -50.0, 100.0, -100.0, 1e-30, -1e-30])]).cuda().view(-1, 1)
+    for kind in ("relu", "silu", "gelu"):
+        y = linear(z, one, activation=kind)
+        want, slope = act_formula(z.double(), kind)
+        # exp's argument z^2 / 2 is rounded (98 u at 14), everything else by a few ulps
+        close(y, want, 1e-5 * want.abs() + 1e-37, kind)
+        x = z.clone().requires_grad_(True)
+        (g,) = torch.autograd.grad(linear(x, one, activation=kind), x, torch.ones_like(z))
+        close(g, slope, 1e-5 * slope.abs() + 4e-6 * torch.exp(-z.double().square() / 4) + 1e-30, "slope of " + kind)
+    for dtype in TYPES:
+        x, w = randn((40, 64), 1, dtype), randn((48, 64), 2, dtype)
+        clean = linear(x, w, activation="gelu")
+        x[3, 5], x[20, 63], x[39, 0] = float("nan"), float("inf"), float("-inf")
+        y = linear(x, w, activation="gelu")
+        assert bool(torch.isnan(y[3]).all()) and not bool(torch.isfinite(y[20]).all()) and not bool(torch.isfinite(y[39]).all())
+        rest = [i for i in range(40) if i not in (3, 20, 39)]
+        assert torch.equal(y[rest], clean[rest])
+        assert bool(torch.isnan(linear(x, w, activation="relu")[3]).all())
+
+
+def test_linear_empty_batch():
+    from diffusion_model_nemo_amd.modules import linear
+    for kind in (None, "gelu"):
+        x, w, b = (v.requires_grad_(True) for v in (randn((0, 24), 1, BF), randn((16, 24), 2, BF), randn((16,), 3, BF)))
+        y = linear(x, w, b, kind)
+        dx, dw, db = torch.autograd.grad(y, (x, w, b), torch.empty((0, 16), dtype=BF, device="cuda"))
+        assert y.shape == (0, 16) and dx.shape == (0, 24) and not dw.any() and not db.any()
+
+
+def test_linear_refusals():
+    from diffusion_model_nemo_amd.modules import Linear, linear
+    x, w = randn((4, 8), 1), randn((6, 8), 2)
+    for args in ((x, randn((6, 7), 3)), (x, w, randn((5,), 3)), (x, w.bfloat16()), (x, w, None, "tanh"),
+                 (x, w, None, None, randn((4, 5), 3)), (x, w, None, None, randn((6,), 3)), (x.double(), w.double()),
+                 (x, randn((0, 8), 3)), (x, randn((8,), 3))):
+        with pytest.raises(ValueError):
+            linear(*args)
+    with pytest.raises(RuntimeError):
+        linear(x, w.cpu())
+    with pytest.raises(ValueError):
+        Linear(8, 6, activation="tanh")
+    p = x.clone().requires_grad_(True)
+    (g,) = torch.autograd.grad(linear(p, w, activation="silu").sum(), p, create_graph=True)
+    with pytest.raises(RuntimeError):
+        g.sum().backward()          # the backward pass is not differentiable
+
+
+@pytest.mark.parametrize("kind", [None, "silu", "gelu"])
+def test_linear_gradient_agrees_with_differences(kind):
+    from diffusion_model_nemo_amd.modules import linear
+    parts = {"x": randn((5, 12), 1), "w": randn((9, 12), 2, scale=0.3), "b": randn((9,), 3), "r": randn((5, 9), 4)}
+    dy = randn((5, 9), 5)
+    leaves = {k: v.clone().requires_grad_(True) for k, v in parts.items()}
+    y = linear(leaves["x"], leaves["w"], leaves["b"], kind, leaves["r"])
+    grads = dict(zip(leaves, torch.autograd.grad(y, list(leaves.values()), dy)))
+    h = 2.0 ** -7
+    for i, (name, v) in enumerate(parts.items()):
+        way = randn(v.shape, 20 + i)
+        way /= way.abs().max()
+        ends = []
+        for s in (h, -h):
+            p = dict(parts)
+            p[name] = v + s * way
+            ends.append((linear(p["x"], p["w"], p["b"], kind, p["r"]).double() * dy.double()).sum())
+        slope, want = float((ends[0] - ends[1]) / (2 * h)), float((grads[name].double() * way.double()).sum())
+        # the values' rounding over the step; the third derivative (at most 2.4) times h^2 / 6 times the inputs' sizes cubed
+        reach = float((parts["x"].abs().sum(1).max() + 1) ** 3 * dy.abs().sum())
+        assert abs(slope - want) <= 64 * U * 20 * float(dy.abs().sum()) / h + 0.4 * h * h * reach, (name, slope, want)
+
+
+# ---- the operators together -----------------------------------------------------------------------------------------------
+
+def test_block_trains_with_clipping_in_eager_mode_and_in_a_graph():
+    """x + W2 gelu(W1 norm(x) + b1) + b2, its gradients against float64 autograd, clipped together; then the same step recorded
+    and replayed on new inputs."""
+    from diffusion_model_nemo_amd.modules import LayerNorm, Linear
+    from diffusion_model_nemo_amd.training import clip_grad_norm_
+    torch.manual_seed(0)
+    norm, up, down = LayerNorm(136).cuda(), Linear(136, 544, activation="gelu").cuda(), Linear(544, 136).cuda()
+    params = [p for m in (norm, up, down) for p in m.parameters()]
+    x, dy = randn((203, 136), 1), randn((203, 136), 2)
+    out = [torch.zeros_like(p) for p in params]
+
+    def step():
+        for p in params:
+            p.grad = None
+        y = down(up(norm(x)), residual=x)
+        for p, g in zip(params, torch.autograd.grad(y, params, dy)):
+            p.grad = g
+        return y.detach(), clip_grad_norm_(params, 5.0, out=out)
+
+    y, total = step()
+    ref = [p.detach().double().requires_grad_(True) for p in params]
+    n, w1, b1, w2, b2 = None, ref[2], ref[3], ref[4], ref[5]
+    n = torch.nn.functional.layer_norm(x.double(), (136,), ref[0], ref[1])
+    want_y = torch.nn.functional.gelu(n @ w1.t() + b1) @ w2.t() + b2 + x.double()
+    grads, want_y = torch.autograd.grad(want_y, ref, dy.double()), want_y.detach()
+    want_total, want = clip_formula(grads, 5.0, 2.0)
+    # float32 sums of up to 544 products and 203 rows: a few hundred u of values of order one to ten
+    assert float((y.double() - want_y).abs().max()) <= 1000 * U * 8
+    assert float(want_total) > 5.0 and abs(float(total) - float(want_total)) <= 1000 * U * float(want_total)
+    for o, w in zip(out, want):
+        assert float((o.double() - w).abs().max()) <= 1000 * U * float(w.abs().max() + 1)
+    for p in params:
+        p.grad = None
+    del y, total
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = step()
+    for turn in range(3):
+        x.copy_(randn((203, 136), 40 + turn))
+        graph.replay()
+        kept = [got[0].clone(), got[1].clone()] + [o.clone() for o in out]
+        eager = step()
+        torch.cuda.synchronize()
+        assert all(torch.equal(p, q) for p, q in zip([eager[0], eager[1]] + out, kept)), turn
+
+
 # ---- gradient clipping -----------------------------------------------------------------------------------------------------
 
 def params_with(grads):
