@@ -50,10 +50,16 @@ template <typename T> __device__ __forceinline__ float normal_cdf(float z, float
     const float tail = normal_tail_scaled<T>(fabsf(z)) * e;
     return z < 0.f ? tail : 1.0f - tail;
 }
+// z Phi(z) as max(z, 0) - |z| Phi(-|z|): no cancellation, a NaN stays (through exp), and infinities give their limits (the
+// factor |z| is held at 40, where Phi(-|z|) is zero in float32).
+template <typename T> __device__ __forceinline__ float gelu(float z) {
+    const float az = fminf(fabsf(z), 40.f), e = __expf(-0.5f * z * z);
+    return __builtin_fmaf(-az, normal_tail_scaled<T>(az) * e, fmaxf(z, 0.f));
+}
 template <typename T> __device__ __forceinline__ float activate(float z, int act) {
     if (act == ACT_RELU) return z < 0.f ? 0.f : z;   // a NaN stays
     if (act == ACT_SILU) return z * __builtin_amdgcn_rcpf(1.0f + __expf(-z));
-    if (act == ACT_GELU) return z * normal_cdf<T>(z, __expf(-0.5f * z * z));
+    if (act == ACT_GELU) return gelu<T>(z);
     return z;
 }
 template <typename T> __device__ __forceinline__ float act_backward(float dy, float z, int act) {
@@ -90,7 +96,7 @@ struct GemmArgs {
 template <typename T> struct Frag;
 template <> struct Frag<float> {
     typedef f32x4 type;
-    static constexpr int KSTEP = 16;
+    static constexpr int KSTEP = 16, MMAS = 4;
     static __device__ __forceinline__ void mma(const type& p, const type& q, f32x4& c) {
 #pragma unroll
         for (int s = 0; s < 4; ++s) c = __builtin_amdgcn_mfma_f32_16x16x4f32(p[s], q[s], c, 0, 0, 0);
@@ -98,29 +104,31 @@ template <> struct Frag<float> {
 };
 template <> struct Frag<__bf16> {
     typedef bf16x8 type;
-    static constexpr int KSTEP = 32;
+    static constexpr int KSTEP = 32, MMAS = 1;
     static __device__ __forceinline__ void mma(const type& p, const type& q, f32x4& c) { c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(p, q, c, 0, 0, 0); }
 };
 template <> struct Frag<f16> {
     typedef f16x8 type;
-    static constexpr int KSTEP = 32;
+    static constexpr int KSTEP = 32, MMAS = 1;
     static __device__ __forceinline__ void mma(const type& p, const type& q, f32x4& c) { c = __builtin_amdgcn_mfma_f32_16x16x32_f16(p, q, c, 0, 0, 0); }
 };
 
-// One operand's tile in LDS: R rows of m (or n) by 128 bytes of k, R * 8 chunks of 16 bytes.
-//   K tile: chunk (row, c): 8 chunks per row, stored at row * 8 + (c ^ (row / 2 % 8)): the 16 rows a fragment read touches
-//           at one k cover all 64 banks once.
-//   X tile: chunk (k, c): R / E chunks per k row, stored at k * (R / E) + (c ^ swz(k)): the k rows that one read touches
+// One operand's tile in LDS: R rows of m (or n) by KB bytes of k, in chunks of 16 bytes.
+//   K tile: chunk (row, c): KB / 16 chunks per row, stored at row * (KB / 16) + (c ^ swizzle(row)). A fragment read is
+//           served 16 lanes at a time, in the groups {0-3, 12-15, 20-23, 24-27}, {4-11, 16-19, 28-31} and these + 32
+//           (found from the counted bank conflicts of four layouts): the swizzles make each group cover all 64 banks once.
+//   X tile: chunk (k, c): R / E chunks per k row, stored at k * (R / E) + (c ^ swizzle(k)): the k rows that one read touches
 //           lie in different banks.
-template <typename T, bool X, int R> struct Tile {
+template <typename T, bool X, int R, int KB> struct Tile {
     static constexpr int E = 16 / sizeof(T);               // elements per chunk
-    static constexpr int BK = 128 / sizeof(T);
-    static constexpr int CHUNKS = R * 8;
-    static constexpr int CPR = X ? R / E : 8;              // chunks per stored row
+    static constexpr int BK = KB / sizeof(T);
+    static constexpr int CHUNKS = R * KB / 16;
+    static constexpr int CPR = X ? R / E : KB / 16;        // chunks per stored row
+    static constexpr int READS = !X ? 1 : sizeof(T) == 4 ? 4 : 2;   // LDS instructions of one fragment
     static constexpr int SWZ16 = CPR >= 16 ? 7 : CPR / 2 - 1;
 
     static __device__ __forceinline__ int swizzle(int row) {
-        if constexpr (!X) return (row >> 1) & 7;
+        if constexpr (!X) return KB == 128 ? (row >> 1) & 7 : -(row >> 2) & 3;
         else if constexpr (sizeof(T) == 4) return ((row >> 2) & 3) << 2;
         else return (((row & 3) | ((row >> 3) & 1) << 2) & SWZ16) << 1;
     }
@@ -134,7 +142,7 @@ template <typename T, bool X, int R> struct Tile {
         typedef typename Frag<T>::type frag;
         if constexpr (!X) {
             const int row = r0 + (lane & 15), c = step * 4 + (lane >> 4);
-            return *(const frag*)(lds + row * 128 + ((c ^ swizzle(row)) << 4));
+            return *(const frag*)(lds + row * KB + ((c ^ swizzle(row)) << 4));
         } else if constexpr (sizeof(T) == 4) {
             frag f;
             const int r = r0 + (lane & 15);
@@ -159,119 +167,176 @@ template <typename T, bool X, int R> struct Tile {
     }
 };
 
-constexpr unsigned kOutOfRange = 0x80000000u;   // byte offset behind every buffer: such a load gives zero
 
-// Staging of one operand: `rows` m/n rows from r0, k from k0 of K. Elements outside the matrix become zero.
-// DIRECT: memory -> LDS without registers in 16-byte pieces through a buffer descriptor, whose range check supplies the
-// zeros; base, row stride and the contiguous extent must be multiples of 16 bytes. Otherwise through registers, for any
-// alignment.
-template <typename T, bool X, int R, int NT, bool DIRECT> struct Stager {
-    typedef Tile<T, X, R> Tl;
+// Staging of one operand through registers, for any alignment: `R` m/n rows from r0, k from k0. Elements outside the matrix
+// become zero.
+template <typename T, bool X, int R, int NT, int KB> struct Stager {
+    typedef Tile<T, X, R, KB> Tl;
     static constexpr int PER = Tl::CHUNKS / NT;
     static_assert(Tl::CHUNKS % NT == 0, "whole chunks per thread");
     const T* base;
     long long ld;
     int extent, K;                // extent of m/n, of k
-    unsigned off[DIRECT ? PER : 1];
-    typename Pack<T>::vec reg[DIRECT ? 1 : PER];
+    typename Pack<T>::vec reg[PER];
 
     __device__ __forceinline__ void init(const void* p, long long ld_, int r0, int extent_, int K_) {
         ld = ld_;
         extent = extent_ - r0;
         K = K_;
         base = (const T*)p + (X ? (long long)r0 : (long long)r0 * ld_);
-        if constexpr (DIRECT) {
+    }
+    __device__ __forceinline__ void fetch(int k0) {
 #pragma unroll
-            for (int i = 0; i < PER; ++i) {
-                int k, r;
-                Tl::place(i * NT + threadIdx.x, k, r);
-                off[i] = r < extent ? (unsigned)((X ? k * ld + r : r * ld + k) * sizeof(T)) : kOutOfRange;
-            }
+        for (int i = 0; i < PER; ++i) {
+            int k, r;
+            Tl::place(i * NT + threadIdx.x, k, r);
+            typename Pack<T>::vec v;
+#pragma unroll
+            for (int j = 0; j < Pack<T>::N; ++j) v[j] = (T)0.f;
+            if (k0 + k < K && r < extent) v = X ? load16_tail(base + (long long)(k0 + k) * ld, r, extent) : load16_tail(base + r * ld, k0 + k, K);
+            reg[i] = v;
         }
     }
-    __device__ __forceinline__ void fetch(int k0, char* lds) {
-        if constexpr (DIRECT) {
-            const T* p = base + (X ? (long long)k0 * ld : (long long)k0);
-            __amdgpu_buffer_rsrc_t rsrc = __builtin_amdgcn_make_buffer_rsrc((void*)p, 0, 0x7fffffff, 0x00020000);
-            const int left = K - k0;
+    __device__ __forceinline__ void commit(char* lds) {
 #pragma unroll
-            for (int i = 0; i < PER; ++i) {
-                unsigned o = off[i];
-                if (left < Tl::BK) {
-                    int k, r;
-                    Tl::place(i * NT + threadIdx.x, k, r);
-                    if (k >= left) o = kOutOfRange;
-                }
-                __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (__attribute__((address_space(3))) void*)(lds + (i * NT + (threadIdx.x & ~63)) * 16), 16, o, 0, 0, 0);
-            }
-        } else {
+        for (int i = 0; i < PER; ++i) *(typename Pack<T>::vec*)(lds + (i * NT + threadIdx.x) * 16) = reg[i];
+    }
+};
+
+constexpr unsigned kOutOfRange = 0x80000000u;   // byte offset behind every buffer: such a load gives zero
+
+// 16 bytes per lane from a buffer to LDS, lane l's at dst + 16 l. As assembly, because behind the builtin the compiler
+// waits for ALL outstanding requests in front of every transposing LDS read, which leaves nothing in flight (the
+// narrow dx product took 80 us instead of 41). No register is written; the kernel waits for arrivals itself. The s_nop
+// covers the wait states between a scalar write of m0 (or a vector write of the descriptor) and the request; nothing else in
+// these kernels uses m0.
+__device__ __forceinline__ void load_to_lds(u32x4 rsrc, unsigned offset, unsigned dst) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" : : "s"(dst), "v"(offset), "s"(rsrc));
+}
+__device__ __forceinline__ unsigned lds_address(const char* p) { return (unsigned)(uintptr_t)(__attribute__((address_space(3))) const char*)p; }
+
+// Staging of one operand from memory to LDS without registers, in 16-byte pieces through a buffer descriptor whose range
+// check supplies the zeros outside the matrix. Base, row stride and the contiguous extent are multiples of 16 bytes.
+template <typename T, bool X, int R, int NT, int KB> struct DirectStager {
+    typedef Tile<T, X, R, KB> Tl;
+    static constexpr int PER = Tl::CHUNKS / NT;
+    static_assert(Tl::CHUNKS % NT == 0, "whole chunks per thread");
+    const T* next;        // first element of the k rows that the next request takes
+    long long step;
+    unsigned off[PER];
+
+    __device__ __forceinline__ void init(const void* p, long long ld, int r0, int extent, int k0) {
+        next = (const T*)p + (X ? (long long)k0 * ld + r0 : (long long)r0 * ld + k0);
+        step = X ? Tl::BK * ld : Tl::BK;
 #pragma unroll
-            for (int i = 0; i < PER; ++i) {
-                int k, r;
-                Tl::place(i * NT + threadIdx.x, k, r);
-                typename Pack<T>::vec v;
-#pragma unroll
-                for (int j = 0; j < Pack<T>::N; ++j) v[j] = (T)0.f;
-                if (k0 + k < K && r < extent) {
-                    const long long kk = k0 + k;
-                    v = X ? load16_tail(base + kk * ld, r, extent) : load16_tail(base + r * ld, (int)kk, K);
-                }
-                reg[i] = v;
-            }
+        for (int i = 0; i < PER; ++i) {
+            int k, r;
+            Tl::place(i * NT + threadIdx.x, k, r);
+            off[i] = r0 + r < extent ? (unsigned)((X ? k * ld + r : r * ld + k) * (long long)sizeof(T)) : kOutOfRange;
         }
     }
-    __device__ __forceinline__ void commit(char* lds) {   // not DIRECT: registers -> LDS
-        if constexpr (!DIRECT) {
+    // the next tile, of whose k rows only `left` (or none, or all) exist, to LDS from address `dst` + 16 * lane of the wave
+    __device__ __forceinline__ void fetch(int left, unsigned dst) {
+        // raw buffer: address, no stride, bytes, flags
+        const u32x4 rsrc = {(unsigned)(uintptr_t)next, (unsigned)((uintptr_t)next >> 32) & 0xffffu, 0x7fffffffu, 0x00020000u};
+        next += step;
 #pragma unroll
-            for (int i = 0; i < PER; ++i) *(typename Pack<T>::vec*)(lds + (i * NT + threadIdx.x) * 16) = reg[i];
+        for (int i = 0; i < PER; ++i) {
+            unsigned o = off[i];
+            if (left < Tl::BK) {
+                int k, r;
+                Tl::place(i * NT + threadIdx.x, k, r);
+                if (k >= left) o = kOutOfRange;
+            }
+            load_to_lds(rsrc, o, dst + i * NT * 16);
         }
     }
 };
 
-// Four neighbouring results of row m from column n.
-template <typename T> __device__ __forceinline__ void epilogue4(const GemmArgs& g, int m, int n, f32x4 v) {
-    typedef T vec4 __attribute__((ext_vector_type(4)));
-    const bool whole = n + 4 <= g.N;
-    auto get = [&](const T* p, float* out) {
-        if (whole) {
-            vec4 t;
-            __builtin_memcpy(&t, p, sizeof(t));
+// Pack<T>::N neighbouring results of row m from column n < N, whose bias is given. EDGE: the row may end among them.
+template <typename T, bool EDGE> __device__ __forceinline__ void epilogue(const GemmArgs& g, int m, int n, const float* acc, const float* bias, int act) {
+    constexpr int V = Pack<T>::N;
+    float z[V];
+    typename Pack<T>::vec v;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) out[i] = (float)t[i];
-        } else {
+    for (int i = 0; i < V; ++i) z[i] = acc[i] + bias[i];
+    if (g.z) {   // kept for the backward in the operands' type: half the traffic of float32, one rounding of the slope's argument
 #pragma unroll
-            for (int i = 0; i < 4; ++i) out[i] = n + i < g.N ? (float)p[i] : 0.f;
-        }
-    };
-    auto put = [&](T* p, const float* in) {
-        if (whole) {
-            vec4 t;
-#pragma unroll
-            for (int i = 0; i < 4; ++i) t[i] = (T)in[i];
-            __builtin_memcpy(p, &t, sizeof(t));
-        } else {
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-                if (n + i < g.N) p[i] = (T)in[i];
-        }
-    };
-    float z[4], o[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) z[i] = v[i];
-    if (g.bias) {
-        get((const T*)g.bias + n, o);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) z[i] += o[i];
+        for (int i = 0; i < V; ++i) v[i] = (T)z[i];
+        T* p = (T*)g.z + (long long)m * g.N;
+        if (EDGE) store16_tail(p, n, g.N, v);
+        else store16(p + n, v);
     }
-    if (g.z) put((T*)g.z + (long long)m * g.N + n, z);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) z[i] = activate<T>(z[i], g.act);
+    for (int i = 0; i < V; ++i) z[i] = activate<T>(z[i], act);
     if (g.res) {
-        get((const T*)g.res + (long long)m * g.ldr + n, o);
+        const T* p = (const T*)g.res + (long long)m * g.ldr;
+        v = EDGE ? load16_tail(p, n, g.N) : load16(p + n);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) z[i] += o[i];
+        for (int i = 0; i < V; ++i) z[i] += (float)v[i];
     }
-    put((T*)g.y + (long long)m * g.N + n, z);
+#pragma unroll
+    for (int i = 0; i < V; ++i) v[i] = (T)z[i];
+    T* p = (T*)g.y + (long long)m * g.N;
+    if (EDGE) store16_tail(p, n, g.N, v);
+    else store16(p + n, v);
+}
+template <typename T> __device__ __forceinline__ void load_bias(const GemmArgs& g, int n, float* bias) {
+#pragma unroll
+    for (int i = 0; i < Pack<T>::N; ++i) bias[i] = 0.f;
+    if (g.bias && n < g.N) {
+        const auto v = load16_tail((const T*)g.bias, n, g.N);
+#pragma unroll
+        for (int i = 0; i < Pack<T>::N; ++i) bias[i] = (float)v[i];
+    }
+}
+
+// Accumulators -> results. A lane holds four neighbouring columns of one of 16 rows; through LDS (two pieces of its own for
+// every wave, in turn, 16 rows at a time) it comes to hold 16 bytes of a row, so that rows are read and written in whole
+// pieces. The vector units do this while the matrix cores stand still, so it is kept short: a lane's columns stay the same
+// (its bias is read once), and tiles inside the matrix check nothing.
+template <typename T, int FM, int FN, bool EDGE> __device__ __forceinline__ void store_rows(const GemmArgs& g, f32x4 (&acc)[FM][FN], int m0, int n0, char* lds, int act) {
+    constexpr int V = Pack<T>::N, WN = FN * 16, PITCH = WN + 4, LPR = WN / V, ROWS = 64 / LPR;
+    const int lane = threadIdx.x & 63;
+    const int c = lane % LPR * V, n = n0 + c;
+    float bias[V];
+    if (!g.part) load_bias<T>(g, n, bias);
+#pragma unroll
+    for (int i = 0; i < FM; ++i) {
+        float* sh = (float*)lds + ((threadIdx.x >> 6) * 2 + (i & 1)) * 16 * PITCH;
+#pragma unroll
+        for (int j = 0; j < FN; ++j) *(f32x4*)(sh + (lane & 15) * PITCH + j * 16 + (lane >> 4) * 4) = acc[i][j];
+#pragma unroll
+        for (int r0 = 0; r0 < 16; r0 += ROWS) {
+            const int r = r0 + lane / LPR, m = m0 + i * 16 + r;
+            float v[V];
+#pragma unroll
+            for (int e = 0; e < V; e += 4) {
+                const f32x4 q = *(const f32x4*)(sh + r * PITCH + c + e);
+#pragma unroll
+                for (int k = 0; k < 4; ++k) v[e + k] = q[k];
+            }
+            if (EDGE && (m >= g.M || n >= g.N)) continue;
+            if (g.part) {
+                float* p = g.part + ((long long)blockIdx.y * g.M + m) * g.N;
+#pragma unroll
+                for (int e = 0; e < V; e += 4) {
+                    const f32x4 q = {v[e], v[e + 1], v[e + 2], v[e + 3]};
+                    if (!EDGE) store16(p + n + e, q);
+                    else if (n + e < g.N) store16_tail(p, n + e, g.N, q);
+                }
+            } else {
+                epilogue<T, EDGE>(g, m, n, v, bias, act);
+            }
+        }
+    }
+}
+template <typename T, bool FORWARD, int FM, int FN> __device__ __forceinline__ void store_tile(const GemmArgs& g, f32x4 (&acc)[FM][FN], int m0, int n0, char* lds) {
+    if (m0 + FM * 16 > g.M || n0 + FN * 16 > g.N) store_rows<T, FM, FN, true>(g, acc, m0, n0, lds, FORWARD ? g.act : ACT_NONE);
+    else if (FORWARD && g.act == ACT_GELU) store_rows<T, FM, FN, false>(g, acc, m0, n0, lds, ACT_GELU);
+    else if (FORWARD && g.act == ACT_SILU) store_rows<T, FM, FN, false>(g, acc, m0, n0, lds, ACT_SILU);
+    else if (FORWARD && g.act == ACT_RELU) store_rows<T, FM, FN, false>(g, acc, m0, n0, lds, ACT_RELU);
+    else store_rows<T, FM, FN, false>(g, acc, m0, n0, lds, ACT_NONE);
 }
 
 // Tile of workgroup `b`: workgroups go round the eight XCDs, each with an L2 of its own, so each XCD gets a run of
@@ -284,13 +349,14 @@ __device__ __forceinline__ void tile_of(int b, int tm, int tn, int& im, int& in)
     in = (t % band) / rows;
 }
 
-template <typename T, bool XA, bool XB, int BM, int BN, int WM, int WN, bool DIRECT>
+// The product for operands on any alignment: one tile is multiplied while the next is on its way to registers.
+template <typename T, bool XA, bool XB, int BM, int BN, int WM, int WN>
 __global__ __launch_bounds__((BM / WM) * (BN / WN) * 64) void gemm_kernel(const GemmArgs g) {
-    constexpr int NT = (BM / WM) * (BN / WN) * 64;
-    typedef Tile<T, XA, BM> TA;
-    typedef Tile<T, XB, BN> TB;
+    constexpr int NT = (BM / WM) * (BN / WN) * 64, KB = 128;
+    typedef Tile<T, XA, BM, KB> TA;
+    typedef Tile<T, XB, BN, KB> TB;
     typedef typename Frag<T>::type frag;
-    constexpr int BK = TA::BK, A_BYTES = BM * 128, B_BYTES = BN * 128, FM = WM / 16, FN = WN / 16;
+    constexpr int BK = TA::BK, A_BYTES = BM * KB, B_BYTES = BN * KB, FM = WM / 16, FN = WN / 16;
     extern __shared__ __attribute__((aligned(16))) char lds[];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int wm = wave % (BM / WM) * WM, wn = wave / (BM / WM) * WN;
@@ -299,8 +365,8 @@ __global__ __launch_bounds__((BM / WM) * (BN / WN) * 64) void gemm_kernel(const 
     const int m0 = im * BM, n0 = in * BN;
     const int k_tiles = (g.K + BK - 1) / BK, t0 = blockIdx.y * g.tiles_per_split;
     const int t1 = t0 + g.tiles_per_split < k_tiles ? t0 + g.tiles_per_split : k_tiles;
-    Stager<T, XA, BM, NT, DIRECT> sa;
-    Stager<T, XB, BN, NT, DIRECT> sb;
+    Stager<T, XA, BM, NT, KB> sa;
+    Stager<T, XB, BN, NT, KB> sb;
     sa.init(g.a, g.lda, m0, g.M, g.K);
     sb.init(g.b, g.ldb, n0, g.N, g.K);
     f32x4 acc[FM][FN];
@@ -308,19 +374,17 @@ __global__ __launch_bounds__((BM / WM) * (BN / WN) * 64) void gemm_kernel(const 
     for (int i = 0; i < FM; ++i)
 #pragma unroll
         for (int j = 0; j < FN; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
-    if (t0 < t1) {
-        sa.fetch(t0 * BK, lds);
-        sb.fetch(t0 * BK, lds + A_BYTES);
-        sa.commit(lds);
-        sb.commit(lds + A_BYTES);
-    }
+    sa.fetch(t0 * BK);
+    sb.fetch(t0 * BK);
+    sa.commit(lds);
+    sb.commit(lds + A_BYTES);
     for (int t = t0; t < t1; ++t) {
         __syncthreads();   // this tile has arrived, and nobody reads the other buffer any more
         char* cur = lds + ((t - t0) & 1) * (A_BYTES + B_BYTES);
         char* nxt = lds + ((t - t0 + 1) & 1) * (A_BYTES + B_BYTES);
         if (t + 1 < t1) {
-            sa.fetch((t + 1) * BK, nxt);
-            sb.fetch((t + 1) * BK, nxt + A_BYTES);
+            sa.fetch((t + 1) * BK);
+            sb.fetch((t + 1) * BK);
         }
 #pragma unroll
         for (int s = 0; s < BK / Frag<T>::KSTEP; ++s) {
@@ -339,46 +403,221 @@ __global__ __launch_bounds__((BM / WM) * (BN / WN) * 64) void gemm_kernel(const 
             sb.commit(nxt + A_BYTES);
         }
     }
+    __syncthreads();   // the tiles' memory is free
+    store_tile<T, !XB, FM, FN>(g, acc, m0 + wm, n0 + wn, lds);
+}
+
+template <int N> struct Int { static constexpr int value = N; };
+
+// The product for operands on 16-byte boundaries. S tiles of 128 bytes of k go round in LDS, each worked off in two steps;
+// the fragments of the next step come out of LDS while the matrix cores work on the present one's, which are in
+// registers. One barrier per tile, in front of its second step: behind it the tile's fragments of every wave are in
+// registers, so that the request for the tile S further on may take its place, and the next tile has arrived (each wave has
+// waited for its own part of it). Requests go on behind the last tile (they read nothing and give zeros), so that the count
+// of outstanding ones is the same for every tile.
+template <typename T, bool XA, bool XB, int BM, int BN, int WM, int WN, int S>
+__global__ __launch_bounds__((BM / WM) * (BN / WN) * 64) void gemm_pipe_kernel(const GemmArgs g) {
+    constexpr int NT = (BM / WM) * (BN / WN) * 64, KB = 128;
+    typedef Tile<T, XA, BM, KB> TA;
+    typedef Tile<T, XB, BN, KB> TB;
+    typedef DirectStager<T, XA, BM, NT, KB> SA;
+    typedef DirectStager<T, XB, BN, NT, KB> SB;
+    typedef typename Frag<T>::type frag;
+    constexpr int BK = TA::BK, A_BYTES = BM * KB, STAGE = (BM + BN) * KB, FM = WM / 16, FN = WN / 16;
+    constexpr int WAIT = (S - 2) * (SA::PER + SB::PER);
+    static_assert(BK == 2 * Frag<T>::KSTEP && S >= 2 && WAIT + SA::PER + SB::PER < 64, "pipeline");
+    extern __shared__ __attribute__((aligned(16))) char lds[];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int wm = wave % (BM / WM) * WM, wn = wave / (BM / WM) * WN;
+    int im, in;
+    tile_of(blockIdx.x, (g.M + BM - 1) / BM, (g.N + BN - 1) / BN, im, in);
+    const int m0 = im * BM, n0 = in * BN;
+    const int k_tiles = (g.K + BK - 1) / BK, t0 = blockIdx.y * g.tiles_per_split;
+    const int t1 = t0 + g.tiles_per_split < k_tiles ? t0 + g.tiles_per_split : k_tiles;
+    int left = (t1 * BK < g.K ? t1 * BK : g.K) - t0 * BK;   // k rows that the next requests may still take
+    SA sa;
+    SB sb;
+    sa.init(g.a, g.lda, m0, g.M, t0 * BK);
+    sb.init(g.b, g.ldb, n0, g.N, t0 * BK);
+    const unsigned lds0 = __builtin_amdgcn_readfirstlane(lds_address(lds) + (threadIdx.x & ~63) * 16);
+    f32x4 acc[FM][FN];
 #pragma unroll
-    for (int i = 0; i < FM; ++i) {
-        const int m = m0 + wm + i * 16 + (lane & 15);
-        if (m >= g.M) continue;
+    for (int i = 0; i < FM; ++i)
 #pragma unroll
-        for (int j = 0; j < FN; ++j) {
-            const int n = n0 + wn + j * 16 + (lane >> 4) * 4;
-            if (n >= g.N) continue;
-            if (g.part) {
-                float* p = g.part + ((long long)blockIdx.y * g.M + m) * g.N + n;
-                if (n + 4 <= g.N) __builtin_memcpy(p, &acc[i][j], 16);
-                else
-                    for (int e = 0; n + e < g.N; ++e) p[e] = acc[i][j][e];
-            } else {
-                epilogue4<T>(g, m, n, acc[i][j]);
+        for (int j = 0; j < FN; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+    auto fetch = [&](int stage) {
+        sa.fetch(left, lds0 + stage * STAGE);
+        sb.fetch(left, lds0 + stage * STAGE + A_BYTES);
+        left -= BK;
+    };
+    frag fa[2][FM], fb[2][FN];
+    auto read = [&](auto step, int stage) {
+        constexpr int P = decltype(step)::value;
+        const char* cur = lds + stage * STAGE;
+#pragma unroll
+        for (int i = 0; i < FM; ++i) fa[P][i] = TA::read(cur, wm + i * 16, P, lane);
+#pragma unroll
+        for (int j = 0; j < FN; ++j) fb[P][j] = TB::read(cur + A_BYTES, wn + j * 16, P, lane);
+    };
+    auto multiply = [&](auto step) {
+        constexpr int P = decltype(step)::value;
+#pragma unroll
+        for (int i = 0; i < FM; ++i)
+#pragma unroll
+            for (int j = 0; j < FN; ++j) Frag<T>::mma(fb[P][j], fa[P][i], acc[i][j]);
+        // LDS reads between the matrix instructions, not in front of them or (what the compiler would do) behind them
+        constexpr int READS = FM * TA::READS + FN * TB::READS, MMAS = FM * FN * Frag<T>::MMAS, EACH = MMAS / READS > 0 ? MMAS / READS : 1;
+#pragma unroll
+        for (int i = 0; i < READS; ++i) {
+            __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);      // a read of LDS
+            __builtin_amdgcn_sched_group_barrier(0x008, EACH, 0);   // matrix instructions
+        }
+    };
+#pragma unroll
+    for (int i = 0; i < S; ++i) fetch(i);
+    asm volatile("s_waitcnt vmcnt(%0)" : : "n"(WAIT + SA::PER + SB::PER) : "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" : : : "memory");
+    read(Int<0>{}, 0);
+    int stage = 0;
+    for (int t = t0; t < t1; ++t) {
+        read(Int<1>{}, stage);
+        multiply(Int<0>{});
+        __builtin_amdgcn_sched_barrier(0);
+        asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" : : "n"(WAIT) : "memory");
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" : : : "memory");
+        fetch(stage);
+        stage = stage + 1 == S ? 0 : stage + 1;
+        read(Int<0>{}, stage);
+        multiply(Int<1>{});
+        __builtin_amdgcn_sched_barrier(0);
+    }
+    asm volatile("s_waitcnt vmcnt(0)" : : : "memory");
+    __syncthreads();   // the requests behind the end have landed, the tiles' memory is free
+    store_tile<T, !XB, FM, FN>(g, acc, m0 + wm, n0 + wn, lds);
+}
+
+// The forward product for few rows (M <= 16 MF): bound by reading the weight once. A workgroup takes 16 NF columns; its waves
+// share k out among themselves in runs of 128 bytes, each reading whole cache lines of 16 weight rows straight into
+// matrix-core operands (x in the same k order; rows behind M repeat the last one and are dropped), several runs in flight.
+// The waves' sums meet in LDS in a fixed order. Any alignment.
+template <typename T, int MF, int NF, int WAVES> __global__ __launch_bounds__(WAVES * 64) void gemm_few_rows_kernel(const GemmArgs g) {
+    typedef typename Pack<T>::vec vec;
+    constexpr int V = Pack<T>::N, RUN = 8 * V, U = MF * NF >= 8 ? 1 : MF * NF >= 4 ? 2 : 4;
+    extern __shared__ __attribute__((aligned(16))) char lds[];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, n0 = blockIdx.x * 16 * NF, kl = (lane >> 4) * 2 * V;
+    const T *pw[NF], *px[MF];
+#pragma unroll
+    for (int j = 0; j < NF; ++j) {
+        const int n = n0 + j * 16 + (lane & 15);
+        pw[j] = (const T*)g.b + (long long)(n < g.N ? n : g.N - 1) * g.ldb;
+    }
+#pragma unroll
+    for (int i = 0; i < MF; ++i) {
+        const int m = i * 16 + (lane & 15);
+        px[i] = (const T*)g.a + (long long)(m < g.M ? m : g.M - 1) * g.lda;
+    }
+    f32x4 acc[MF][NF];
+#pragma unroll
+    for (int i = 0; i < MF; ++i)
+#pragma unroll
+        for (int j = 0; j < NF; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+    vec fw[U][NF][2], fx[U][MF][2];
+    auto multiply = [&](int u) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int i = 0; i < MF; ++i)
+#pragma unroll
+                for (int j = 0; j < NF; ++j)
+                    Frag<T>::mma(__builtin_bit_cast(typename Frag<T>::type, fw[u][j][h]), __builtin_bit_cast(typename Frag<T>::type, fx[u][i][h]), acc[i][j]);
+    };
+    const int runs = g.K / RUN;
+    int run = wave;
+    for (; run + (U - 1) * WAVES < runs; run += U * WAVES) {
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int k = (run + u * WAVES) * RUN + kl;
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+#pragma unroll
+                for (int j = 0; j < NF; ++j) fw[u][j][h] = load16(pw[j] + k + h * V);
+#pragma unroll
+                for (int i = 0; i < MF; ++i) fx[u][i][h] = load16(px[i] + k + h * V);
             }
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u) multiply(u);
+    }
+    for (; run * RUN < g.K; run += WAVES) {   // the runs left over, the last of which may be short
+        const int k = run * RUN + kl;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            const int at = k + h * V;
+#pragma unroll
+            for (int j = 0; j < NF; ++j) {
+#pragma unroll
+                for (int e = 0; e < V; ++e) fw[0][j][h][e] = (T)0.f;
+                if (at < g.K) fw[0][j][h] = load16_tail(pw[j], at, g.K);
+            }
+#pragma unroll
+            for (int i = 0; i < MF; ++i) {
+#pragma unroll
+                for (int e = 0; e < V; ++e) fx[0][i][h][e] = (T)0.f;
+                if (at < g.K) fx[0][i][h] = load16_tail(px[i], at, g.K);
+            }
+        }
+        multiply(0);
+    }
+    f32x4* sh = (f32x4*)lds;
+#pragma unroll
+    for (int i = 0; i < MF; ++i)
+#pragma unroll
+        for (int j = 0; j < NF; ++j) sh[((wave * MF + i) * NF + j) * 64 + lane] = acc[i][j];
+    __syncthreads();
+    for (int t = threadIdx.x; t < MF * NF * 64; t += WAVES * 64) {
+        const int l = t & 63, j = t / 64 % NF, i = t / 64 / NF, m = i * 16 + (l & 15), n = n0 + j * 16 + (l >> 4) * 4;
+        if (m >= g.M || n >= g.N) continue;
+        f32x4 v = sh[t];
+#pragma unroll
+        for (int w = 1; w < WAVES; ++w) v += sh[w * MF * NF * 64 + t];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            if (n + e >= g.N) break;
+            float z = v[e] + (g.bias ? (float)((const T*)g.bias)[n + e] : 0.f);
+            const long long at = (long long)m * g.N + n + e;
+            if (g.z) ((T*)g.z)[at] = (T)z;
+            z = activate<T>(z, g.act);
+            if (g.res) z += (float)((const T*)g.res)[(long long)m * g.ldr + n + e];
+            ((T*)g.y)[at] = (T)z;
         }
     }
 }
 
-// Joins the partial products of the k ranges in their order and runs the epilogue. The results are taken four at a time
-// along a row.
+// Joins the partial products of the k ranges in their order and runs the epilogue.
 template <typename T> __global__ __launch_bounds__(256) void gemm_join_kernel(const GemmArgs g) {
-    const int quads = (g.N + 3) / 4;
-    const long long total = (long long)g.M * quads, stride = (long long)g.M * g.N;
+    constexpr int V = Pack<T>::N;
+    const int pieces = (g.N + V - 1) / V;
+    const long long total = (long long)g.M * pieces, stride = (long long)g.M * g.N;
     for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < total; i += (long long)gridDim.x * 256) {
-        const int m = (int)(i / quads), n = (int)(i % quads) * 4;
-        const float* p = g.part + (long long)m * g.N + n;
-        f32x4 v = f32x4{0.f, 0.f, 0.f, 0.f};
-        if (n + 4 <= g.N) {
-            for (int s = 0; s < g.splits; ++s) {
-                f32x4 w;
-                __builtin_memcpy(&w, p + s * stride, 16);
-                v += w;
-            }
-        } else {
-            for (int s = 0; s < g.splits; ++s)
-                for (int e = 0; n + e < g.N; ++e) v[e] += p[s * stride + e];
+        const int m = (int)(i / pieces), n = (int)(i % pieces) * V;
+        const float* p = g.part + (long long)m * g.N;
+        float v[V];
+#pragma unroll
+        for (int e = 0; e < V; ++e) v[e] = 0.f;
+        for (int s = 0; s < g.splits; ++s, p += stride) {
+#pragma unroll
+            for (int e = 0; e < V; e += 4)
+                if (n + e < g.N) {
+                    const f32x4 w = load16_tail(p, n + e, g.N);
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) v[e + k] += w[k];
+                }
         }
-        epilogue4<T>(g, m, n, v);
+        float bias[V];
+        load_bias<T>(g, n, bias);
+        epilogue<T, true>(g, m, n, v, bias, g.act);
     }
 }
 
@@ -457,26 +696,41 @@ template <typename T> __global__ __launch_bounds__(256) void zero_kernel(T* p, l
 inline int elem(int dtype) { return dtype == DMN_DT_F32 ? 4 : 2; }
 inline long long ceil_div(long long a, long long b) { return (a + b - 1) / b; }
 
-// Tile and k split of a product, from its sizes and type alone.
+// Tile and k split of a product, from its sizes and type alone, by the time that the tiles were measured to take (MI355X, us):
+// `step` for 128 bytes of k when every CU has one, `least` for one that has its CU to itself, `ends` for what stands
+// around the steps (first request, epilogue, launch). Where there are fewer tiles than CUs, k is split: the partial products
+// are written and read again at some 4 TB/s, in one more launch.
 struct GemmPlan {
-    int bm, bn, splits, per;
+    int tile, splits, per;   // index into kTiles; k tiles are counted in 128 bytes of k
 };
+struct TileShape {
+    int bm, bn;
+    double step16, least16, step32, least32, ends;
+};
+const TileShape kTiles[3] = {{256, 256, 1.60, 1.12, 7.5, 7.2, 8.0}, {128, 128, 0.56, 0.45, 2.0, 1.9, 4.0}, {64, 64, 0.22, 0.28, 0.50, 0.55, 3.0}};
+
 GemmPlan gemm_plan(int M, int N, int K, int dtype) {
-    GemmPlan p;
     const int bk = 128 / elem(dtype);
-    const long long big = ceil_div(M, 128) * ceil_div(N, 128);
-    p.bm = p.bn = big >= 200 ? 128 : 64;
-    const long long tiles = ceil_div(M, p.bm) * ceil_div(N, p.bn), kt = ceil_div(K, bk);
-    long long splits = 1;
-    if (tiles < 256 && kt >= 8) {
-        splits = 512 / tiles;
-        if (splits > kt / 4) splits = kt / 4;
-        if (splits > 64) splits = 64;
-        if (splits < 1) splits = 1;
+    const long long kt = ceil_div(K, bk);
+    GemmPlan best{2, 1, (int)kt};
+    double best_us = 1e30;
+    for (int i = 0; i < 3; ++i) {
+        const TileShape& t = kTiles[i];
+        const double step = dtype == DMN_DT_F32 ? t.step32 : t.step16, least = dtype == DMN_DT_F32 ? t.least32 : t.least16;
+        const long long tiles = ceil_div(M, t.bm) * ceil_div(N, t.bn);
+        for (int splits = 1; splits <= 64; splits *= 2) {
+            if (splits > 1 && kt / splits < 4) break;
+            const long long per = ceil_div(kt, splits), rounds = ceil_div(tiles * splits, 256);
+            const double all = tiles * splits > 128 ? rounds * per * step : 0, one = per * least;
+            double us = (all > one ? all : one) + t.ends * (i == 2 ? 1 : rounds);
+            if (splits > 1) us += 3.0 + (double)splits * M * N * 8 / 4e6;
+            if (us < best_us) {
+                best_us = us;
+                best = {i, (int)ceil_div(kt, per), (int)per};
+            }
+        }
     }
-    p.per = (int)ceil_div(kt, splits);
-    p.splits = (int)ceil_div(kt, p.per);
-    return p;
+    return best;
 }
 size_t gemm_workspace(int M, int N, int K, int dtype) {
     const GemmPlan p = gemm_plan(M, N, K, dtype);
@@ -489,25 +743,64 @@ bool direct_ok(const void* p, long long ld, bool x, int rows, int K, int dtype) 
     return (uintptr_t)p % 16 == 0 && ld * e % 16 == 0 && (long long)(x ? rows : K) * e % 16 == 0;
 }
 
-template <typename T, bool XA, bool XB, int B, int W, bool DIRECT> int gemm_launch(const GemmArgs& g, hipStream_t s) {
-    constexpr int NT = (B / W) * (B / W) * 64, LDS = 2 * 2 * B * 128;
-    const dim3 grid((unsigned)(ceil_div(g.M, B) * ceil_div(g.N, B)), g.splits);
-    gemm_kernel<T, XA, XB, B, B, W, W, DIRECT><<<grid, NT, LDS, s>>>(g);
+template <typename F> int allow_lds(F* kernel, int bytes) {
+    if (bytes > 65536) DMN_HIP_CHECK(hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, bytes));
+    return DMN_OK;
+}
+template <typename T, bool XA, bool XB, int BM, int BN, int WM, int WN, int S> int pipe_launch(const GemmArgs& g, hipStream_t s) {
+    constexpr int NT = (BM / WM) * (BN / WN) * 64, LDS = S * (BM + BN) * 128;
+    static_assert((NT / 64) * 2 * 16 * (WN + 4) * 4 <= LDS, "the epilogue's pieces fit the tiles' memory");
+    auto* kernel = gemm_pipe_kernel<T, XA, XB, BM, BN, WM, WN, S>;
+    const int rc = allow_lds(kernel, LDS);
+    if (rc) return rc;
+    kernel<<<dim3((unsigned)(ceil_div(g.M, BM) * ceil_div(g.N, BN)), g.splits), NT, LDS, s>>>(g);
     DMN_BLOCK_LAUNCH_CHECK();
     return DMN_OK;
 }
+template <typename T, bool XA, bool XB, int B, int W> int any_launch(const GemmArgs& g, hipStream_t s) {
+    constexpr int NT = (B / W) * (B / W) * 64, LDS = 2 * 2 * B * 128;
+    static_assert((NT / 64) * 2 * 16 * (W + 4) * 4 <= LDS, "the epilogue's pieces fit the tiles' memory");
+    gemm_kernel<T, XA, XB, B, B, W, W><<<dim3((unsigned)(ceil_div(g.M, B) * ceil_div(g.N, B)), g.splits), NT, LDS, s>>>(g);
+    DMN_BLOCK_LAUNCH_CHECK();
+    return DMN_OK;
+}
+// Up to 64 rows the forward reads the weight once whatever it does, and the tiles' kernel cannot fill the chip.
+bool few_rows(int M) { return M <= 64; }
+template <typename T, int MF, int NF, int WAVES> int few_rows_launch(const GemmArgs& g, hipStream_t s) {
+    constexpr int LDS = WAVES * MF * NF * 1024;
+    static_assert(LDS <= 65536, "LDS without an attribute");
+    gemm_few_rows_kernel<T, MF, NF, WAVES><<<(unsigned)ceil_div(g.N, 16 * NF), WAVES * 64, LDS, s>>>(g);
+    DMN_BLOCK_LAUNCH_CHECK();
+    return DMN_OK;
+}
+template <typename T> int few_rows_run(const GemmArgs& g, hipStream_t s) {
+    // columns per workgroup: more of them read x less often, fewer fill the chip; waves: some eight per CU
+    const long long cols = ceil_div(g.N, 16);
+    if (g.M <= 16) return cols >= 512 ? few_rows_launch<T, 1, 1, 4>(g, s) : cols >= 256 ? few_rows_launch<T, 1, 1, 8>(g, s) : few_rows_launch<T, 1, 1, 16>(g, s);
+    if (g.M <= 32) return cols >= 512 ? few_rows_launch<T, 2, 2, 8>(g, s) : few_rows_launch<T, 2, 1, 16>(g, s);
+    return cols >= 1024 ? few_rows_launch<T, 4, 4, 4>(g, s) : cols >= 512 ? few_rows_launch<T, 4, 2, 8>(g, s) : few_rows_launch<T, 4, 1, 16>(g, s);
+}
+
 template <typename T, bool XA, bool XB> int gemm_run(GemmArgs& g, int dtype, void* ws, hipStream_t s) {
+    if (!XB && few_rows(g.M)) {
+        if constexpr (!XB) return few_rows_run<T>(g, s);
+    }
     const GemmPlan p = gemm_plan(g.M, g.N, g.K, dtype);
     g.splits = p.splits;
     g.tiles_per_split = p.per;
     g.part = p.splits > 1 ? (float*)ws : nullptr;
     const bool direct = direct_ok(g.a, g.lda, XA, g.M, g.K, dtype) && direct_ok(g.b, g.ldb, XB, g.N, g.K, dtype);
     int rc;
-    if (p.bm == 128) rc = direct ? gemm_launch<T, XA, XB, 128, 64, true>(g, s) : gemm_launch<T, XA, XB, 128, 64, false>(g, s);
-    else rc = direct ? gemm_launch<T, XA, XB, 64, 32, true>(g, s) : gemm_launch<T, XA, XB, 64, 32, false>(g, s);
-    if (rc || p.splits == 1) return rc;
-    const long long quads = (long long)g.M * ceil_div(g.N, 4);
-    gemm_join_kernel<T><<<(unsigned)(quads < 256 * 4096 ? ceil_div(quads, 256) : 4096), 256, 0, s>>>(g);
+    if (direct) {
+        if (p.tile == 0) rc = pipe_launch<T, XA, XB, 256, 256, 128, 64, 2>(g, s);
+        else if (p.tile == 1) rc = pipe_launch<T, XA, XB, 128, 128, 64, 32, 4>(g, s);
+        else rc = pipe_launch<T, XA, XB, 64, 64, 32, 32, 3>(g, s);
+    } else {
+        rc = p.tile < 2 ? any_launch<T, XA, XB, 128, 64>(g, s) : any_launch<T, XA, XB, 64, 32>(g, s);
+    }
+    if (rc || g.splits == 1) return rc;
+    const long long pieces = (long long)g.M * ceil_div(g.N, Pack<T>::N);
+    gemm_join_kernel<T><<<(unsigned)(pieces < 256 * 4096 ? ceil_div(pieces, 256) : 4096), 256, 0, s>>>(g);
     DMN_BLOCK_LAUNCH_CHECK();
     return DMN_OK;
 }
@@ -594,7 +887,7 @@ int backward_run(const void* dy, long long lddy, const void* x, long long ldx, c
 }  // namespace
 
 extern "C" size_t dmn_linear_forward_workspace_bytes(int64_t rows, int in, int out, int dtype) {
-    if (rows <= 0 || rows >= (1 << 27) || in <= 0 || out <= 0 || dtype < 0 || dtype > 2) return 0;
+    if (rows <= 0 || rows >= (1 << 27) || in <= 0 || out <= 0 || dtype < 0 || dtype > 2 || few_rows((int)rows)) return 0;
     return gemm_workspace((int)rows, out, in, dtype);
 }
 
