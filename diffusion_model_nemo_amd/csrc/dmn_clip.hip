@@ -16,14 +16,14 @@
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kMaxChunks = 2048;    // workgroups a large total is spread over: eight per CU, resident together
-constexpr int kMinChunk = 8192;     // elements of one workgroup at least
+constexpr int kBlocks = 2048;       // workgroups of one launch: eight per CU, resident together
+constexpr int64_t kKeep = 80 << 20;  // bytes that the cache behind the L2s is trusted to keep between the passes
+constexpr int kPiece = 8192;        // elements that a workgroup takes at a time: neighbouring workgroups read neighbouring pieces
 
-// Tensors of one launch: entry i owns the workgroups [first[i], first[i + 1]).
+// Tensors of one launch: entry i owns the pieces [first[i], first[i + 1]).
 template <bool OUT> struct ClipTable {
     static constexpr int K = OUT ? 136 : 192;
-    int count, part_base;           // entries; index of the launch's first workgroup among all
-    long long chunk;                // elements per workgroup
+    int count, part_base;           // entries; index of the launch's first partial among all
     int first[K + 1];
     unsigned long long meta[K];     // element count << 8 | type of dst << 4 | type of src
     const void* src[K];
@@ -56,19 +56,24 @@ __device__ __forceinline__ double block_join(double v, int inf_norm, double* sh)
     return v;
 }
 
-template <typename T, bool INF> __device__ __forceinline__ double chunk_norm(const T* p, long long n) {
+// STREAM: the data is not kept in the caches.
+template <typename T, bool INF, bool STREAM> __device__ __forceinline__ double piece_norm(const T* p, int n) {
     constexpr int V = Pack<T>::N;
     double acc[4] = {0., 0., 0., 0.};
     auto add = [&](float x, int k) {
         if constexpr (INF) acc[k & 3] = max_nan(acc[k & 3], (double)fabsf(x));
         else acc[k & 3] = __builtin_fma((double)x, (double)x, acc[k & 3]);
     };
-    long long i = (long long)threadIdx.x * V;
+    int i = threadIdx.x * V;
     constexpr int STEP = kThreads * V;
+    typedef typename Pack<T>::vec loose __attribute__((aligned(sizeof(T))));
     for (; i + 3 * STEP + V <= n; i += 4 * STEP) {
         typename Pack<T>::vec v[4];
 #pragma unroll
-        for (int k = 0; k < 4; ++k) v[k] = load16(p + i + k * STEP);
+        for (int k = 0; k < 4; ++k) {
+            if constexpr (STREAM) v[k] = __builtin_nontemporal_load((const loose*)(p + i + k * STEP));
+            else v[k] = load16(p + i + k * STEP);
+        }
 #pragma unroll
         for (int k = 0; k < 4; ++k)
 #pragma unroll
@@ -86,30 +91,38 @@ template <typename T, bool INF> __device__ __forceinline__ double chunk_norm(con
     return INF ? max_nan(max_nan(acc[0], acc[1]), max_nan(acc[2], acc[3])) : (acc[0] + acc[1]) + (acc[2] + acc[3]);
 }
 
-// Entry of workgroup `b` (b < first[count]): binary search over scalars.
-template <bool OUT> __device__ __forceinline__ int find_entry(const ClipTable<OUT>& t, int b) {
+// Entry of piece `p` (p < first[count]): binary search over scalars.
+template <bool OUT> __device__ __forceinline__ int find_entry(const ClipTable<OUT>& t, int p) {
     int lo = 0, hi = t.count;
     while (hi - lo > 1) {
         const int mid = (lo + hi) >> 1;
-        if (t.first[mid] <= b) lo = mid;
+        if (t.first[mid] <= p) lo = mid;
         else hi = mid;
     }
     return lo;
 }
 
-template <bool INF> __global__ __launch_bounds__(kThreads) void grad_norm_kernel(const ClipTable<false> t, double* part) {
+template <bool INF, bool STREAM> __device__ __forceinline__ double piece_norm_of(const void* src, int dt, long long at, int n) {
+    if (dt == DMN_DT_F32) return piece_norm<float, INF, STREAM>((const float*)src + at, n);
+    if (dt == DMN_DT_BF16) return piece_norm<__bf16, INF, STREAM>((const __bf16*)src + at, n);
+    return piece_norm<f16, INF, STREAM>((const f16*)src + at, n);
+}
+// Pieces below `stream_pieces` are read past the caches.
+template <bool INF> __global__ __launch_bounds__(kThreads) void grad_norm_kernel(const ClipTable<false> t, double* part, int stream_pieces) {
     __shared__ double sh[kThreads / 64];
-    const int b = blockIdx.x, e = find_entry(t, b);
-    const unsigned long long meta = t.meta[e];
-    const long long at = (long long)(b - t.first[e]) * t.chunk, n = (long long)(meta >> 8);
-    const long long len = n - at < t.chunk ? n - at : t.chunk;
-    const int dt = (int)(meta & 15);
-    double v;
-    if (dt == DMN_DT_F32) v = chunk_norm<float, INF>((const float*)t.src[e] + at, len);
-    else if (dt == DMN_DT_BF16) v = chunk_norm<__bf16, INF>((const __bf16*)t.src[e] + at, len);
-    else v = chunk_norm<f16, INF>((const f16*)t.src[e] + at, len);
+    const int pieces = t.first[t.count];
+    double v = 0.;
+    int e = find_entry(t, blockIdx.x);
+    for (int p = blockIdx.x; p < pieces; p += gridDim.x) {
+        while (t.first[e + 1] <= p) ++e;
+        const unsigned long long meta = t.meta[e];
+        const long long at = (long long)(p - t.first[e]) * kPiece, n = (long long)(meta >> 8);
+        const int len = (int)(n - at < kPiece ? n - at : kPiece), dt = (int)(meta & 15);
+        const double w = p < stream_pieces ? piece_norm_of<INF, true>(t.src[e], dt, at, len) : piece_norm_of<INF, false>(t.src[e], dt, at, len);
+        v = INF ? max_nan(v, w) : v + w;
+    }
     v = block_join(v, INF, sh);
-    if (threadIdx.x == 0) part[t.part_base + b] = v;
+    if (threadIdx.x == 0) part[t.part_base + blockIdx.x] = v;
 }
 
 // The factor of every element from the partials of all launches.
@@ -123,9 +136,9 @@ __device__ __forceinline__ float clip_factor(const ClipScale& c, double* sh, flo
     return (float)((f >= 1.0 ? 1.0 : f) * (double)c.grad_scale);   // a NaN stays
 }
 
-template <typename S, typename D> __device__ __forceinline__ void chunk_scale(const S* src, D* dst, long long n, float f) {
+template <typename S, typename D> __device__ __forceinline__ void piece_scale(const S* src, D* dst, int n, float f) {
     constexpr int V = Pack<S>::N, W = Pack<D>::N, STEP = kThreads * V;
-    auto put = [&](typename Pack<S>::vec v, long long i) {
+    auto put = [&](typename Pack<S>::vec v, int i) {
         if constexpr (V >= W) {
 #pragma unroll
             for (int k = 0; k < V / W; ++k) {
@@ -141,7 +154,7 @@ template <typename S, typename D> __device__ __forceinline__ void chunk_scale(co
             __builtin_memcpy(dst + i, o, sizeof(o));
         }
     };
-    long long i = (long long)threadIdx.x * V;
+    int i = threadIdx.x * V;
     for (; i + 3 * STEP + V <= n; i += 4 * STEP) {
         typename Pack<S>::vec v[4];
 #pragma unroll
@@ -156,11 +169,11 @@ template <typename S, typename D> __device__ __forceinline__ void chunk_scale(co
     }
 }
 
-template <typename S> __device__ __forceinline__ void chunk_scale_to(const void* src, void* dst, int dt, long long at, long long n, float f) {
+template <typename S> __device__ __forceinline__ void piece_scale_to(const void* src, void* dst, int dt, long long at, int n, float f) {
     const S* s = (const S*)src + at;
-    if (dt == DMN_DT_F32) chunk_scale(s, (float*)dst + at, n, f);
-    else if (dt == DMN_DT_BF16) chunk_scale(s, (__bf16*)dst + at, n, f);
-    else chunk_scale(s, (f16*)dst + at, n, f);
+    if (dt == DMN_DT_F32) piece_scale(s, (float*)dst + at, n, f);
+    else if (dt == DMN_DT_BF16) piece_scale(s, (__bf16*)dst + at, n, f);
+    else piece_scale(s, (f16*)dst + at, n, f);
 }
 
 template <bool OUT> __global__ __launch_bounds__(kThreads) void grad_scale_kernel(const ClipTable<OUT> t, const ClipScale c) {
@@ -169,15 +182,19 @@ template <bool OUT> __global__ __launch_bounds__(kThreads) void grad_scale_kerne
     const float f = clip_factor(c, sh, &norm);
     if (c.write_norm && blockIdx.x == 0 && threadIdx.x == 0) *c.norm = norm;
     if (!OUT && f == 1.0f) return;    // in place and within the limit: the tensors are what they should be
-    const int b = gridDim.x - 1 - blockIdx.x, e = find_entry(t, b);   // last read first: it may still be in the cache
-    const unsigned long long meta = t.meta[e];
-    const long long at = (long long)(b - t.first[e]) * t.chunk, n = (long long)(meta >> 8);
-    const long long len = n - at < t.chunk ? n - at : t.chunk;
-    const int st = (int)(meta & 15), dt = (int)((meta >> 4) & 15);
-    void* dst = OUT ? t.dst[e] : (void*)t.src[e];
-    if (st == DMN_DT_F32) chunk_scale_to<float>(t.src[e], dst, OUT ? dt : DMN_DT_F32, at, len, f);
-    else if (st == DMN_DT_BF16) chunk_scale_to<__bf16>(t.src[e], dst, OUT ? dt : DMN_DT_BF16, at, len, f);
-    else chunk_scale_to<f16>(t.src[e], dst, OUT ? dt : DMN_DT_F16, at, len, f);
+    // from the end, which was read last and may still be in the cache
+    int e = t.count - 1;
+    for (int p = t.first[t.count] - 1 - (int)blockIdx.x; p >= 0; p -= gridDim.x) {
+        while (t.first[e] > p) --e;
+        const unsigned long long meta = t.meta[e];
+        const long long at = (long long)(p - t.first[e]) * kPiece, n = (long long)(meta >> 8);
+        const int len = (int)(n - at < kPiece ? n - at : kPiece);
+        const int st = (int)(meta & 15), dt = (int)((meta >> 4) & 15);
+        void* dst = OUT ? t.dst[e] : (void*)t.src[e];
+        if (st == DMN_DT_F32) piece_scale_to<float>(t.src[e], dst, OUT ? dt : DMN_DT_F32, at, len, f);
+        else if (st == DMN_DT_BF16) piece_scale_to<__bf16>(t.src[e], dst, OUT ? dt : DMN_DT_BF16, at, len, f);
+        else piece_scale_to<f16>(t.src[e], dst, OUT ? dt : DMN_DT_F16, at, len, f);
+    }
 }
 
 __global__ __launch_bounds__(kThreads) void grad_norm_only_kernel(const ClipScale c) {
@@ -222,13 +239,20 @@ int ranges_overlap(const DmnGradTensor* t, int n) {
     return bad;
 }
 
-// Hands `emit` one launch's table after the other; part indices run on over the launches.
-template <bool OUT, typename F> int for_tables(const DmnGradTensor* t, int n, long long chunk, F emit) {
+// Workgroups of one of the launches that n tensors need (at most): fewer where there are many launches, because every
+// workgroup of the second kind adds the partials of all of them.
+int blocks_per_launch(int n) {
+    const int launches = (n + ClipTable<false>::K - 1) / ClipTable<false>::K;
+    return launches <= 4 ? kBlocks : launches <= 16 ? kBlocks / 4 : kBlocks / 16;
+}
+
+// Hands `emit` one launch's table after the other with its workgroups; the partials' indices run on over the launches.
+template <bool OUT, typename F> int for_tables(const DmnGradTensor* t, int n, F emit) {
     ClipTable<OUT> tab;
     tab.count = 0;
     tab.part_base = 0;
-    tab.chunk = chunk;
     tab.first[0] = 0;
+    const int most = blocks_per_launch(n);
     int rc = DMN_OK;
     for (int i = 0; i < n && !rc; ++i) {
         if (t[i].numel > 0) {
@@ -236,11 +260,12 @@ template <bool OUT, typename F> int for_tables(const DmnGradTensor* t, int n, lo
             tab.src[k] = t[i].src;
             if (OUT) tab.dst[OUT ? k : 0] = t[i].dst;
             tab.meta[k] = (unsigned long long)t[i].numel << 8 | (unsigned)t[i].dst_dtype << 4 | (unsigned)t[i].src_dtype;
-            tab.first[k + 1] = tab.first[k] + (int)((t[i].numel + chunk - 1) / chunk);
+            tab.first[k + 1] = tab.first[k] + (int)((t[i].numel + kPiece - 1) / kPiece);
         }
         if (tab.count == ClipTable<OUT>::K || (i == n - 1 && tab.count)) {
-            rc = emit(tab, tab.first[tab.count]);
-            tab.part_base += tab.first[tab.count];
+            const int pieces = tab.first[tab.count], blocks = pieces < most ? pieces : most;
+            rc = emit(tab, blocks);
+            tab.part_base += blocks;
             tab.count = 0;
         }
     }
@@ -250,7 +275,9 @@ template <bool OUT, typename F> int for_tables(const DmnGradTensor* t, int n, lo
 }  // namespace
 
 extern "C" size_t dmn_clip_grads_workspace_bytes(int n_tensors) {
-    return n_tensors < 0 ? 0 : (size_t)(kMaxChunks + (size_t)n_tensors) * sizeof(double) + 256;
+    if (n_tensors < 0) return 0;
+    const size_t launches = ((size_t)n_tensors + ClipTable<false>::K - 1) / ClipTable<false>::K;
+    return launches * blocks_per_launch(n_tensors) * sizeof(double) + 256;
 }
 
 extern "C" int dmn_clip_grads(const DmnGradTensor* tensors, int n_tensors, int inf_norm, float max_norm, float grad_scale, float* norm,
@@ -261,7 +288,7 @@ extern "C" int dmn_clip_grads(const DmnGradTensor* tensors, int n_tensors, int i
                 "dmn_clip_grads: inf_norm must be 0 or 1, max_norm >= 0 and grad_scale finite");
     DMN_REQUIRE((uintptr_t)workspace % 8 == 0 && workspace_bytes >= dmn_clip_grads_workspace_bytes(n_tensors), DMN_ERR_WORKSPACE,
                 "dmn_clip_grads: workspace of %zu bytes, %zu needed (8-byte aligned)", workspace_bytes, dmn_clip_grads_workspace_bytes(n_tensors));
-    long long total = 0;
+    int64_t total = 0, bytes = 0;
     int writes = 0, separate = 0;
     for (int i = 0; i < n_tensors; ++i) {
         const DmnGradTensor& t = tensors[i];
@@ -271,20 +298,19 @@ extern "C" int dmn_clip_grads(const DmnGradTensor* tensors, int n_tensors, int i
         DMN_REQUIRE(t.src && (uintptr_t)t.src % dt_bytes(t.src_dtype) == 0 && (uintptr_t)t.dst % dt_bytes(t.dst_dtype) == 0, DMN_ERR_INVALID,
                     "dmn_clip_grads: tensor %d has no address, or one that is not aligned to its type", i);
         total += t.numel;
+        bytes += t.numel * dt_bytes(t.src_dtype);
         writes += t.dst != nullptr;
         separate |= t.dst && (t.dst != t.src || t.dst_dtype != t.src_dtype);
     }
     int used = 0;
     for (int i = 0; i < n_tensors; ++i) used += tensors[i].numel > 0;
-    DMN_REQUIRE(total < ((int64_t)1 << 42), DMN_ERR_LIMIT, "dmn_clip_grads: more than 2^42 elements");
+    DMN_REQUIRE(total < ((int64_t)1 << 43), DMN_ERR_LIMIT, "dmn_clip_grads: more than 2^43 elements");   // pieces count in 31 bits
     DMN_REQUIRE(writes == 0 || writes == used, DMN_ERR_INVALID, "dmn_clip_grads: either every tensor has a destination or none");
     if (writes) {
         const int bad = ranges_overlap(tensors, n_tensors);
         DMN_REQUIRE(bad != 2, DMN_ERR_LIMIT, "dmn_clip_grads: out of host memory");
         DMN_REQUIRE(bad == 0, DMN_ERR_INVALID, "dmn_clip_grads: a tensor that is written overlaps another one (or is listed twice)");
     }
-    long long chunk = (total + kMaxChunks - 1) / kMaxChunks;
-    chunk = chunk < kMinChunk ? kMinChunk : (chunk + 2047) / 2048 * 2048;
     hipStream_t s = (hipStream_t)stream;
     double* part = (double*)workspace;
     ClipScale c{};
@@ -293,9 +319,19 @@ extern "C" int dmn_clip_grads(const DmnGradTensor* tensors, int n_tensors, int i
     c.max_norm = max_norm;
     c.grad_scale = grad_scale;
     c.norm = norm;
-    int rc = for_tables<false>(tensors, n_tensors, chunk, [&](const ClipTable<false>& t, int blocks) -> int {
-        if (inf_norm) grad_norm_kernel<true><<<blocks, kThreads, 0, s>>>(t, part);
-        else grad_norm_kernel<false><<<blocks, kThreads, 0, s>>>(t, part);
+    // What the caches cannot hold until the second pass is read past them, all but the end, where that pass begins. Norm and
+    // scaling of 403 M bfloat16 elements (0.8 GB) into float32, us: 125 + 499 with nothing kept, 130 + 490 with 80 MB, 156 +
+    // 477 with 160 MB, 176 + 480 with everything through the caches.
+    int64_t before = 0;
+    int rc = for_tables<false>(tensors, n_tensors, [&](const ClipTable<false>& t, int blocks) -> int {
+        int stream = 0;
+        for (int i = 0; i < t.count && before < bytes - kKeep; ++i) {
+            before += (int64_t)(t.meta[i] >> 8) * dt_bytes((int)(t.meta[i] & 15));
+            stream = t.first[i + 1];
+            if (before > bytes - kKeep) stream -= (int)((before - (bytes - kKeep)) / dt_bytes((int)(t.meta[i] & 15)) / kPiece);
+        }
+        if (inf_norm) grad_norm_kernel<true><<<blocks, kThreads, 0, s>>>(t, part, stream);
+        else grad_norm_kernel<false><<<blocks, kThreads, 0, s>>>(t, part, stream);
         c.parts = t.part_base + blocks;
         DMN_BLOCK_LAUNCH_CHECK();
         return DMN_OK;
@@ -313,5 +349,5 @@ extern "C" int dmn_clip_grads(const DmnGradTensor* tensors, int n_tensors, int i
         DMN_BLOCK_LAUNCH_CHECK();
         return DMN_OK;
     };
-    return separate ? for_tables<true>(tensors, n_tensors, chunk, scale) : for_tables<false>(tensors, n_tensors, chunk, scale);
+    return separate ? for_tables<true>(tensors, n_tensors, scale) : for_tables<false>(tensors, n_tensors, scale);
 }

@@ -336,24 +336,27 @@ template <typename A> __global__ __launch_bounds__(1024) void ln_params_kernel(c
     }
 }
 
-// Threads per row, vectors per thread, threads per workgroup for rows of `vecs` 16-byte vectors.
+// Threads per row, vectors per thread, threads per workgroup for rows of `vecs` 16-byte vectors of `per` elements. A thread
+// holds at most 16 elements of a row: with 32 (64 threads for a row of 2048 bfloat16) the backward's registers leave one
+// wave per SIMD, and 16384 rows took 64 us instead of 47; 16 float32 elements in four vectors are better than in one (81
+// against 87 us for 32768 rows of 1024).
 struct LnPlan {
     int tpr, nv, nt;
 };
-LnPlan ln_plan(long long vecs) {
+LnPlan ln_plan(long long vecs, int per) {
     if (vecs <= 8) return {8, 1, 256};
     if (vecs <= 16) return {16, 1, 256};
     if (vecs <= 32) return {32, 1, 256};
     if (vecs <= 64) return {64, 1, 256};
     if (vecs <= 128) return {64, 2, 256};
-    if (vecs <= 256) return {64, 4, 256};
+    if (vecs <= 256) return per == 4 ? LnPlan{64, 4, 256} : LnPlan{256, 1, 256};
     if (vecs <= 512) return {256, 2, 256};
-    if (vecs <= 1024) return {256, 4, 256};
+    if (vecs <= 1024) return per == 4 ? LnPlan{256, 4, 256} : LnPlan{512, 2, 512};
     if (vecs <= 2048) return {1024, 2, 1024};
     return {0, 0, 0};
 }
 inline int elem_bytes(int dtype) { return dtype == DMN_DT_F32 ? 4 : 2; }
-inline long long ln_vecs(int width, int dtype) { return ((long long)width * elem_bytes(dtype) + 15) / 16; }
+inline LnPlan ln_plan(int width, int dtype) { return ln_plan(((long long)width * elem_bytes(dtype) + 15) / 16, 16 / elem_bytes(dtype)); }
 
 int ln_fwd_blocks(long long rows, const LnPlan& p) {
     const long long need = p.tpr ? (rows + p.nt / p.tpr - 1) / (p.nt / p.tpr) : rows;
@@ -362,49 +365,42 @@ int ln_fwd_blocks(long long rows, const LnPlan& p) {
 }
 int ln_bwd_blocks(long long rows, const LnPlan& p) {
     const long long need = p.tpr ? (rows + p.nt / p.tpr - 1) / (p.nt / p.tpr) : (rows + 15) / 16;
-    const long long cap = p.nt == 1024 ? 256 : p.tpr == 256 ? 512 : p.tpr ? 1024 : 64;
+    const long long cap = p.nt == 1024 ? 256 : p.tpr >= 256 ? 512 : p.tpr ? 1024 : 64;
     return (int)(need < cap ? need : cap);
+}
+
+template <int A, int B, int C> struct LnShape { static constexpr int TPR = A, NV = B, NT = C; };
+// Calls f with the shape of the plan (one that ln_plan gives for the type).
+template <typename T, typename F> void ln_dispatch(const LnPlan& p, F f) {
+    auto is = [&](auto shape) {
+        if (p.tpr != shape.TPR || p.nv != shape.NV) return false;
+        f(shape);
+        return true;
+    };
+    if (is(LnShape<8, 1, 256>{}) || is(LnShape<16, 1, 256>{}) || is(LnShape<32, 1, 256>{}) || is(LnShape<64, 1, 256>{}) ||
+        is(LnShape<64, 2, 256>{}) || is(LnShape<256, 2, 256>{}) || is(LnShape<1024, 2, 1024>{}))
+        return;
+    if constexpr (Pack<T>::N == 4) (void)(is(LnShape<64, 4, 256>{}) || is(LnShape<256, 4, 256>{}));
+    else (void)(is(LnShape<256, 1, 256>{}) || is(LnShape<512, 2, 512>{}));
 }
 
 template <typename T, typename A> int ln_forward(const LnArgs& a, const LnPlan& p, hipStream_t s) {
     const int grid = ln_fwd_blocks(a.rows, p);
-#define LN_CASE(TPR_, NV_, NT_) \
-    else if (p.tpr == TPR_ && p.nv == NV_) ln_fwd_kernel<T, A, TPR_, NV_, NT_><<<grid, NT_, 0, s>>>(a)
     if (p.tpr == 0) ln_fwd_wide_kernel<T, A><<<grid, 1024, 0, s>>>(a);
-    LN_CASE(8, 1, 256);
-    LN_CASE(16, 1, 256);
-    LN_CASE(32, 1, 256);
-    LN_CASE(64, 1, 256);
-    LN_CASE(64, 2, 256);
-    LN_CASE(64, 4, 256);
-    LN_CASE(256, 2, 256);
-    LN_CASE(256, 4, 256);
-    LN_CASE(1024, 2, 1024);
-#undef LN_CASE
+    else ln_dispatch<T>(p, [&](auto h) { ln_fwd_kernel<T, A, h.TPR, h.NV, h.NT><<<grid, h.NT, 0, s>>>(a); });
     DMN_BLOCK_LAUNCH_CHECK();
     return DMN_OK;
 }
 
 template <typename T, typename A> int ln_backward(const LnArgs& a, const LnPlan& p, void* dw, void* db, hipStream_t s) {
     const int grid = ln_bwd_blocks(a.rows, p);
-    if (grid > 0) {
-#define LN_CASE(TPR_, NV_, NT_) \
-    else if (p.tpr == TPR_ && p.nv == NV_) ln_bwd_kernel<T, A, TPR_, NV_, NT_><<<grid, NT_, 0, s>>>(a)
-        if (p.tpr == 0) {
-            if (a.dx) ln_bwd_wide_kernel<T, A><<<(int)(a.rows < 512 ? a.rows : 512), 1024, 0, s>>>(a);
-            DMN_BLOCK_LAUNCH_CHECK();
-            if (a.want_params) ln_params_wide_kernel<T><<<dim3((a.width + 255) / 256, grid), 256, 0, s>>>(a);
-        }
-        LN_CASE(8, 1, 256);
-        LN_CASE(16, 1, 256);
-        LN_CASE(32, 1, 256);
-        LN_CASE(64, 1, 256);
-        LN_CASE(64, 2, 256);
-        LN_CASE(64, 4, 256);
-        LN_CASE(256, 2, 256);
-        LN_CASE(256, 4, 256);
-        LN_CASE(1024, 2, 1024);
-#undef LN_CASE
+    if (grid > 0 && p.tpr == 0) {
+        if (a.dx) ln_bwd_wide_kernel<T, A><<<(int)(a.rows < 512 ? a.rows : 512), 1024, 0, s>>>(a);
+        DMN_BLOCK_LAUNCH_CHECK();
+        if (a.want_params) ln_params_wide_kernel<T><<<dim3((a.width + 255) / 256, grid), 256, 0, s>>>(a);
+        DMN_BLOCK_LAUNCH_CHECK();
+    } else if (grid > 0) {
+        ln_dispatch<T>(p, [&](auto h) { ln_bwd_kernel<T, A, h.TPR, h.NV, h.NT><<<grid, h.NT, 0, s>>>(a); });
         DMN_BLOCK_LAUNCH_CHECK();
     }
     if (a.want_params) {
@@ -440,7 +436,7 @@ extern "C" int dmn_layer_norm_forward(const void* x, int64_t ldx, const void* we
     a.ldx = ldx;
     a.width = width;
     a.eps = eps;
-    const LnPlan p = ln_plan(ln_vecs(width, dtype));
+    const LnPlan p = ln_plan(width, dtype);
     hipStream_t s = (hipStream_t)stream;
     if (dtype == DMN_DT_F32) return ln_forward<float, float>(a, p, s);
     if (dtype == DMN_DT_BF16) return affine_dtype == dtype ? ln_forward<__bf16, __bf16>(a, p, s) : ln_forward<__bf16, float>(a, p, s);
@@ -449,7 +445,7 @@ extern "C" int dmn_layer_norm_forward(const void* x, int64_t ldx, const void* we
 
 extern "C" size_t dmn_layer_norm_workspace_bytes(int64_t rows, int width, int dtype) {
     if (rows < 0 || width <= 0 || dtype < 0 || dtype > 2) return 0;
-    return (size_t)2 * ln_bwd_blocks(rows, ln_plan(ln_vecs(width, dtype))) * width * sizeof(float) + 256;
+    return (size_t)2 * ln_bwd_blocks(rows, ln_plan(width, dtype)) * width * sizeof(float) + 256;
 }
 
 extern "C" int dmn_layer_norm_backward(const void* dy, int64_t lddy, const void* x, int64_t ldx, const void* weight,
@@ -474,7 +470,7 @@ extern "C" int dmn_layer_norm_backward(const void* dy, int64_t lddy, const void*
     DMN_REQUIRE(!a.want_params || (workspace && (uintptr_t)workspace % 16 == 0 && workspace_bytes >= dmn_layer_norm_workspace_bytes(rows, width, dtype)),
                 DMN_ERR_WORKSPACE, "dmn_layer_norm_backward: workspace of %zu bytes, %zu needed (16-byte aligned)", workspace_bytes,
                 dmn_layer_norm_workspace_bytes(rows, width, dtype));
-    const LnPlan p = ln_plan(ln_vecs(width, dtype));
+    const LnPlan p = ln_plan(width, dtype);
     hipStream_t s = (hipStream_t)stream;
     if (dtype == DMN_DT_F32) return ln_backward<float, float>(a, p, dweight, dbias, s);
     if (dtype == DMN_DT_BF16)

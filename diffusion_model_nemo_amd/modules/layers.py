@@ -27,70 +27,80 @@ def _check_tensor(t: torch.Tensor, what: str):
         raise ValueError(f"{what}: dtype must be float32, bfloat16 or float16, got {t.dtype}")
 
 
-def _check_param(p: Optional[torch.Tensor], name: str, shape, x: torch.Tensor, dtypes):
-    if p is None:
-        return
+def _check_param(p: torch.Tensor, name: str, shape, x: torch.Tensor, other=None):
+    """`p` on x's device, of `shape` and of x's type (or `other`)."""
     if p.device != x.device:
         raise RuntimeError(f"{name} on {p.device}, input on {x.device}")
-    if tuple(p.shape) != tuple(shape):
+    if p.shape != shape:
         raise ValueError(f"{name} must have shape {tuple(shape)}, got {tuple(p.shape)}")
-    if p.dtype not in dtypes:
-        raise ValueError(f"{name} must be {' or '.join(str(d) for d in dtypes)}, got {p.dtype}")
+    if p.dtype != x.dtype and p.dtype != other:
+        raise ValueError(f"{name} must be {x.dtype}{'' if other is None else f' or {other}'}, got {p.dtype}")
 
 
 def _rows(t: torch.Tensor):
     """(tensor, row stride): `t` as rows of contiguous elements, copied only where its strides do not allow that."""
     width = t.shape[-1]
-    if t.dim() == 2 and (t.stride(1) == 1 or width == 1) and (t.stride(0) >= width or t.shape[0] <= 1):
-        return t, max(t.stride(0), width)
     if t.is_contiguous():
         return t, width
+    if t.dim() == 2 and (t.stride(1) == 1 or width == 1) and t.stride(0) >= width:
+        return t, t.stride(0)
     return t.contiguous(), width
+
+
+def _empty_like(t: torch.Tensor) -> torch.Tensor:
+    return torch.empty_like(t) if t.is_contiguous() else torch.empty(t.shape, dtype=t.dtype, device=t.device)
 
 
 # ---- layer norm ------------------------------------------------------------------------------------------------------
 
-def _layer_norm_forward(x, ldx, rows, weight, bias, eps, want_stats):
+def _layer_norm_forward(x, ldx, weight, bias, eps, want_stats):
     width = x.shape[-1]
-    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    rows = x.numel() // width
+    y = _empty_like(x)
     stats = torch.empty((rows, 2), dtype=torch.float32, device=x.device) if want_stats else None
-    affine = weight if weight is not None else bias
     code = N.DTYPE_CODES[x.dtype]
-    N.launch(x.device, N.lib().dmn_layer_norm_forward, x.data_ptr(), ldx, N.ptr(weight), N.ptr(bias), y.data_ptr(), N.ptr(stats),
-             rows, width, code, code if affine is None else N.DTYPE_CODES[affine.dtype], eps)
-    return y, stats
+    affine = code if weight is bias is None else N.DTYPE_CODES[(bias if weight is None else weight).dtype]
+    N.launch(x.get_device(), N.lib().dmn_layer_norm_forward, x.data_ptr(), ldx, None if weight is None else weight.data_ptr(),
+             None if bias is None else bias.data_ptr(), y.data_ptr(), None if stats is None else stats.data_ptr(), rows, width, code,
+             affine, eps)
+    return y, stats, rows, code, affine
 
 
 class _LayerNormFunction(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, eps):
         x, ldx = _rows(x)
-        rows = x.numel() // x.shape[-1]
-        y, stats = _layer_norm_forward(x, ldx, rows, weight, bias, eps, True)
-        ctx.save_for_backward(x, weight, stats)
-        ctx.ldx = ldx
-        ctx.affine_dtype = weight.dtype if weight is not None else bias.dtype if bias is not None else x.dtype
+        y, stats, rows, code, affine = _layer_norm_forward(x, ldx, weight, bias, eps, True)
+        ctx.save_for_backward(x, weight, bias, stats)
+        ctx.plan = ldx, rows, code, affine
         return y
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, dy):
-        x, weight, stats = ctx.saved_tensors
+        # the decorator that refuses a second differentiation costs more than the work below where nobody asks for one
+        return _LayerNormFunction._once(ctx, dy) if torch.is_grad_enabled() else _LayerNormFunction._gradients(ctx, dy)
+
+    @staticmethod
+    def _gradients(ctx, dy):
+        x, weight, bias, stats = ctx.saved_tensors
+        ldx, rows, code, affine = ctx.plan
         dy, lddy = _rows(dy)
         width = x.shape[-1]
-        rows = stats.shape[0]
-        need_x, need_w, need_b = ctx.needs_input_grad[:3]
-        dx = torch.empty(x.shape, dtype=x.dtype, device=x.device) if need_x else None
-        dw = torch.empty(width, dtype=ctx.affine_dtype, device=x.device) if need_w else None
-        db = torch.empty(width, dtype=ctx.affine_dtype, device=x.device) if need_b else None
-        code, lib, ws, nbytes = N.DTYPE_CODES[x.dtype], N.lib(), None, 0
+        need_x, need_w, need_b, _ = ctx.needs_input_grad
+        dx = _empty_like(x) if need_x else None
+        dw = torch.empty_like(weight) if need_w else None
+        db = torch.empty_like(bias) if need_b else None
+        lib, ws, nbytes = N.lib(), None, 0
         if need_w or need_b:
             nbytes = lib.dmn_layer_norm_workspace_bytes(rows, width, code)
             ws = torch.empty(nbytes, dtype=torch.uint8, device=x.device)
-        N.launch(x.device, lib.dmn_layer_norm_backward, dy.data_ptr(), lddy, x.data_ptr(), ctx.ldx, N.ptr(weight),
-                 stats.data_ptr(), N.ptr(dx), N.ptr(dw), N.ptr(db), rows, width, code, N.DTYPE_CODES[ctx.affine_dtype],
-                 N.ptr(ws), nbytes)
+        N.launch(x.get_device(), lib.dmn_layer_norm_backward, dy.data_ptr(), lddy, x.data_ptr(), ldx,
+                 None if weight is None else weight.data_ptr(), stats.data_ptr(), None if dx is None else dx.data_ptr(),
+                 None if dw is None else dw.data_ptr(), None if db is None else db.data_ptr(), rows, width, code, affine,
+                 None if ws is None else ws.data_ptr(), nbytes)
         return dx, dw, db, None
+
+    _once = staticmethod(once_differentiable(_gradients.__func__))
 
 
 def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Optional[torch.Tensor] = None,
@@ -101,21 +111,21 @@ def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Opt
     _check_tensor(x, "layer_norm")
     if x.dim() == 0 or x.shape[-1] == 0:
         raise ValueError("layer_norm needs a last axis of at least one element")
-    width = x.shape[-1]
-    _check_param(weight, "weight", (width,), x, (x.dtype, torch.float32))
-    _check_param(bias, "bias", (width,), x, (x.dtype, torch.float32))
-    if weight is not None and bias is not None and weight.dtype != bias.dtype:
-        raise ValueError(f"weight and bias must have one type, got {weight.dtype} and {bias.dtype}")
-    eps = float(eps)
     if not eps >= 0.0:
         raise ValueError(f"eps must be >= 0, got {eps}")
-    weight = weight if weight is None else weight.contiguous()
-    bias = bias if bias is None else bias.contiguous()
-    if torch.is_grad_enabled() and (x.requires_grad or (weight is not None and weight.requires_grad)
-                                    or (bias is not None and bias.requires_grad)):
+    shape, grad = x.shape[-1:], x.requires_grad
+    if weight is not None:
+        _check_param(weight, "weight", shape, x, torch.float32)
+        weight, grad = weight.contiguous(), grad or weight.requires_grad
+    if bias is not None:
+        _check_param(bias, "bias", shape, x, torch.float32)
+        if weight is not None and weight.dtype != bias.dtype:
+            raise ValueError(f"weight and bias must have one type, got {weight.dtype} and {bias.dtype}")
+        bias, grad = bias.contiguous(), grad or bias.requires_grad
+    if grad and torch.is_grad_enabled():
         return _LayerNormFunction.apply(x, weight, bias, eps)
     x, ldx = _rows(x)
-    return _layer_norm_forward(x, ldx, x.numel() // width, weight, bias, eps, False)[0]
+    return _layer_norm_forward(x, ldx, weight, bias, eps, False)[0]
 
 
 class LayerNorm(nn.Module):
@@ -141,55 +151,60 @@ class LayerNorm(nn.Module):
 ACTIVATIONS = {None: 0, "relu": 1, "silu": 2, "gelu": 3}
 
 
-def _workspace(nbytes: int, device) -> Optional[torch.Tensor]:
-    return torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
-
-
-def _linear_forward(x, ldx, weight, bias, residual, ldr, code, want_z):
+def _linear_forward(x, ldx, weight, bias, residual, ldr, activation, want_z):
     out, width = weight.shape
     rows = x.numel() // width
     y = torch.empty(x.shape[:-1] + (out,), dtype=x.dtype, device=x.device)
-    z = torch.empty((rows, out), dtype=x.dtype, device=x.device) if want_z else None
-    lib, dt = N.lib(), N.DTYPE_CODES[x.dtype]
-    nbytes = lib.dmn_linear_forward_workspace_bytes(rows, width, out, dt)
-    ws = _workspace(nbytes, x.device)
-    N.launch(x.device, lib.dmn_linear_forward, x.data_ptr(), ldx, weight.data_ptr(), N.ptr(bias), N.ptr(residual), ldr, y.data_ptr(),
-             N.ptr(z), rows, width, out, code, dt, N.ptr(ws), nbytes)
-    return y, z
+    z = torch.empty_like(y) if want_z else None
+    lib, code = N.lib(), N.DTYPE_CODES[x.dtype]
+    nbytes = lib.dmn_linear_forward_workspace_bytes(rows, width, out, code)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=x.device) if nbytes else None
+    N.launch(x.get_device(), lib.dmn_linear_forward, x.data_ptr(), ldx, weight.data_ptr(), None if bias is None else bias.data_ptr(),
+             None if residual is None else residual.data_ptr(), ldr, y.data_ptr(), None if z is None else z.data_ptr(), rows, width,
+             out, activation, code, None if ws is None else ws.data_ptr(), nbytes)
+    return y, z, rows, code
 
 
 class _LinearFunction(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, weight, bias, residual, code):
+    def forward(ctx, x, weight, bias, residual, activation):
         x, ldx = _rows(x)
         ldr = 0
         if residual is not None:
             residual, ldr = _rows(residual)
         # the value in front of the activation is all the backward needs of the forward's results
-        y, z = _linear_forward(x, ldx, weight, bias, residual, ldr, code, code != 0 and any(ctx.needs_input_grad[:3]))
-        ctx.save_for_backward(x, weight, z)
-        ctx.ldx, ctx.code = ldx, code
+        y, z, rows, code = _linear_forward(x, ldx, weight, bias, residual, ldr, activation,
+                                           activation != 0 and any(ctx.needs_input_grad[:3]))
+        ctx.save_for_backward(x, weight, bias, z)
+        ctx.plan = ldx, rows, code, activation
         return y
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, dy):
-        x, weight, z = ctx.saved_tensors
-        need_x, need_w, need_b, need_r = ctx.needs_input_grad[:4]
+        return _LinearFunction._once(ctx, dy) if torch.is_grad_enabled() else _LinearFunction._gradients(ctx, dy)
+
+    @staticmethod
+    def _gradients(ctx, dy):
+        x, weight, bias, z = ctx.saved_tensors
+        ldx, rows, code, activation = ctx.plan
+        need_x, need_w, need_b, need_r, _ = ctx.needs_input_grad
         dx = dw = db = None
         if need_x or need_w or need_b:
             rows_dy, lddy = _rows(dy)
             out, width = weight.shape
-            rows = x.numel() // width
-            dx = torch.empty(x.shape, dtype=x.dtype, device=x.device) if need_x else None
-            dw = torch.empty((out, width), dtype=x.dtype, device=x.device) if need_w else None
-            db = torch.empty(out, dtype=x.dtype, device=x.device) if need_b else None
-            lib, dt = N.lib(), N.DTYPE_CODES[x.dtype]
-            nbytes = lib.dmn_linear_backward_workspace_bytes(rows, width, out, ctx.code, dt)
-            ws = _workspace(nbytes, x.device)
-            N.launch(x.device, lib.dmn_linear_backward, rows_dy.data_ptr(), lddy, x.data_ptr(), ctx.ldx, weight.data_ptr(), N.ptr(z),
-                     N.ptr(dx), N.ptr(dw), N.ptr(db), rows, width, out, ctx.code, dt, N.ptr(ws), nbytes)
+            dx = _empty_like(x) if need_x else None
+            dw = torch.empty_like(weight) if need_w else None
+            db = torch.empty_like(bias) if need_b else None
+            lib = N.lib()
+            nbytes = lib.dmn_linear_backward_workspace_bytes(rows, width, out, activation, code)
+            ws = torch.empty(nbytes, dtype=torch.uint8, device=x.device) if nbytes else None
+            N.launch(x.get_device(), lib.dmn_linear_backward, rows_dy.data_ptr(), lddy, x.data_ptr(), ldx, weight.data_ptr(),
+                     None if z is None else z.data_ptr(), None if dx is None else dx.data_ptr(), None if dw is None else dw.data_ptr(),
+                     None if db is None else db.data_ptr(), rows, width, out, activation, code, None if ws is None else ws.data_ptr(),
+                     nbytes)
         return dx, dw, db, dy if need_r else None, None
+
+    _once = staticmethod(once_differentiable(_gradients.__func__))
 
 
 def linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] = None, activation: Optional[str] = None,
@@ -205,15 +220,18 @@ def linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] =
     out, width = weight.shape
     if x.dim() == 0 or x.shape[-1] != width:
         raise ValueError(f"expected a last axis of {width}, got {tuple(x.shape)}")
-    if activation not in ACTIVATIONS:
+    code = ACTIVATIONS.get(activation)
+    if code is None:
         raise ValueError(f"activation must be one of {list(ACTIVATIONS)}, got {activation!r}")
-    _check_param(weight, "weight", (out, width), x, (x.dtype,))
-    _check_param(bias, "bias", (out,), x, (x.dtype,))
-    _check_param(residual, "residual", x.shape[:-1] + (out,), x, (x.dtype,))
-    weight = weight.contiguous()
-    bias = bias if bias is None else bias.contiguous()
-    code = ACTIVATIONS[activation]
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, bias, residual)):
+    _check_param(weight, "weight", weight.shape, x)
+    weight, grad = weight.contiguous(), x.requires_grad or weight.requires_grad
+    if bias is not None:
+        _check_param(bias, "bias", (out,), x)
+        bias, grad = bias.contiguous(), grad or bias.requires_grad
+    if residual is not None:
+        _check_param(residual, "residual", x.shape[:-1] + (out,), x)
+        grad = grad or residual.requires_grad
+    if grad and torch.is_grad_enabled():
         return _LinearFunction.apply(x, weight, bias, residual, code)
     x, ldx = _rows(x)
     ldr = 0

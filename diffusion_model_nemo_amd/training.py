@@ -228,6 +228,21 @@ class UnetTrainer:
         self.unet._weights_version = None   # the sampling handle repacks from the updated parameters
 
 
+def _refuse_shared_memory(scattered: Sequence[torch.Tensor], every: Sequence[torch.Tensor]):
+    """Raises if an element of a scattered tensor is also another of its elements or one of another tensor: it would not be
+    clear how often it is scaled. (Tensors without gaps are checked by their address ranges in the library.)"""
+    for base in {t.untyped_storage().data_ptr(): t for t in scattered}.values():
+        mates = [t for t in every if t.untyped_storage().data_ptr() == base.untyped_storage().data_ptr()]
+        seen = torch.zeros(base.untyped_storage().nbytes() // base.element_size(), dtype=torch.uint8)
+        for t in mates:
+            if t.dtype == base.dtype and all(st > 0 or sz <= 1 for st, sz in zip(t.stride(), t.shape)):
+                seen.as_strided(t.shape, t.stride(), t.storage_offset()).add_(1)
+            else:
+                seen.fill_(2)
+        if bool((seen > 1).any()):
+            raise ValueError("a gradient shares memory with another one, or with itself (an expanded tensor)")
+
+
 def _dense(t: torch.Tensor) -> bool:
     """Whether `t` covers its memory without gaps or overlaps, in whatever order of its axes."""
     if t.is_contiguous():
@@ -273,24 +288,28 @@ def clip_grad_norm_(parameters: Union[torch.Tensor, Iterable[torch.Tensor]], max
     grads = [g for g in grads if g is not None]
     if not grads:
         return torch.zeros(())
-    dev = grads[0].device
+    # a few hundred gradients: every look-up runs over all of them at once, and only what is out of the ordinary one by one
+    dev, dtypes = grads[0].device, {g.dtype for g in grads}
     if dev.type != "cuda":
         raise RuntimeError("clip_grad_norm_ runs only on MI355X device tensors (no CPU implementation)")
+    if len(set(map(torch.Tensor.get_device, grads))) != 1:
+        raise RuntimeError("the gradients must all be on one device")
+    if not all(t in N.DTYPE_CODES for t in dtypes):
+        raise ValueError(f"gradients must be float32, bfloat16 or float16, got {sorted(map(str, dtypes))}")
     copied = []   # (gradient, its dense copy): scattered gradients are clipped in a copy and written back
-    for i, g in enumerate(grads):
-        if g.device != dev:
-            raise RuntimeError(f"gradients on {dev} and {g.device}: all must be on one device")
-        if g.layout != torch.strided or g.dtype not in N.DTYPE_CODES:
-            raise ValueError(f"gradients must be dense float32, bfloat16 or float16 tensors, got {g.dtype} ({g.layout})")
-        if not g.is_contiguous() and (out is not None or not _dense(g)):
-            if out is None and any(st == 0 and sz > 1 for st, sz in zip(g.stride(), g.shape)):
-                raise ValueError("a gradient is an expanded tensor: several of its elements are one place in memory")
-            grads[i] = g.contiguous()
-            copied.append((g, grads[i]))
+    if not all(map(torch.Tensor.is_contiguous, grads)):
+        for i, g in enumerate(grads):
+            if g.layout != torch.strided:
+                raise ValueError(f"gradients must be dense tensors, got one of layout {g.layout}")
+            if not g.is_contiguous() and (out is not None or not _dense(g)):
+                copied.append((g, g.contiguous()))
+                grads[i] = copied[-1][1]
+        if out is None and copied:
+            _refuse_shared_memory([g for g, _ in copied], [p.grad for p in params if p.grad is not None])
     table = np.empty((len(grads), 4), dtype=np.int64)   # DmnGradTensor: src, dst, numel, types
-    table[:, 0] = [g.data_ptr() for g in grads]
-    table[:, 2] = [g.numel() for g in grads]
-    table[:, 3] = [N.DTYPE_CODES[g.dtype] for g in grads]
+    table[:, 0] = list(map(torch.Tensor.data_ptr, grads))
+    table[:, 2] = list(map(torch.Tensor.numel, grads))
+    table[:, 3] = N.DTYPE_CODES[grads[0].dtype] if len(dtypes) == 1 else [N.DTYPE_CODES[g.dtype] for g in grads]
     if out is None:
         table[:, 1] = table[:, 0]
         table[:, 3] *= (1 << 32) + 1
@@ -299,7 +318,7 @@ def clip_grad_norm_(parameters: Union[torch.Tensor, Iterable[torch.Tensor]], max
             if o.device != dev or o.shape != g.shape or o.dtype not in N.DTYPE_CODES or not o.is_contiguous():
                 raise ValueError("out must hold contiguous float32 / bfloat16 / float16 tensors of the gradients' shapes, on "
                                  "their device")
-        table[:, 1] = [o.data_ptr() for o in out]
+        table[:, 1] = list(map(torch.Tensor.data_ptr, out))
         table[:, 3] += np.array([N.DTYPE_CODES[o.dtype] for o in out], dtype=np.int64) << 32
     lib = N.lib()
     nbytes = lib.dmn_clip_grads_workspace_bytes(len(grads))
@@ -307,7 +326,7 @@ def clip_grad_norm_(parameters: Union[torch.Tensor, Iterable[torch.Tensor]], max
     norm = torch.empty((), dtype=torch.float32, device=dev)
 
     def call(rows):
-        N.launch(dev, lib.dmn_clip_grads, rows.ctypes.data, len(rows), int(norm_type != 2.0), max_norm, grad_scale,
+        N.launch(grads[0].get_device(), lib.dmn_clip_grads, rows.ctypes.data, len(rows), int(norm_type != 2.0), max_norm, grad_scale,
                  norm.data_ptr(), ws.data_ptr(), nbytes)
 
     if error_if_nonfinite:

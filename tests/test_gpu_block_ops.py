@@ -603,6 +603,10 @@ def test_clip_refuses_overlaps_and_bad_arguments():
     for grads in ([g, g], [g[:60], g[59:]], [g[10:20], g]):
         with pytest.raises(DmnError, match="overlaps"):
             clip_grad_norm_(params_with(grads), 1.0)
+    square = g.view(10, 10)
+    for grads in ([square[:, :5], square[:, :5]], [square[:, :5], square[:, 4:]], [square[:, :5], g]):   # scattered ones too
+        with pytest.raises(ValueError, match="shares memory"):
+            clip_grad_norm_(params_with(grads), 1.0)
     out = torch.zeros(100, device="cuda")
     with pytest.raises(DmnError, match="overlaps"):
         clip_grad_norm_(params_with([g, g]), 1.0, out=[out, out])
