@@ -84,9 +84,9 @@ SIGNATURES = {
     "dmn_layer_norm_forward": (_i, [_vp, _i64, _vp, _vp, _vp, _vp, _i64, _i, _i, _i, _f, _vp]),
     "dmn_layer_norm_workspace_bytes": (_sz, [_i64, _i, _i]),
     "dmn_layer_norm_backward": (_i, [_vp, _i64, _vp, _i64, _vp, _vp, _vp, _vp, _vp, _i64, _i, _i, _i, _vp, _sz, _vp]),
-    "dmn_linear_forward_workspace_bytes": (_sz, [_i64, _i, _i, _i]),
+    "dmn_linear_forward_workspace_bytes": (_sz, [_vp, _i64, _vp, _i64, _i, _i, _i]),
     "dmn_linear_forward": (_i, [_vp, _i64, _vp, _vp, _vp, _i64, _vp, _vp, _i64, _i, _i, _i, _i, _vp, _sz, _vp]),
-    "dmn_linear_backward_workspace_bytes": (_sz, [_i64, _i, _i, _i, _i]),
+    "dmn_linear_backward_workspace_bytes": (_sz, [_vp, _i64, _vp, _i64, _vp, _i64, _i, _i, _i, _i]),
     "dmn_linear_backward": (_i, [_vp, _i64, _vp, _i64, _vp, _vp, _vp, _vp, _vp, _i64, _i, _i, _i, _i, _vp, _sz, _vp]),
     "dmn_clip_grads_workspace_bytes": (_sz, [_i]),
     "dmn_clip_grads": (_i, [_vp, _i, _i, _f, _f, _vp, _vp, _sz, _vp]),

@@ -50,10 +50,11 @@ template <typename T> __device__ __forceinline__ float normal_cdf(float z, float
     const float tail = normal_tail_scaled<T>(fabsf(z)) * e;
     return z < 0.f ? tail : 1.0f - tail;
 }
+__device__ __forceinline__ float normal_bell(float z) { return __builtin_amdgcn_exp2f(-0.72134752f * z * z); }   // exp(-z^2 / 2)
 // z Phi(z) as max(z, 0) - |z| Phi(-|z|): no cancellation, a NaN stays (through exp), and infinities give their limits (the
 // factor |z| is held at 40, where Phi(-|z|) is zero in float32).
 template <typename T> __device__ __forceinline__ float gelu(float z) {
-    const float az = fminf(fabsf(z), 40.f), e = __expf(-0.5f * z * z);
+    const float az = fminf(fabsf(z), 40.f), e = normal_bell(z);
     return __builtin_fmaf(-az, normal_tail_scaled<T>(az) * e, fmaxf(z, 0.f));
 }
 template <typename T> __device__ __forceinline__ float activate(float z, int act) {
@@ -69,7 +70,7 @@ template <typename T> __device__ __forceinline__ float act_backward(float dy, fl
         return dy * (s * __builtin_fmaf(z, 1.0f - s, 1.0f));
     }
     if (act == ACT_GELU) {
-        const float e = __expf(-0.5f * z * z);
+        const float e = normal_bell(z);
         return dy * __builtin_fmaf(z * 0.3989422804014327f, e, normal_cdf<T>(z, e));
     }
     return dy;
@@ -168,41 +169,6 @@ template <typename T, bool X, int R, int KB> struct Tile {
 };
 
 
-// Staging of one operand through registers, for any alignment: `R` m/n rows from r0, k from k0. Elements outside the matrix
-// become zero.
-template <typename T, bool X, int R, int NT, int KB> struct Stager {
-    typedef Tile<T, X, R, KB> Tl;
-    static constexpr int PER = Tl::CHUNKS / NT;
-    static_assert(Tl::CHUNKS % NT == 0, "whole chunks per thread");
-    const T* base;
-    long long ld;
-    int extent, K;                // extent of m/n, of k
-    typename Pack<T>::vec reg[PER];
-
-    __device__ __forceinline__ void init(const void* p, long long ld_, int r0, int extent_, int K_) {
-        ld = ld_;
-        extent = extent_ - r0;
-        K = K_;
-        base = (const T*)p + (X ? (long long)r0 : (long long)r0 * ld_);
-    }
-    __device__ __forceinline__ void fetch(int k0) {
-#pragma unroll
-        for (int i = 0; i < PER; ++i) {
-            int k, r;
-            Tl::place(i * NT + threadIdx.x, k, r);
-            typename Pack<T>::vec v;
-#pragma unroll
-            for (int j = 0; j < Pack<T>::N; ++j) v[j] = (T)0.f;
-            if (k0 + k < K && r < extent) v = X ? load16_tail(base + (long long)(k0 + k) * ld, r, extent) : load16_tail(base + r * ld, k0 + k, K);
-            reg[i] = v;
-        }
-    }
-    __device__ __forceinline__ void commit(char* lds) {
-#pragma unroll
-        for (int i = 0; i < PER; ++i) *(typename Pack<T>::vec*)(lds + (i * NT + threadIdx.x) * 16) = reg[i];
-    }
-};
-
 constexpr unsigned kOutOfRange = 0x80000000u;   // byte offset behind every buffer: such a load gives zero
 
 // 16 bytes per lane from a buffer to LDS, lane l's at dst + 16 l. As assembly, because behind the builtin the compiler
@@ -216,8 +182,9 @@ __device__ __forceinline__ void load_to_lds(u32x4 rsrc, unsigned offset, unsigne
 __device__ __forceinline__ unsigned lds_address(const char* p) { return (unsigned)(uintptr_t)(__attribute__((address_space(3))) const char*)p; }
 
 // Staging of one operand from memory to LDS without registers, in 16-byte pieces through a buffer descriptor whose range
-// check supplies the zeros outside the matrix. Base, row stride and the contiguous extent are multiples of 16 bytes.
-template <typename T, bool X, int R, int NT, int KB> struct DirectStager {
+// check supplies the zeros outside the matrix. Base and row stride are multiples of 16 bytes; where a row ends inside a
+// piece, the rest of the piece is there and, along k, holds zeros (pad_copy_kernel).
+template <typename T, bool X, int R, int NT, int KB> struct Stager {
     typedef Tile<T, X, R, KB> Tl;
     static constexpr int PER = Tl::CHUNKS / NT;
     static_assert(Tl::CHUNKS % NT == 0, "whole chunks per thread");
@@ -349,79 +316,20 @@ __device__ __forceinline__ void tile_of(int b, int tm, int tn, int& im, int& in)
     in = (t % band) / rows;
 }
 
-// The product for operands on any alignment: one tile is multiplied while the next is on its way to registers.
-template <typename T, bool XA, bool XB, int BM, int BN, int WM, int WN>
-__global__ __launch_bounds__((BM / WM) * (BN / WN) * 64) void gemm_kernel(const GemmArgs g) {
-    constexpr int NT = (BM / WM) * (BN / WN) * 64, KB = 128;
-    typedef Tile<T, XA, BM, KB> TA;
-    typedef Tile<T, XB, BN, KB> TB;
-    typedef typename Frag<T>::type frag;
-    constexpr int BK = TA::BK, A_BYTES = BM * KB, B_BYTES = BN * KB, FM = WM / 16, FN = WN / 16;
-    extern __shared__ __attribute__((aligned(16))) char lds[];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int wm = wave % (BM / WM) * WM, wn = wave / (BM / WM) * WN;
-    int im, in;
-    tile_of(blockIdx.x, (g.M + BM - 1) / BM, (g.N + BN - 1) / BN, im, in);
-    const int m0 = im * BM, n0 = in * BN;
-    const int k_tiles = (g.K + BK - 1) / BK, t0 = blockIdx.y * g.tiles_per_split;
-    const int t1 = t0 + g.tiles_per_split < k_tiles ? t0 + g.tiles_per_split : k_tiles;
-    Stager<T, XA, BM, NT, KB> sa;
-    Stager<T, XB, BN, NT, KB> sb;
-    sa.init(g.a, g.lda, m0, g.M, g.K);
-    sb.init(g.b, g.ldb, n0, g.N, g.K);
-    f32x4 acc[FM][FN];
-#pragma unroll
-    for (int i = 0; i < FM; ++i)
-#pragma unroll
-        for (int j = 0; j < FN; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
-    sa.fetch(t0 * BK);
-    sb.fetch(t0 * BK);
-    sa.commit(lds);
-    sb.commit(lds + A_BYTES);
-    for (int t = t0; t < t1; ++t) {
-        __syncthreads();   // this tile has arrived, and nobody reads the other buffer any more
-        char* cur = lds + ((t - t0) & 1) * (A_BYTES + B_BYTES);
-        char* nxt = lds + ((t - t0 + 1) & 1) * (A_BYTES + B_BYTES);
-        if (t + 1 < t1) {
-            sa.fetch((t + 1) * BK);
-            sb.fetch((t + 1) * BK);
-        }
-#pragma unroll
-        for (int s = 0; s < BK / Frag<T>::KSTEP; ++s) {
-            frag fa[FM], fb[FN];
-#pragma unroll
-            for (int i = 0; i < FM; ++i) fa[i] = TA::read(cur, wm + i * 16, s, lane);
-#pragma unroll
-            for (int j = 0; j < FN; ++j) fb[j] = TB::read(cur + A_BYTES, wn + j * 16, s, lane);
-#pragma unroll
-            for (int i = 0; i < FM; ++i)
-#pragma unroll
-                for (int j = 0; j < FN; ++j) Frag<T>::mma(fb[j], fa[i], acc[i][j]);
-        }
-        if (t + 1 < t1) {
-            sa.commit(nxt);
-            sb.commit(nxt + A_BYTES);
-        }
-    }
-    __syncthreads();   // the tiles' memory is free
-    store_tile<T, !XB, FM, FN>(g, acc, m0 + wm, n0 + wn, lds);
-}
-
 template <int N> struct Int { static constexpr int value = N; };
 
-// The product for operands on 16-byte boundaries. S tiles of 128 bytes of k go round in LDS, each worked off in two steps;
-// the fragments of the next step come out of LDS while the matrix cores work on the present one's, which are in
-// registers. One barrier per tile, in front of its second step: behind it the tile's fragments of every wave are in
-// registers, so that the request for the tile S further on may take its place, and the next tile has arrived (each wave has
-// waited for its own part of it). Requests go on behind the last tile (they read nothing and give zeros), so that the count
-// of outstanding ones is the same for every tile.
+// The product. S tiles of 128 bytes of k go round in LDS, each worked off in two steps; the fragments of the next step come out
+// of LDS while the matrix cores work on the present one's, which are in registers. One barrier per tile, in front of its
+// second step: behind it the tile's fragments of every wave are in registers, so that the request for the tile S further on
+// may take its place, and the next tile has arrived (each wave has waited for its own part of it). Requests go on behind the
+// last tile (they read nothing and give zeros), so that the count of outstanding ones is the same for every tile.
 template <typename T, bool XA, bool XB, int BM, int BN, int WM, int WN, int S>
 __global__ __launch_bounds__((BM / WM) * (BN / WN) * 64) void gemm_pipe_kernel(const GemmArgs g) {
     constexpr int NT = (BM / WM) * (BN / WN) * 64, KB = 128;
     typedef Tile<T, XA, BM, KB> TA;
     typedef Tile<T, XB, BN, KB> TB;
-    typedef DirectStager<T, XA, BM, NT, KB> SA;
-    typedef DirectStager<T, XB, BN, NT, KB> SB;
+    typedef Stager<T, XA, BM, NT, KB> SA;
+    typedef Stager<T, XB, BN, NT, KB> SB;
     typedef typename Frag<T>::type frag;
     constexpr int BK = TA::BK, A_BYTES = BM * KB, STAGE = (BM + BN) * KB, FM = WM / 16, FN = WN / 16;
     constexpr int WAIT = (S - 2) * (SA::PER + SB::PER);
@@ -595,18 +503,22 @@ template <typename T, int MF, int NF, int WAVES> __global__ __launch_bounds__(WA
     }
 }
 
-// Joins the partial products of the k ranges in their order and runs the epilogue.
-template <typename T> __global__ __launch_bounds__(256) void gemm_join_kernel(const GemmArgs g) {
-    constexpr int V = Pack<T>::N;
-    const int pieces = (g.N + V - 1) / V;
-    const long long total = (long long)g.M * pieces, stride = (long long)g.M * g.N;
-    for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < total; i += (long long)gridDim.x * 256) {
-        const int m = (int)(i / pieces), n = (int)(i % pieces) * V;
-        const float* p = g.part + (long long)m * g.N;
-        float v[V];
+// Joins the partial products of the k ranges and runs the epilogue: 256 / G pieces of a row per workgroup, G threads per piece
+// that add every G-th range each and meet in LDS, in a fixed order.
+template <typename T, int G> __global__ __launch_bounds__(256) void gemm_join_kernel(const GemmArgs g) {
+    constexpr int V = Pack<T>::N, P = 256 / G;
+    __shared__ float sh[G > 1 ? 256 * (V + 1) : 1];
+    const int pieces = (g.N + V - 1) / V, group = threadIdx.x / P;
+    const long long i = (long long)blockIdx.x * P + threadIdx.x % P, stride = (long long)g.M * g.N;
+    const bool in = i < (long long)g.M * pieces;
+    const int m = in ? (int)(i / pieces) : 0, n = in ? (int)(i % pieces) * V : 0;
+    float v[V];
 #pragma unroll
-        for (int e = 0; e < V; ++e) v[e] = 0.f;
-        for (int s = 0; s < g.splits; ++s, p += stride) {
+    for (int e = 0; e < V; ++e) v[e] = 0.f;
+    if (in) {
+        const float* p = g.part + (long long)m * g.N + group * stride;
+#pragma unroll 4
+        for (int s = group; s < g.splits; s += G, p += G * stride) {
 #pragma unroll
             for (int e = 0; e < V; e += 4)
                 if (n + e < g.N) {
@@ -615,10 +527,21 @@ template <typename T> __global__ __launch_bounds__(256) void gemm_join_kernel(co
                     for (int k = 0; k < 4; ++k) v[e + k] += w[k];
                 }
         }
-        float bias[V];
-        load_bias<T>(g, n, bias);
-        epilogue<T, true>(g, m, n, v, bias, g.act);
     }
+    if constexpr (G > 1) {
+#pragma unroll
+        for (int e = 0; e < V; ++e) sh[threadIdx.x * (V + 1) + e] = v[e];
+        __syncthreads();
+        if (group) return;
+#pragma unroll
+        for (int s = 1; s < G; ++s)
+#pragma unroll
+            for (int e = 0; e < V; ++e) v[e] += sh[(threadIdx.x + s * P) * (V + 1) + e];
+    }
+    if (!in) return;
+    float bias[V];
+    load_bias<T>(g, n, bias);
+    epilogue<T, true>(g, m, n, v, bias, g.act);
 }
 
 // ---- what stands in front of the backward's products ------------------------------------------------------------------
@@ -627,7 +550,8 @@ template <typename T> __global__ __launch_bounds__(256) void gemm_join_kernel(co
 struct DzArgs {
     const void *dy, *z;
     long long lddy;
-    void* dz;             // null: only the column sums of dy
+    void* dz;             // [M][lddz], the rows' padding zero; null: only the column sums
+    long long lddz;
     float* part;          // [gridDim.y][N] or null
     int M, N, act;
 };
@@ -642,7 +566,7 @@ template <typename T> __global__ __launch_bounds__(256) void dz_kernel(const DzA
     if (n < a.N) {
         for (int m = m0 + r; m < m1; m += 16) {
             auto v = load16_tail((const T*)a.dy + (long long)m * a.lddy, n, a.N);
-            if (a.dz) {
+            if (a.act != ACT_NONE) {
                 const auto z = load16_tail((const T*)a.z + (long long)m * a.N, n, a.N);
 #pragma unroll
                 for (int i = 0; i < V; ++i) {
@@ -650,7 +574,7 @@ template <typename T> __global__ __launch_bounds__(256) void dz_kernel(const DzA
                     sum[i] += d;
                     v[i] = (T)d;
                 }
-                store16_tail((T*)a.dz + (long long)m * a.N, n, a.N, v);
+                if (a.dz) store16((T*)a.dz + (long long)m * a.lddz + n, v);   // behind the row's end dy and z read as zero, dz is
             } else {
 #pragma unroll
                 for (int i = 0; i < V; ++i) sum[i] += (float)v[i];
@@ -692,37 +616,68 @@ template <typename T> __global__ __launch_bounds__(256) void zero_kernel(T* p, l
     for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < n; i += (long long)gridDim.x * 256) p[i] = (T)0.f;
 }
 
+// Copies of operands whose rows do not lie on 16-byte boundaries, rows padded with zeros to whole 16-byte pieces: the copy
+// moves each element twice, where reading it unaligned into the tiles cost the products half of their rate and more
+// (8191 x 2047 x 8191 bf16: 613 to 961 us).
+struct CopyJob {
+    const void* src;
+    void* dst;
+    long long ld;
+    int rows, width, pitch;   // of src, in elements; of dst: rows x pitch
+};
+struct CopyArgs {
+    CopyJob job[3];
+};
+template <typename T> __global__ __launch_bounds__(256) void pad_copy_kernel(const CopyArgs a) {
+    constexpr int V = Pack<T>::N;
+    const CopyJob& j = a.job[blockIdx.y];
+    const int pieces = j.pitch / V;
+    const long long total = (long long)j.rows * pieces;
+    for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < total; i += (long long)gridDim.x * 256) {
+        const long long row = total < 0x7fffffff ? (int)i / pieces : i / pieces;
+        const int at = (int)(i - row * pieces) * V;
+        store16((T*)j.dst + row * j.pitch + at, load16_tail((const T*)j.src + row * j.ld, at, j.width));
+    }
+}
+
 // ---- host side ---------------------------------------------------------------------------------------------------------
 inline int elem(int dtype) { return dtype == DMN_DT_F32 ? 4 : 2; }
 inline long long ceil_div(long long a, long long b) { return (a + b - 1) / b; }
 
-// Tile and k split of a product, from its sizes and type alone, by the time that the tiles were measured to take (MI355X, us):
-// `step` for 128 bytes of k when every CU has one, `least` for one that has its CU to itself, `ends` for what stands
-// around the steps (first request, epilogue, launch). Where there are fewer tiles than CUs, k is split: the partial products
-// are written and read again at some 4 TB/s, in one more launch.
+// Tile and k split of a product, from its sizes and type alone, by the times that the tiles were measured to take (MI355X, us):
+// `step` per 128 bytes of k and tile of a CU that works through several, `least` for a tile that is alone on its CU, `ends`
+// for what stands around the steps (first requests, epilogue, launch); `together` tiles share a CU. The large tile moves the
+// fewest bytes per product (8192^3 bf16: 820 us; 128 x 128: 1100, 64 x 64: 1520), the others leave fewer CUs without work:
+// 4096 x 1024 out of k = 4096 takes 94 us in 64 large tiles and 37 us in 256 tiles of 128 x 128 with four stages each, which
+// two stages and two tiles per CU turn into 47 us; with 1024 such tiles it is the other way round (52 against 38 us).
+// Where there are too few tiles for the CUs, k is split: the partial products are written and read again at some 4 TB/s, in
+// one more launch.
 struct GemmPlan {
     int tile, splits, per;   // index into kTiles; k tiles are counted in 128 bytes of k
 };
 struct TileShape {
-    int bm, bn;
+    int bm, bn, together;
     double step16, least16, step32, least32, ends;
 };
-const TileShape kTiles[3] = {{256, 256, 1.60, 1.12, 7.5, 7.2, 8.0}, {128, 128, 0.56, 0.45, 2.0, 1.9, 4.0}, {64, 64, 0.22, 0.28, 0.50, 0.55, 3.0}};
+const TileShape kTiles[4] = {{256, 256, 1, 1.60, 1.12, 7.4, 7.2, 8.0},
+                             {128, 128, 1, 0.56, 0.45, 2.0, 1.9, 4.0},
+                             {128, 128, 2, 0.50, 0.68, 1.9, 2.0, 4.0},
+                             {64, 64, 4, 0.22, 0.28, 0.50, 0.55, 3.0}};
 
 GemmPlan gemm_plan(int M, int N, int K, int dtype) {
     const int bk = 128 / elem(dtype);
     const long long kt = ceil_div(K, bk);
-    GemmPlan best{2, 1, (int)kt};
+    GemmPlan best{3, 1, (int)kt};
     double best_us = 1e30;
-    for (int i = 0; i < 3; ++i) {
+    for (int i = 0; i < 4; ++i) {
         const TileShape& t = kTiles[i];
         const double step = dtype == DMN_DT_F32 ? t.step32 : t.step16, least = dtype == DMN_DT_F32 ? t.least32 : t.least16;
         const long long tiles = ceil_div(M, t.bm) * ceil_div(N, t.bn);
         for (int splits = 1; splits <= 64; splits *= 2) {
             if (splits > 1 && kt / splits < 4) break;
-            const long long per = ceil_div(kt, splits), rounds = ceil_div(tiles * splits, 256);
-            const double all = tiles * splits > 128 ? rounds * per * step : 0, one = per * least;
-            double us = (all > one ? all : one) + t.ends * (i == 2 ? 1 : rounds);
+            const long long per = ceil_div(kt, splits), on_cu = ceil_div(tiles * splits, 256);
+            const double all = tiles * splits > 128 ? on_cu * per * step : 0, one = per * least;
+            double us = (all > one ? all : one) + t.ends * ceil_div(on_cu, t.together);
             if (splits > 1) us += 3.0 + (double)splits * M * N * 8 / 4e6;
             if (us < best_us) {
                 best_us = us;
@@ -737,10 +692,40 @@ size_t gemm_workspace(int M, int N, int K, int dtype) {
     return p.splits > 1 ? block_align256((size_t)p.splits * M * N * sizeof(float)) : 0;
 }
 
-// 16-byte pieces of the operand can be addressed one by one
-bool direct_ok(const void* p, long long ld, bool x, int rows, int K, int dtype) {
+// An operand in memory: rows of `width` elements, `ld` apart.
+struct Operand {
+    const void* p;
+    long long ld;
+    int rows, width;
+};
+int padded(int width, int dtype) { return (int)ceil_div(width, 16 / elem(dtype)) * (16 / elem(dtype)); }
+// Bytes of the copy that the products need of it: none where its rows are whole 16-byte pieces.
+size_t copy_bytes(const Operand& o, int dtype) {
     const int e = elem(dtype);
-    return (uintptr_t)p % 16 == 0 && ld * e % 16 == 0 && (long long)(x ? rows : K) * e % 16 == 0;
+    if ((uintptr_t)o.p % 16 == 0 && (o.ld * e % 16 == 0 || o.rows <= 1) && (long long)o.width * e % 16 == 0) return 0;
+    return block_align256((size_t)o.rows * padded(o.width, dtype) * e);
+}
+// Replaces the operands that need it by their copies, which take the workspace from `ws` on.
+template <typename T> int copy_operands(Operand** list, int n, int dtype, char*& ws, hipStream_t s) {
+    CopyArgs a{};
+    int jobs = 0;
+    long long most = 0;
+    for (int i = 0; i < n; ++i) {
+        Operand& o = *list[i];
+        const size_t bytes = copy_bytes(o, dtype);
+        if (!bytes) continue;
+        const int pitch = padded(o.width, dtype);
+        a.job[jobs++] = {o.p, ws, o.ld, o.rows, o.width, pitch};
+        most = bytes / 16 > (size_t)most ? (long long)(bytes / 16) : most;
+        o.p = ws;
+        o.ld = pitch;
+        ws += bytes;
+    }
+    if (!jobs) return DMN_OK;
+    const long long blocks = ceil_div(most, 256);
+    pad_copy_kernel<T><<<dim3((unsigned)(blocks < 4096 ? blocks : 4096), jobs), 256, 0, s>>>(a);
+    DMN_BLOCK_LAUNCH_CHECK();
+    return DMN_OK;
 }
 
 template <typename F> int allow_lds(F* kernel, int bytes) {
@@ -757,10 +742,8 @@ template <typename T, bool XA, bool XB, int BM, int BN, int WM, int WN, int S> i
     DMN_BLOCK_LAUNCH_CHECK();
     return DMN_OK;
 }
-template <typename T, bool XA, bool XB, int B, int W> int any_launch(const GemmArgs& g, hipStream_t s) {
-    constexpr int NT = (B / W) * (B / W) * 64, LDS = 2 * 2 * B * 128;
-    static_assert((NT / 64) * 2 * 16 * (W + 4) * 4 <= LDS, "the epilogue's pieces fit the tiles' memory");
-    gemm_kernel<T, XA, XB, B, B, W, W><<<dim3((unsigned)(ceil_div(g.M, B) * ceil_div(g.N, B)), g.splits), NT, LDS, s>>>(g);
+template <typename T, int G> int join_launch(const GemmArgs& g, hipStream_t s) {
+    gemm_join_kernel<T, G><<<(unsigned)ceil_div((long long)g.M * ceil_div(g.N, Pack<T>::N), 256 / G), 256, 0, s>>>(g);
     DMN_BLOCK_LAUNCH_CHECK();
     return DMN_OK;
 }
@@ -781,28 +764,33 @@ template <typename T> int few_rows_run(const GemmArgs& g, hipStream_t s) {
     return cols >= 1024 ? few_rows_launch<T, 4, 4, 4>(g, s) : cols >= 512 ? few_rows_launch<T, 4, 2, 8>(g, s) : few_rows_launch<T, 4, 1, 16>(g, s);
 }
 
+// C = sum_k A B with the operands on 16-byte boundaries (copy_operands).
 template <typename T, bool XA, bool XB> int gemm_run(GemmArgs& g, int dtype, void* ws, hipStream_t s) {
-    if (!XB && few_rows(g.M)) {
-        if constexpr (!XB) return few_rows_run<T>(g, s);
-    }
     const GemmPlan p = gemm_plan(g.M, g.N, g.K, dtype);
     g.splits = p.splits;
     g.tiles_per_split = p.per;
     g.part = p.splits > 1 ? (float*)ws : nullptr;
-    const bool direct = direct_ok(g.a, g.lda, XA, g.M, g.K, dtype) && direct_ok(g.b, g.ldb, XB, g.N, g.K, dtype);
     int rc;
-    if (direct) {
-        if (p.tile == 0) rc = pipe_launch<T, XA, XB, 256, 256, 128, 64, 2>(g, s);
-        else if (p.tile == 1) rc = pipe_launch<T, XA, XB, 128, 128, 64, 32, 4>(g, s);
-        else rc = pipe_launch<T, XA, XB, 64, 64, 32, 32, 3>(g, s);
-    } else {
-        rc = p.tile < 2 ? any_launch<T, XA, XB, 128, 64>(g, s) : any_launch<T, XA, XB, 64, 32>(g, s);
-    }
-    if (rc || g.splits == 1) return rc;
-    const long long pieces = (long long)g.M * ceil_div(g.N, Pack<T>::N);
-    gemm_join_kernel<T><<<(unsigned)(pieces < 256 * 4096 ? ceil_div(pieces, 256) : 4096), 256, 0, s>>>(g);
-    DMN_BLOCK_LAUNCH_CHECK();
-    return DMN_OK;
+    if (p.tile == 0) rc = pipe_launch<T, XA, XB, 256, 256, 128, 64, 2>(g, s);
+    else if (p.tile == 1) rc = pipe_launch<T, XA, XB, 128, 128, 64, 32, 4>(g, s);
+    else if (p.tile == 2) rc = pipe_launch<T, XA, XB, 128, 128, 64, 32, 2>(g, s);
+    else rc = pipe_launch<T, XA, XB, 64, 64, 32, 32, 2>(g, s);
+    if (rc || p.splits == 1) return rc;
+    // eight threads per piece where there are few of them
+    return p.splits >= 8 && (long long)g.M * g.N < (1 << 20) ? join_launch<T, 8>(g, s) : join_launch<T, 1>(g, s);
+}
+
+template <typename T> int forward_run(GemmArgs& g, int dtype, char* ws, hipStream_t s) {
+    if (few_rows(g.M)) return few_rows_run<T>(g, s);
+    Operand x{g.a, g.lda, g.M, g.K}, w{g.b, g.ldb, g.N, g.K};
+    Operand* list[2] = {&x, &w};
+    const int rc = copy_operands<T>(list, 2, dtype, ws, s);
+    if (rc) return rc;
+    g.a = x.p;
+    g.lda = x.ld;
+    g.b = w.p;
+    g.ldb = w.ld;
+    return gemm_run<T, false, false>(g, dtype, ws, s);
 }
 
 constexpr int kMaxDzRuns = 64;
@@ -832,14 +820,14 @@ int backward_run(const void* dy, long long lddy, const void* x, long long ldx, c
     float* part = (float*)ws;
     const int runs = dz_runs(rows);
     ws += block_align256((size_t)runs * out * sizeof(float));
-    const void* dz = dy;
-    long long lddz = lddy;
+    Operand z_{dy, lddy, rows, out}, w_{w, in, out, in}, x_{x, ldx, rows, in};
     if (act != ACT_NONE || db) {
         DzArgs a{};
         a.dy = dy;
         a.z = z;
         a.lddy = lddy;
-        a.dz = act != ACT_NONE ? ws : nullptr;
+        a.dz = act != ACT_NONE && (dx || dw) ? ws : nullptr;
+        a.lddz = padded(out, dtype);
         a.part = db ? part : nullptr;
         a.M = rows;
         a.N = out;
@@ -851,18 +839,24 @@ int backward_run(const void* dy, long long lddy, const void* x, long long ldx, c
             DMN_BLOCK_LAUNCH_CHECK();
         }
         if (act != ACT_NONE) {
-            dz = ws;
-            lddz = out;
-            ws += block_align256((size_t)rows * out * sizeof(T));
+            z_.p = ws;
+            z_.ld = a.lddz;
+            z_.width = (int)a.lddz;
+            ws += block_align256((size_t)rows * a.lddz * sizeof(T));
         }
     }
-    int rc = DMN_OK;
-    if (dx) {
+    Operand* list[3];
+    int n = 0;
+    if (dx || dw) list[n++] = &z_;
+    if (dx) list[n++] = &w_;
+    if (dw) list[n++] = &x_;
+    int rc = copy_operands<T>(list, n, dtype, ws, s);
+    if (dx && !rc) {
         GemmArgs g{};
-        g.a = dz;
-        g.lda = lddz;
-        g.b = w;
-        g.ldb = in;
+        g.a = z_.p;
+        g.lda = z_.ld;
+        g.b = w_.p;
+        g.ldb = w_.ld;
         g.M = rows;
         g.N = in;
         g.K = out;
@@ -871,10 +865,10 @@ int backward_run(const void* dy, long long lddy, const void* x, long long ldx, c
     }
     if (dw && !rc) {
         GemmArgs g{};
-        g.a = dz;
-        g.lda = lddz;
-        g.b = x;
-        g.ldb = ldx;
+        g.a = z_.p;
+        g.lda = z_.ld;
+        g.b = x_.p;
+        g.ldb = x_.ld;
         g.M = out;
         g.N = in;
         g.K = rows;
@@ -886,9 +880,9 @@ int backward_run(const void* dy, long long lddy, const void* x, long long ldx, c
 
 }  // namespace
 
-extern "C" size_t dmn_linear_forward_workspace_bytes(int64_t rows, int in, int out, int dtype) {
+extern "C" size_t dmn_linear_forward_workspace_bytes(const void* x, int64_t ldx, const void* weight, int64_t rows, int in, int out, int dtype) {
     if (rows <= 0 || rows >= (1 << 27) || in <= 0 || out <= 0 || dtype < 0 || dtype > 2 || few_rows((int)rows)) return 0;
-    return gemm_workspace((int)rows, out, in, dtype);
+    return gemm_workspace((int)rows, out, in, dtype) + copy_bytes({x, ldx, (int)rows, in}, dtype) + copy_bytes({weight, in, out, in}, dtype);
 }
 
 extern "C" int dmn_linear_forward(const void* x, int64_t ldx, const void* weight, const void* bias, const void* residual, int64_t ldr,
@@ -898,9 +892,9 @@ extern "C" int dmn_linear_forward(const void* x, int64_t ldx, const void* weight
     if (rc || rows == 0) return rc;
     DMN_REQUIRE(x && weight && y, DMN_ERR_INVALID, "dmn_linear_forward: null argument");
     DMN_REQUIRE(!residual || rows <= 1 || ldr >= out, DMN_ERR_INVALID, "dmn_linear_forward: row stride of the residual below its width");
-    const size_t need = dmn_linear_forward_workspace_bytes(rows, in, out, dtype);
-    DMN_REQUIRE(need == 0 || (workspace && (uintptr_t)workspace % 16 == 0 && workspace_bytes >= need), DMN_ERR_WORKSPACE,
-                "dmn_linear_forward: workspace of %zu bytes, %zu needed (16-byte aligned)", workspace_bytes, need);
+    const size_t need = dmn_linear_forward_workspace_bytes(x, ldx, weight, rows, in, out, dtype);
+    DMN_REQUIRE(need == 0 || (workspace && (uintptr_t)workspace % 256 == 0 && workspace_bytes >= need), DMN_ERR_WORKSPACE,
+                "dmn_linear_forward: workspace of %zu bytes, %zu needed (256-byte aligned)", workspace_bytes, need);
     GemmArgs g{};
     g.a = x;
     g.lda = ldx;
@@ -916,16 +910,19 @@ extern "C" int dmn_linear_forward(const void* x, int64_t ldx, const void* weight
     g.z = z;
     g.act = activation;
     hipStream_t s = (hipStream_t)stream;
-    if (dtype == DMN_DT_F32) return gemm_run<float, false, false>(g, dtype, workspace, s);
-    if (dtype == DMN_DT_BF16) return gemm_run<__bf16, false, false>(g, dtype, workspace, s);
-    return gemm_run<f16, false, false>(g, dtype, workspace, s);
+    char* ws = (char*)workspace;
+    if (dtype == DMN_DT_F32) return forward_run<float>(g, dtype, ws, s);
+    if (dtype == DMN_DT_BF16) return forward_run<__bf16>(g, dtype, ws, s);
+    return forward_run<f16>(g, dtype, ws, s);
 }
 
-extern "C" size_t dmn_linear_backward_workspace_bytes(int64_t rows, int in, int out, int activation, int dtype) {
+extern "C" size_t dmn_linear_backward_workspace_bytes(const void* dy, int64_t lddy, const void* x, int64_t ldx, const void* weight, int64_t rows,
+                                                      int in, int out, int activation, int dtype) {
     if (rows <= 0 || rows >= (1 << 27) || in <= 0 || out <= 0 || dtype < 0 || dtype > 2) return 0;
     const size_t dx = gemm_workspace((int)rows, in, out, dtype), dw = gemm_workspace(out, in, (int)rows, dtype);
-    return block_align256((size_t)dz_runs((int)rows) * out * sizeof(float)) +
-           (activation != ACT_NONE ? block_align256((size_t)rows * out * elem(dtype)) : 0) + (dx > dw ? dx : dw);
+    const size_t dz = activation != ACT_NONE ? block_align256((size_t)rows * padded(out, dtype) * elem(dtype)) : copy_bytes({dy, lddy, (int)rows, out}, dtype);
+    return block_align256((size_t)dz_runs((int)rows) * out * sizeof(float)) + dz + copy_bytes({x, ldx, (int)rows, in}, dtype) +
+           copy_bytes({weight, in, out, in}, dtype) + (dx > dw ? dx : dw);
 }
 
 extern "C" int dmn_linear_backward(const void* dy, int64_t lddy, const void* x, int64_t ldx, const void* weight, const void* z, void* dx,
@@ -938,7 +935,7 @@ extern "C" int dmn_linear_backward(const void* dy, int64_t lddy, const void* x, 
                 "dmn_linear_backward: null argument");
     DMN_REQUIRE(rows <= 1 || lddy >= out, DMN_ERR_INVALID, "dmn_linear_backward: row stride of dy below its width");
     DMN_REQUIRE(lddy < (1 << 20), DMN_ERR_LIMIT, "dmn_linear_backward: row stride of dy must be below 2^20 elements");
-    const size_t need = dmn_linear_backward_workspace_bytes(rows, in, out, activation, dtype);
+    const size_t need = dmn_linear_backward_workspace_bytes(dy, lddy, x, ldx, weight, rows, in, out, activation, dtype);
     DMN_REQUIRE(need == 0 || (workspace && (uintptr_t)workspace % 256 == 0 && workspace_bytes >= need), DMN_ERR_WORKSPACE,
                 "dmn_linear_backward: workspace of %zu bytes, %zu needed (256-byte aligned)", workspace_bytes, need);
     hipStream_t s = (hipStream_t)stream;

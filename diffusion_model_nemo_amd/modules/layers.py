@@ -157,9 +157,10 @@ def _linear_forward(x, ldx, weight, bias, residual, ldr, activation, want_z):
     y = torch.empty(x.shape[:-1] + (out,), dtype=x.dtype, device=x.device)
     z = torch.empty_like(y) if want_z else None
     lib, code = N.lib(), N.DTYPE_CODES[x.dtype]
-    nbytes = lib.dmn_linear_forward_workspace_bytes(rows, width, out, code)
+    px, pw = x.data_ptr(), weight.data_ptr()
+    nbytes = lib.dmn_linear_forward_workspace_bytes(px, ldx, pw, rows, width, out, code)
     ws = torch.empty(nbytes, dtype=torch.uint8, device=x.device) if nbytes else None
-    N.launch(x.get_device(), lib.dmn_linear_forward, x.data_ptr(), ldx, weight.data_ptr(), None if bias is None else bias.data_ptr(),
+    N.launch(x.get_device(), lib.dmn_linear_forward, px, ldx, pw, None if bias is None else bias.data_ptr(),
              None if residual is None else residual.data_ptr(), ldr, y.data_ptr(), None if z is None else z.data_ptr(), rows, width,
              out, activation, code, None if ws is None else ws.data_ptr(), nbytes)
     return y, z, rows, code
@@ -196,9 +197,10 @@ class _LinearFunction(torch.autograd.Function):
             dw = torch.empty_like(weight) if need_w else None
             db = torch.empty_like(bias) if need_b else None
             lib = N.lib()
-            nbytes = lib.dmn_linear_backward_workspace_bytes(rows, width, out, activation, code)
+            pd, px, pw = rows_dy.data_ptr(), x.data_ptr(), weight.data_ptr()
+            nbytes = lib.dmn_linear_backward_workspace_bytes(pd, lddy, px, ldx, pw, rows, width, out, activation, code)
             ws = torch.empty(nbytes, dtype=torch.uint8, device=x.device) if nbytes else None
-            N.launch(x.get_device(), lib.dmn_linear_backward, rows_dy.data_ptr(), lddy, x.data_ptr(), ldx, weight.data_ptr(),
+            N.launch(x.get_device(), lib.dmn_linear_backward, pd, lddy, px, ldx, pw,
                      None if z is None else z.data_ptr(), None if dx is None else dx.data_ptr(), None if dw is None else dw.data_ptr(),
                      None if db is None else db.data_ptr(), rows, width, out, activation, code, None if ws is None else ws.data_ptr(),
                      nbytes)

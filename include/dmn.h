@@ -294,15 +294,18 @@ int dmn_layer_norm_backward(const void* dy, int64_t lddy, const void* x, int64_t
  * (ldr apart) or NULL, all of `dtype`; y [rows][out]. activation: 0 none, 1 ReLU, 2 SiLU, 3 GELU (exact). z: optional
  * [rows][out], receives x weight^T + bias rounded to dtype for the backward. rows may be 0; rows < 2^27, in, out and row
  * strides of x and dy < 2^20. Products run on the matrix cores with float32 accumulation (float32 operands exactly).
- * workspace: 16-byte aligned; 0 bytes needed: may be NULL. */
-size_t dmn_linear_forward_workspace_bytes(int64_t rows, int in, int out, int dtype);
+ * workspace: 256-byte aligned; 0 bytes needed: may be NULL. What is needed depends on the sizes and on whether the operands'
+ * rows lie on 16-byte boundaries (the workspace functions look at the addresses for nothing else): copies of those that do
+ * not, partial products where k is split, the backward's dz. */
+size_t dmn_linear_forward_workspace_bytes(const void* x, int64_t ldx, const void* weight, int64_t rows, int in, int out, int dtype);
 int dmn_linear_forward(const void* x, int64_t ldx, const void* weight, const void* bias, const void* residual, int64_t ldr,
                        void* y, void* z, int64_t rows, int in, int out, int activation, int dtype, void* workspace,
                        size_t workspace_bytes, void* stream);
 /* dx [rows][in], dweight [out][in], dbias [out] (each optional, overwritten) from dy [rows][out] (lddy apart) and the
  * forward's x, weight and z (z only with an activation). The residual's gradient is dy. dz = dy act'(z) is rounded to dtype
- * where it enters the products, not where dbias adds it up. workspace: 256-byte aligned. */
-size_t dmn_linear_backward_workspace_bytes(int64_t rows, int in, int out, int activation, int dtype);
+ * where it enters the products, not where dbias adds it up. */
+size_t dmn_linear_backward_workspace_bytes(const void* dy, int64_t lddy, const void* x, int64_t ldx, const void* weight,
+                                           int64_t rows, int in, int out, int activation, int dtype);
 int dmn_linear_backward(const void* dy, int64_t lddy, const void* x, int64_t ldx, const void* weight, const void* z, void* dx,
                         void* dweight, void* dbias, int64_t rows, int in, int out, int activation, int dtype, void* workspace,
                         size_t workspace_bytes, void* stream);

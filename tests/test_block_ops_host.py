@@ -31,6 +31,33 @@ def test_layer_norm_entry_points_check_their_arguments():
     assert b"needed" in lib.dmn_last_error()
 
 
+def test_linear_entry_points_check_their_arguments():
+    lib = _N().lib()
+    need = lib.dmn_linear_forward_workspace_bytes
+    assert need(X, 1024, X, 64, 1024, 1024, 1) == 0                   # few rows: no workspace
+    assert need(X, 4096, X, 256, 4096, 256, 1) > 0                    # k is split
+    assert need(X, 1000, X, 4096, 1000, 4096, 1) == 0                 # rows of whole 16-byte pieces
+    odd = need(X, 1001, X, 4096, 1001, 4096, 1)
+    assert odd >= (4096 + 4096) * 1008 * 2 and need(X + 2, 1000, X, 4096, 1000, 4096, 1) >= 4096 * 1000 * 2
+    for bad in ((X, 8, X, -1, 8, 8, 0), (X, 8, X, 100, 0, 8, 0), (X, 8, X, 100, 8, 8, 3), (X, 8, X, 1 << 27, 8, 8, 0)):
+        assert need(*bad) == 0
+    fwd = lambda x=X, ldx=1001, w=X, res=None, ldr=0, y=X, rows=4096, k=1001, n=4096, act=0, dt=1, ws=X, nb=odd: lib.dmn_linear_forward(  # noqa: E731
+        x, ldx, w, None, res, ldr, y, None, rows, k, n, act, dt, ws, nb, None)
+    assert fwd(x=None) == -1 and fwd(w=None) == -1 and fwd(y=None) == -1
+    assert fwd(act=4) == -1 and fwd(act=-1) == -1 and fwd(dt=3) == -1 and fwd(rows=-1) == -1 and fwd(k=0) == -1 and fwd(n=0) == -1
+    assert fwd(ldx=1000) == -1 and fwd(res=X, ldr=4095) == -1
+    assert fwd(ldx=1 << 20) == -5 and fwd(rows=1 << 27) == -5 and fwd(k=1 << 20, ldx=1 << 20) == -5
+    assert fwd(ws=None) == -3 and fwd(nb=odd - 1) == -3 and fwd(ws=X + 16) == -3 and b"needed" in lib.dmn_last_error()
+    assert fwd(rows=0, x=None, w=None, y=None) == 0
+    n = lib.dmn_linear_backward_workspace_bytes(X, 4096, X, 1001, X, 4096, 1001, 4096, 3, 1)
+    bwd = lambda dy=X, lddy=4096, x=X, w=X, z=X, dx=X, dw=X, db=X, rows=4096, act=3, ws=X, nb=n: lib.dmn_linear_backward(  # noqa: E731
+        dy, lddy, x, 1001, w, z, dx, dw, db, rows, 1001, 4096, act, 1, ws, nb, None)
+    assert bwd(dy=None) == -1 and bwd(x=None) == -1 and bwd(w=None) == -1 and bwd(z=None) == -1 and bwd(act=5) == -1
+    assert bwd(lddy=4095) == -1 and bwd(lddy=1 << 20) == -5
+    assert bwd(ws=None) == -3 and bwd(nb=n - 1) == -3 and bwd(ws=X + 128) == -3
+    assert bwd(dx=None, dw=None, db=None, dy=None) == 0
+
+
 def test_clip_entry_point_checks_its_arguments():
     N = _N()
     lib = N.lib()
@@ -75,6 +102,18 @@ def test_operators_refuse_host_tensors_and_bad_arguments():
         with pytest.raises(ValueError):
             clip_grad_norm_([p], **bad)
     assert bool((p.grad == 1).all())
+
+
+def test_linear_refuses_host_tensors_and_unknown_activations():
+    from diffusion_model_nemo_amd.modules import Linear, linear
+    with pytest.raises(RuntimeError, match="no CPU"):
+        linear(torch.zeros(2, 8), torch.zeros(4, 8))
+    with pytest.raises(RuntimeError, match="no CPU"):
+        Linear(8, 4)(torch.zeros(2, 8))
+    with pytest.raises(ValueError):
+        Linear(8, 4, activation="tanh")
+    ours, theirs = Linear(8, 4, bias=False, activation="gelu"), torch.nn.Linear(8, 4, bias=False)
+    ours.load_state_dict(theirs.state_dict())
 
 
 def test_layer_norm_module_has_torch_state():

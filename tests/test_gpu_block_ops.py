@@ -362,6 +362,22 @@ def test_linear_activation_tails_and_nonfinite_rows():
         assert bool(torch.isnan(linear(x, w, activation="relu")[3]).all())
 
 
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("kind", [None, "gelu"])
+def test_linear_gradients_asked_for_one_by_one(kind, dtype):
+    from diffusion_model_nemo_amd.modules import linear
+    for shape in ((70, 96, 104), (33, 45, 51)):
+        m, k, n = shape
+        args = [randn((m, k), 1, dtype), randn((n, k), 2, dtype, k ** -0.5), randn((n,), 3, dtype), randn((m, n), 4, dtype)]
+        dy = randn((m, n), 5, dtype)
+        every = [a.clone().requires_grad_(True) for a in args]
+        want = torch.autograd.grad(linear(every[0], every[1], every[2], kind, every[3]), every, dy)
+        for i in range(4):
+            some = [a.clone().requires_grad_(i == j) for j, a in enumerate(args)]
+            (got,) = torch.autograd.grad(linear(some[0], some[1], some[2], kind, some[3]), some[i], dy)
+            assert torch.equal(got, want[i]), (shape, i)
+
+
 def test_linear_empty_batch():
     from diffusion_model_nemo_amd.modules import linear
     for kind in (None, "gelu"):
