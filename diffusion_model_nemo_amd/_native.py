@@ -3,6 +3,7 @@
 There is no CPU fallback: if the library is missing or cannot be loaded the first use raises.
 """
 import ctypes as C
+import importlib.util
 import os
 from typing import Dict, Optional
 
@@ -157,18 +158,27 @@ def current_stream_handle(device=None) -> int:
     return torch.cuda.current_stream(device).cuda_stream
 
 
-def launch(index: int, fn, *args):
-    """Calls an entry point whose last argument is the stream: torch's current stream of GPU `index`, with that device
-    current. (The two look-ups behind torch.cuda.current_stream and current_device without their checks: the caller holds
-    a tensor on the device, and a small operator's whole call takes ten microseconds.)"""
-    stream = torch._C._cuda_getCurrentRawStream(index)
-    if torch._C._cuda_getDevice() == index:
-        rc = fn(*args, stream)
-    else:
-        with torch.cuda.device(index):
-            rc = fn(*args, stream)
-    if rc != 0:
-        check(rc)
+_ops = None
+# entry points that the compiled binding calls, in the order of its `Api`
+BOUND = ("dmn_last_error", "dmn_layer_norm_forward", "dmn_layer_norm_workspace_bytes", "dmn_layer_norm_backward",
+         "dmn_linear_forward_workspace_bytes", "dmn_linear_forward", "dmn_linear_backward_workspace_bytes", "dmn_linear_backward",
+         "dmn_clip_grads_workspace_bytes", "dmn_clip_grads")
+
+
+def ops():
+    """The compiled torch side of the trained-block operators (csrc/dmn_torch.cpp), bound to the library's entry points on
+    first use; raises if it is not built."""
+    global _ops
+    if _ops is None:
+        path = os.path.join(_HERE, "lib", "_dmn_torch.so")
+        if not os.path.exists(path):
+            raise DmnError(f"{path} is missing: build it with `python -m diffusion_model_nemo_amd.build`")
+        spec = importlib.util.spec_from_file_location("_dmn_torch", path)
+        module = importlib.util.module_from_spec(spec)
+        spec.loader.exec_module(module)
+        module.bind([C.cast(getattr(lib(), name), C.c_void_p).value for name in BOUND], DmnError, torch._C._cuda_getCurrentRawStream)
+        _ops = module
+    return _ops
 
 
 def make_tensor_descs(params: Dict[str, np.ndarray]):

@@ -13,6 +13,7 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 LIB_DIR = os.path.join(HERE, "lib")
 LIB_PATH = os.path.join(LIB_DIR, "libdmn_hip.so")
+TORCH_LIB_PATH = os.path.join(LIB_DIR, "_dmn_torch.so")   # host code only: torch's side of the trained-block operators
 SOURCES = ["dmn_conv.hip", "dmn_elem.hip", "dmn_attn.hip", "dmn_linattn.hip", "dmn_sampler.hip", "dmn_unet.cpp", "dmn_api.cpp",
            "dmn_train_gemm.hip", "dmn_train_ops.hip", "dmn_train.cpp", "dmn_peaks.hip", "dmn_layernorm.hip", "dmn_clip.hip", "dmn_linear.hip"]
 ARCH = "gfx950"
@@ -30,6 +31,18 @@ def _newest_header():
     inc = [os.path.join(CSRC, f) for f in os.listdir(CSRC) if f.endswith(".h")]
     inc.append(os.path.join(os.path.dirname(HERE), "include", "dmn.h"))
     return max(os.path.getmtime(p) for p in inc)
+
+
+def _torch_binding_command():
+    """g++ on csrc/dmn_torch.cpp against the installed torch's headers and libraries (no ninja, no generated files)."""
+    import sysconfig
+    import torch
+    from torch.utils.cpp_extension import include_paths, library_paths
+    inc = [f"-I{p}" for p in (sysconfig.get_paths()["include"], *include_paths())]
+    lib = [f for p in library_paths() for f in (f"-L{p}", f"-Wl,-rpath,{p}")]
+    return ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-Wall", "-Wno-sign-compare", "-Wno-unknown-pragmas", *inc,
+            f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", os.path.join(CSRC, "dmn_torch.cpp"), "-o", TORCH_LIB_PATH,
+            *lib, "-lc10", "-ltorch_cpu", "-ltorch", "-ltorch_python"]
 
 
 def build(force: bool = False, verbose: bool = False) -> str:
@@ -65,18 +78,23 @@ def build(force: bool = False, verbose: bool = False) -> str:
             cmd = [hipcc, *flags, *extra.get(src, []), "-x", "hip", "-c", sp, "-o", op]
             jobs.append(cmd)
 
+    torch_src = os.path.join(CSRC, "dmn_torch.cpp")
+    torch_jobs = []
+    if force or not os.path.exists(TORCH_LIB_PATH) or os.path.getmtime(TORCH_LIB_PATH) < max(os.path.getmtime(torch_src), hdr_time):
+        torch_jobs.append(_torch_binding_command())
+
     def run(cmd):
         if verbose:
             print(" ".join(cmd), flush=True)
         r = subprocess.run(cmd, capture_output=True, text=True)
         if r.returncode != 0:
-            raise RuntimeError(f"hipcc failed:\n{' '.join(cmd)}\n{r.stdout}\n{r.stderr}")
+            raise RuntimeError(f"{os.path.basename(cmd[0])} failed:\n{' '.join(cmd)}\n{r.stdout}\n{r.stderr}")
         if verbose and r.stderr.strip():
             print(r.stderr)
 
-    if jobs:
-        with ThreadPoolExecutor(max_workers=min(6, len(jobs))) as ex:
-            list(ex.map(run, jobs))
+    if jobs or torch_jobs:
+        with ThreadPoolExecutor(max_workers=min(6, len(jobs) + len(torch_jobs))) as ex:
+            list(ex.map(run, torch_jobs + jobs))
     if jobs or not os.path.exists(LIB_PATH):
         run([hipcc, "-shared", "-fPIC", f"--offload-arch={ARCH}", "-o", LIB_PATH, *objs])
         # the flags above are only as good as what they produce: disassemble the result and refuse a library that

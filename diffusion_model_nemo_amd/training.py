@@ -12,7 +12,6 @@ import ctypes as C
 import math
 from typing import Dict, Iterable, Optional, Sequence, Union
 
-import numpy as np
 import torch
 
 from . import _native as N
@@ -256,6 +255,65 @@ def _dense(t: torch.Tensor) -> bool:
 
 
 @torch.no_grad()
+def _clip_one_by_one(params, norm_type, max_norm, error_if_nonfinite, grad_scale, out):
+    """`clip_grad_norm_` where it has to wait for the norm, and for gradients out of the ordinary: none at all, scattered or
+    permuted ones, and those it refuses."""
+    grads = [p.grad for p in params]
+    if out is not None:
+        out = [o for o, g in zip(out, grads) if g is not None]
+    grads = [g for g in grads if g is not None]
+    if not grads:
+        return torch.zeros(())
+    dev = grads[0].device
+    if dev.type != "cuda":
+        raise RuntimeError("clip_grad_norm_ runs only on MI355X device tensors (no CPU implementation)")
+    copied = []   # (gradient, its dense copy): scattered gradients are clipped in a copy and written back
+    for i, g in enumerate(grads):
+        if g.device != dev:
+            raise RuntimeError(f"gradients on {dev} and {g.device}: all must be on one device")
+        if g.layout != torch.strided or g.dtype not in N.DTYPE_CODES:
+            raise ValueError(f"gradients must be dense float32, bfloat16 or float16 tensors, got {g.dtype} ({g.layout})")
+        if not g.is_contiguous() and (out is not None or not _dense(g)):
+            copied.append((g, g.contiguous()))
+    if out is None and copied:
+        _refuse_shared_memory([g for g, _ in copied], grads)
+    dense = {id(g): c for g, c in copied}
+    srcs = [dense.get(id(g), g) for g in grads]
+    if out is not None:
+        for o, g in zip(out, grads):
+            if o.device != dev or o.shape != g.shape or o.dtype not in N.DTYPE_CODES or not o.is_contiguous():
+                raise ValueError("out must hold contiguous float32 / bfloat16 / float16 tensors of the gradients' shapes, on "
+                                 "their device")
+    dsts = srcs if out is None else out
+    table = (N.DmnGradTensor * len(srcs))(*[N.DmnGradTensor(s.data_ptr(), d.data_ptr(), s.numel(), N.DTYPE_CODES[s.dtype], N.DTYPE_CODES[d.dtype])
+                                            for s, d in zip(srcs, dsts)])
+    lib = N.lib()
+    nbytes = lib.dmn_clip_grads_workspace_bytes(len(table))
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+    norm = torch.empty((), dtype=torch.float32, device=dev)
+
+    def call():
+        with torch.cuda.device(dev):
+            N.check(lib.dmn_clip_grads(C.addressof(table), len(table), int(norm_type != 2.0), max_norm, grad_scale, norm.data_ptr(),
+                                       ws.data_ptr(), nbytes, N.current_stream_handle(dev)))
+
+    if error_if_nonfinite:
+        kept = [t.dst for t in table]
+        for t in table:
+            t.dst = None
+        call()
+        for t, dst in zip(table, kept):
+            t.dst = dst
+        if not bool(torch.isfinite(norm)):
+            raise RuntimeError(f"the total norm of the gradients is non-finite ({float(norm)}); they were not clipped")
+    call()
+    if out is None:
+        for g, c in copied:
+            g.copy_(c)
+    torch.autograd.graph.increment_version(dsts)
+    return norm
+
+
 def clip_grad_norm_(parameters: Union[torch.Tensor, Iterable[torch.Tensor]], max_norm: float, norm_type: float = 2.0,
                     error_if_nonfinite: bool = False, *, grad_scale: float = 1.0,
                     out: Optional[Sequence[torch.Tensor]] = None) -> torch.Tensor:
@@ -280,67 +338,13 @@ def clip_grad_norm_(parameters: Union[torch.Tensor, Iterable[torch.Tensor]], max
         raise ValueError(f"max_norm must be >= 0, got {max_norm}")
     if not math.isfinite(grad_scale):
         raise ValueError(f"grad_scale must be finite, got {grad_scale}")
-    grads = [p.grad for p in params]
-    if out is not None:
-        if len(out) != len(params):
-            raise ValueError(f"out holds {len(out)} tensors for {len(params)} parameters")
-        out = [o for o, g in zip(out, grads) if g is not None]
-    grads = [g for g in grads if g is not None]
-    if not grads:
-        return torch.zeros(())
-    # a few hundred gradients: every look-up runs over all of them at once, and only what is out of the ordinary one by one
-    dev, dtypes = grads[0].device, {g.dtype for g in grads}
-    if dev.type != "cuda":
-        raise RuntimeError("clip_grad_norm_ runs only on MI355X device tensors (no CPU implementation)")
-    if len(set(map(torch.Tensor.get_device, grads))) != 1:
-        raise RuntimeError("the gradients must all be on one device")
-    if not all(t in N.DTYPE_CODES for t in dtypes):
-        raise ValueError(f"gradients must be float32, bfloat16 or float16, got {sorted(map(str, dtypes))}")
-    copied = []   # (gradient, its dense copy): scattered gradients are clipped in a copy and written back
-    if not all(map(torch.Tensor.is_contiguous, grads)):
-        for i, g in enumerate(grads):
-            if g.layout != torch.strided:
-                raise ValueError(f"gradients must be dense tensors, got one of layout {g.layout}")
-            if not g.is_contiguous() and (out is not None or not _dense(g)):
-                copied.append((g, g.contiguous()))
-                grads[i] = copied[-1][1]
-        if out is None and copied:
-            _refuse_shared_memory([g for g, _ in copied], [p.grad for p in params if p.grad is not None])
-    table = np.empty((len(grads), 4), dtype=np.int64)   # DmnGradTensor: src, dst, numel, types
-    table[:, 0] = list(map(torch.Tensor.data_ptr, grads))
-    table[:, 2] = list(map(torch.Tensor.numel, grads))
-    table[:, 3] = N.DTYPE_CODES[grads[0].dtype] if len(dtypes) == 1 else [N.DTYPE_CODES[g.dtype] for g in grads]
-    if out is None:
-        table[:, 1] = table[:, 0]
-        table[:, 3] *= (1 << 32) + 1
-    else:
-        for o, g in zip(out, grads):
-            if o.device != dev or o.shape != g.shape or o.dtype not in N.DTYPE_CODES or not o.is_contiguous():
-                raise ValueError("out must hold contiguous float32 / bfloat16 / float16 tensors of the gradients' shapes, on "
-                                 "their device")
-        table[:, 1] = list(map(torch.Tensor.data_ptr, out))
-        table[:, 3] += np.array([N.DTYPE_CODES[o.dtype] for o in out], dtype=np.int64) << 32
-    lib = N.lib()
-    nbytes = lib.dmn_clip_grads_workspace_bytes(len(grads))
-    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
-    norm = torch.empty((), dtype=torch.float32, device=dev)
-
-    def call(rows):
-        N.launch(grads[0].get_device(), lib.dmn_clip_grads, rows.ctypes.data, len(rows), int(norm_type != 2.0), max_norm, grad_scale,
-                 norm.data_ptr(), ws.data_ptr(), nbytes)
-
-    if error_if_nonfinite:
-        only = table.copy()
-        only[:, 1] = 0
-        call(only)
-        if not bool(torch.isfinite(norm)):
-            raise RuntimeError(f"the total norm of the gradients is non-finite ({float(norm)}); they were not clipped")
-    call(table)
-    if out is None:
-        for g, c in copied:
-            g.copy_(c)
-    torch.autograd.graph.increment_version(grads if out is None else out)
-    return norm
+    if out is not None and len(out) != len(params):
+        raise ValueError(f"out holds {len(out)} tensors for {len(params)} parameters")
+    if not error_if_nonfinite:
+        norm = N.ops().clip_grads(params, None if out is None else list(out), norm_type != 2.0, max_norm, grad_scale)
+        if norm is not None:
+            return norm
+    return _clip_one_by_one(params, norm_type, max_norm, error_if_nonfinite, grad_scale, out)
 
 
 def cosine_annealing_lr(step: int, max_steps: int, base_lr: float, min_lr: float, warmup_steps: int = 0) -> float:
