@@ -747,8 +747,14 @@ template <typename T, int G> int join_launch(const GemmArgs& g, hipStream_t s) {
     DMN_BLOCK_LAUNCH_CHECK();
     return DMN_OK;
 }
-// Up to 64 rows the forward reads the weight once whatever it does, and the tiles' kernel cannot fill the chip.
-bool few_rows(int M) { return M <= 64; }
+// Whether the forward takes the kernel for few rows. Its workgroups read all of x each, so x has to be small (us, this kernel
+// against tiles, weights not in the caches: 64 x 2048 into 8192 bf16 19 : 25, 32 x 1000 into 1531 7 : 14, but 32 x 8192 into
+// 2048 28 : 19 and 64 x 8192 44 : 19); and few columns of a long k leave it CUs without work (16 x 8192 into 2048 19 : 15,
+// 16 x 4096 into 512 11 : 9; one row 14 : 14).
+bool few_rows(int M, int N, int K, int dtype) {
+    const long long bytes = (long long)K * elem(dtype);
+    return M <= 64 && M * bytes <= 256 * 1024 && (M < 8 || N >= 4096 || bytes < 8192);
+}
 template <typename T, int MF, int NF, int WAVES> int few_rows_launch(const GemmArgs& g, hipStream_t s) {
     constexpr int LDS = WAVES * MF * NF * 1024;
     static_assert(LDS <= 65536, "LDS without an attribute");
@@ -757,9 +763,9 @@ template <typename T, int MF, int NF, int WAVES> int few_rows_launch(const GemmA
     return DMN_OK;
 }
 template <typename T> int few_rows_run(const GemmArgs& g, hipStream_t s) {
-    // columns per workgroup: more of them read x less often, fewer fill the chip; waves: some eight per CU
+    // columns per workgroup: more of them read x less often, fewer fill the chip; waves: some sixteen per CU
     const long long cols = ceil_div(g.N, 16);
-    if (g.M <= 16) return cols >= 512 ? few_rows_launch<T, 1, 1, 4>(g, s) : cols >= 256 ? few_rows_launch<T, 1, 1, 8>(g, s) : few_rows_launch<T, 1, 1, 16>(g, s);
+    if (g.M <= 16) return cols >= 256 ? few_rows_launch<T, 1, 1, 8>(g, s) : few_rows_launch<T, 1, 1, 16>(g, s);
     if (g.M <= 32) return cols >= 512 ? few_rows_launch<T, 2, 2, 8>(g, s) : few_rows_launch<T, 2, 1, 16>(g, s);
     return cols >= 1024 ? few_rows_launch<T, 4, 4, 4>(g, s) : cols >= 512 ? few_rows_launch<T, 4, 2, 8>(g, s) : few_rows_launch<T, 4, 1, 16>(g, s);
 }
@@ -781,7 +787,7 @@ template <typename T, bool XA, bool XB> int gemm_run(GemmArgs& g, int dtype, voi
 }
 
 template <typename T> int forward_run(GemmArgs& g, int dtype, char* ws, hipStream_t s) {
-    if (few_rows(g.M)) return few_rows_run<T>(g, s);
+    if (few_rows(g.M, g.N, g.K, dtype)) return few_rows_run<T>(g, s);
     Operand x{g.a, g.lda, g.M, g.K}, w{g.b, g.ldb, g.N, g.K};
     Operand* list[2] = {&x, &w};
     const int rc = copy_operands<T>(list, 2, dtype, ws, s);
@@ -881,7 +887,7 @@ int backward_run(const void* dy, long long lddy, const void* x, long long ldx, c
 }  // namespace
 
 extern "C" size_t dmn_linear_forward_workspace_bytes(const void* x, int64_t ldx, const void* weight, int64_t rows, int in, int out, int dtype) {
-    if (rows <= 0 || rows >= (1 << 27) || in <= 0 || out <= 0 || dtype < 0 || dtype > 2 || few_rows((int)rows)) return 0;
+    if (rows <= 0 || rows >= (1 << 27) || in <= 0 || out <= 0 || dtype < 0 || dtype > 2 || few_rows((int)rows, out, in, dtype)) return 0;
     return gemm_workspace((int)rows, out, in, dtype) + copy_bytes({x, ldx, (int)rows, in}, dtype) + copy_bytes({weight, in, out, in}, dtype);
 }
 
