@@ -4,6 +4,7 @@
 // 105 us in Python's side of autograd and 25 us on the GPU. Host code only; streams arrive as handles.
 #include <ATen/ATen.h>
 #include <c10/core/DeviceGuard.h>
+#include <c10/core/impl/DeviceGuardImplInterface.h>
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/autograd/python_variable.h>
@@ -105,6 +106,20 @@ variable_list once_differentiable(variable_list grads) {
     return grads;
 }
 
+// Under capture the gradients of a leaf would be accumulated on the stream on which an eager graph that still lives first
+// used the leaf; torch then touches that stream in the middle of the capture, and the process ends. Such a call is refused.
+void check_capture(bool capturing, const Tensor& x, std::initializer_list<const Tensor*> inputs) {
+    if (!capturing) return;
+    const c10::Stream now = c10::impl::getDeviceGuardImpl(c10::DeviceType::CUDA)->getStream(x.device());
+    for (const Tensor* t : inputs) {
+        if (!t->defined() || !t->requires_grad() || !t->is_leaf()) continue;
+        const auto accumulator = torch::autograd::impl::try_get_grad_accumulator(*t);
+        if (accumulator && accumulator->stream().has_value() && *accumulator->stream() != now)
+            throw std::runtime_error("a graph is being captured while an eager graph over the same parameters or inputs, made on another stream, "
+                                     "still lives: drop its results first (del loss, outputs), or warm up on the capturing stream");
+    }
+}
+
 // ---- layer norm --------------------------------------------------------------------------------------------------------
 
 int affine_code(const Tensor& x, const Tensor& weight, const Tensor& bias) {
@@ -155,7 +170,7 @@ struct LayerNormNode : torch::autograd::Function<LayerNormNode> {
     }
 };
 
-Tensor layer_norm(const Tensor& x, const std::optional<Tensor>& weight_, const std::optional<Tensor>& bias_, double eps, int64_t stream) {
+Tensor layer_norm(const Tensor& x, const std::optional<Tensor>& weight_, const std::optional<Tensor>& bias_, double eps, int64_t stream, bool capturing) {
     check_input(x, "layer_norm");
     if (x.dim() == 0 || x.size(-1) == 0) throw py::value_error("layer_norm needs a last axis of at least one element");
     if (x.size(-1) > INT32_MAX) throw py::value_error("layer_norm: the last axis is too long");
@@ -167,8 +182,10 @@ Tensor layer_norm(const Tensor& x, const std::optional<Tensor>& weight_, const s
     if (weight.defined()) weight = weight.contiguous();
     if (bias.defined()) bias = bias.contiguous();
     c10::DeviceGuard guard(x.device());
-    if (at::GradMode::is_enabled() && (x.requires_grad() || (weight.defined() && weight.requires_grad()) || (bias.defined() && bias.requires_grad())))
+    if (at::GradMode::is_enabled() && (x.requires_grad() || (weight.defined() && weight.requires_grad()) || (bias.defined() && bias.requires_grad()))) {
+        check_capture(capturing, x, {&x, &weight, &bias});
         return LayerNormNode::apply(x, given(weight), given(bias), eps, stream);
+    }
     return layer_norm_run(rows_of(x), weight, bias, eps, stream, nullptr);
 }
 
@@ -236,7 +253,7 @@ struct LinearNode : torch::autograd::Function<LinearNode> {
 };
 
 Tensor linear(const Tensor& x, const Tensor& weight_, const std::optional<Tensor>& bias_, int64_t act, const std::optional<Tensor>& residual_,
-              int64_t stream) {
+              int64_t stream, bool capturing) {
     check_input(x, "linear");
     if (weight_.dim() != 2 || weight_.size(0) == 0 || weight_.size(1) == 0 || weight_.size(0) > INT32_MAX || weight_.size(1) > INT32_MAX)
         throw py::value_error(c10::str("weight must be [out, in], got ", weight_.sizes()));
@@ -249,8 +266,10 @@ Tensor linear(const Tensor& x, const Tensor& weight_, const std::optional<Tensor
     if (bias.defined()) bias = bias.contiguous();
     c10::DeviceGuard guard(x.device());
     if (at::GradMode::is_enabled() && (x.requires_grad() || weight.requires_grad() || (bias.defined() && bias.requires_grad()) ||
-                                       (residual.defined() && residual.requires_grad())))
+                                       (residual.defined() && residual.requires_grad()))) {
+        check_capture(capturing, x, {&x, &weight, &bias, &residual});
         return LinearNode::apply(x, weight, given(bias), given(residual), act, stream);
+    }
     return linear_run(rows_of(x), weight, bias, residual, act, stream, nullptr);
 }
 

@@ -2,14 +2,14 @@
 
 What the reference builds its blocks from outside the convolutions -- `Residual(PreNorm(fn))`
 (diffusion_model_nemo/utils.py:68-93) and the `nn.Linear` / `nn.GELU` pairs of its embedding networks
-(diffusion_model_nemo/modules/unet.py:55-61) -- as calls on device tensors with their backward passes. `layer_norm` and
+(diffusion_model_nemo/modules/unet.py:59-66) -- as calls on device tensors with their backward passes. `layer_norm` and
 `linear` are differentiable torch functions; `LayerNorm` and `Linear` hold the parameters under torch's names, so
 `state_dict`s interchange with `torch.nn`. There is no CPU implementation: a CPU tensor raises.
 
 Results are rounded once, to the input's type; sums, statistics and parameter gradients are formed in float32. The backward
-passes are not differentiable themselves. Calls can be captured into a graph; when a BACKWARD is captured, torch asks that no
-eager graph over the same leaves is still alive (capture after warm-up on the capturing stream, as `torch.cuda.graphs`
-describes).
+passes are not differentiable themselves. Calls and their backward passes can be captured into a graph; a call that would be
+captured while an eager graph over the same leaves, made on another stream, still lives is refused (its backward would end
+the process inside torch).
 """
 from typing import Optional
 
@@ -21,11 +21,11 @@ from .. import _native as N
 ACTIVATIONS = {None: 0, "relu": 1, "silu": 2, "gelu": 3}
 
 
-def _stream(x: torch.Tensor, what: str) -> int:
-    """torch's current stream of x's device; the other checks are in csrc/dmn_torch.cpp."""
+def _stream(x: torch.Tensor, what: str):
+    """(torch's current stream of x's device, whether a graph is being captured); the other checks are in csrc/dmn_torch.cpp."""
     if not x.is_cuda:
         raise RuntimeError(f"{what} runs only on MI355X device tensors (no CPU implementation)")
-    return torch._C._cuda_getCurrentRawStream(x.get_device())
+    return torch._C._cuda_getCurrentRawStream(x.get_device()), torch._C._cuda_isCurrentStreamCapturing()
 
 
 def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Optional[torch.Tensor] = None,
@@ -33,7 +33,7 @@ def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Opt
     """(x - mean) / sqrt(var + eps) * weight + bias over the last axis of `x` [..., width] (float32, bfloat16 or float16).
     `weight` and `bias` [width] (either may be None) are of x's type or float32, both alike; their gradients come in
     that type. Rows with any stride are read in place for a 2-D `x`; other layouts are copied first."""
-    return N.ops().layer_norm(x, weight, bias, eps, _stream(x, "layer_norm"))
+    return N.ops().layer_norm(x, weight, bias, eps, *_stream(x, "layer_norm"))
 
 
 def linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] = None, activation: Optional[str] = None,
@@ -46,7 +46,7 @@ def linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] =
     code = ACTIVATIONS.get(activation)
     if code is None:
         raise ValueError(f"activation must be one of {list(ACTIVATIONS)}, got {activation!r}")
-    return N.ops().linear(x, weight, bias, code, residual, _stream(x, "linear"))
+    return N.ops().linear(x, weight, bias, code, residual, *_stream(x, "linear"))
 
 
 class LayerNorm(nn.Module):

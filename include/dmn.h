@@ -268,7 +268,7 @@ int dmn_adamw_step(float* params, const float* grads, float* exp_avg, float* exp
 
 /* ---- operators of a trained block ---------------------------------------------------------------------------------
  * The layers and the gradient clipping that a block of linear layers beside the network needs: what
- * Residual(PreNorm(fn)) (utils.py:68-93), nn.Linear + GELU (modules/unet.py:55-61) and the trainer's gradient_clip_val are
+ * Residual(PreNorm(fn)) (utils.py:68-93), nn.Linear + GELU (modules/unet.py:59-66) and the trainer's gradient_clip_val are
  * to the network itself, on tensors of the caller. Tensors are DEVICE memory, rows of contiguous elements `ld` elements
  * apart; addresses need the alignment of the element type only. Nothing is allocated, nothing waits for the device, and a
  * call can be recorded into a graph; the device that owns the tensors must be the current one. Two calls that may overlap

@@ -481,6 +481,47 @@ def test_block_trains_with_clipping_in_eager_mode_and_in_a_graph():
         assert all(torch.equal(p, q) for p, q in zip([eager[0], eager[1]] + out, kept)), turn
 
 
+def test_capture_beside_a_living_eager_graph_is_refused_and_large_products_are_captured():
+    from diffusion_model_nemo_amd.modules import layer_norm, linear
+    x = randn((2100, 1032), 1, BF).requires_grad_(True)
+    w, b = randn((2056, 1032), 2, BF, 0.03).requires_grad_(True), randn((2056,), 3, BF).requires_grad_(True)
+    dy = randn((2100, 2056), 4, BF)
+    alive = linear(x, w, b, "gelu")
+    for call in (lambda: linear(x, w, b, "gelu"), lambda: layer_norm(x)):
+        with pytest.raises(RuntimeError, match="still lives"):
+            with torch.cuda.graph(torch.cuda.CUDAGraph()):
+                call()
+    want = alive.detach().clone()
+    del alive
+
+    def step():
+        y = linear(x, w, b, "gelu")
+        y.backward(dy)
+        return y.detach()
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        assert torch.equal(step(), want)
+    torch.cuda.current_stream().wait_stream(side)
+    for p in (x, w, b):
+        p.grad = None
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = step()
+    grads = [p.grad for p in (x, w, b)]          # the graph's own, overwritten by every replay
+    for turn in range(3):
+        with torch.no_grad():
+            x.copy_(randn((2100, 1032), 20 + turn, BF))
+        graph.replay()
+        kept = [got.clone()] + [g.clone() for g in grads]
+        y = linear(x, w, b, "gelu")
+        eager = torch.autograd.grad(y, (x, w, b), dy)
+        torch.cuda.synchronize()
+        assert torch.equal(kept[0], y.detach()) and all(torch.equal(p, q) for p, q in zip(kept[1:], eager)), turn
+        del y, eager
+
+
 # ---- gradient clipping -----------------------------------------------------------------------------------------------------
 
 def params_with(grads):
