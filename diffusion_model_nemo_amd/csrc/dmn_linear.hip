@@ -657,12 +657,12 @@ struct GemmPlan {
 };
 struct TileShape {
     int bm, bn, together;
-    double step16, least16, step32, least32, ends;
+    double step16, least16, ends16, step32, least32, ends32;
 };
-const TileShape kTiles[4] = {{256, 256, 1, 1.60, 1.12, 7.4, 7.2, 8.0},
-                             {128, 128, 1, 0.56, 0.45, 2.0, 1.9, 4.0},
-                             {128, 128, 2, 0.50, 0.68, 1.9, 2.0, 4.0},
-                             {64, 64, 4, 0.22, 0.28, 0.50, 0.55, 3.0}};
+const TileShape kTiles[4] = {{256, 256, 1, 1.60, 1.12, 8.0, 7.4, 7.2, 22.0},
+                             {128, 128, 1, 0.56, 0.45, 4.0, 2.0, 1.9, 8.0},
+                             {128, 128, 2, 0.50, 0.68, 4.0, 1.9, 2.0, 9.0},
+                             {64, 64, 4, 0.22, 0.28, 3.0, 0.55, 0.70, 6.0}};
 
 GemmPlan gemm_plan(int M, int N, int K, int dtype) {
     const int bk = 128 / elem(dtype);
@@ -671,13 +671,14 @@ GemmPlan gemm_plan(int M, int N, int K, int dtype) {
     double best_us = 1e30;
     for (int i = 0; i < 4; ++i) {
         const TileShape& t = kTiles[i];
-        const double step = dtype == DMN_DT_F32 ? t.step32 : t.step16, least = dtype == DMN_DT_F32 ? t.least32 : t.least16;
+        const bool f32 = dtype == DMN_DT_F32;
+        const double step = f32 ? t.step32 : t.step16, least = f32 ? t.least32 : t.least16, ends = f32 ? t.ends32 : t.ends16;
         const long long tiles = ceil_div(M, t.bm) * ceil_div(N, t.bn);
         for (int splits = 1; splits <= 64; splits *= 2) {
             if (splits > 1 && kt / splits < 4) break;
             const long long per = ceil_div(kt, splits), on_cu = ceil_div(tiles * splits, 256);
             const double all = tiles * splits > 128 ? on_cu * per * step : 0, one = per * least;
-            double us = (all > one ? all : one) + t.ends * ceil_div(on_cu, t.together);
+            double us = (all > one ? all : one) + ends * ceil_div(on_cu, t.together);
             if (splits > 1) us += 3.0 + (double)splits * M * N * 8 / 4e6;
             if (us < best_us) {
                 best_us = us;
