@@ -20,16 +20,28 @@ constexpr int kBlocks = 2048;       // workgroups of one launch: eight per CU, r
 constexpr int64_t kKeep = 80 << 20;  // bytes that the cache behind the L2s is trusted to keep between the passes
 constexpr int kPiece = 8192;        // elements that a workgroup takes at a time: neighbouring workgroups read neighbouring pieces
 
-// Tensors of one launch: entry i owns the pieces [first[i], first[i + 1]).
+// Tensors of one launch: entry i owns the pieces [first[i], first[i + 1]). An entry takes twelve bytes, so that the default
+// network's 256 gradients are one launch: where[i] is the address (47 bits, all that user space has), the types as source +
+// 3 * destination (4 bits) and the elements of the last piece less one (13 bits).
 template <bool OUT> struct ClipTable {
-    static constexpr int K = OUT ? 136 : 192;
+    static constexpr int K = OUT ? 196 : 330;
     int count, part_base;           // entries; index of the launch's first partial among all
     int first[K + 1];
-    unsigned long long meta[K];     // element count << 8 | type of dst << 4 | type of src
-    const void* src[K];
+    unsigned long long where[K];
     void* dst[OUT ? K : 1];
 };
-static_assert(sizeof(ClipTable<true>) <= 4000 && sizeof(ClipTable<false>) <= 4000, "kernel arguments");
+static_assert(sizeof(ClipTable<true>) <= 4000 && sizeof(ClipTable<false>) <= 4000 && kPiece == 1 << 13, "kernel arguments");
+
+struct PieceOf {                    // one piece of an entry
+    const void* src;
+    int st, dt, len;
+    long long at;                   // its first element
+};
+template <bool OUT> __device__ __forceinline__ PieceOf piece_of(const ClipTable<OUT>& t, int e, int p) {
+    const unsigned long long w = t.where[e];
+    const int types = (int)(w >> 47) & 15, last = (int)(w >> 51) + 1;
+    return {(const void*)(w & ((1ull << 47) - 1)), types % 3, types / 3, p + 1 == t.first[e + 1] ? last : kPiece, (long long)(p - t.first[e]) * kPiece};
+}
 
 struct ClipScale {
     const double* part;
@@ -115,10 +127,8 @@ template <bool INF> __global__ __launch_bounds__(kThreads) void grad_norm_kernel
     int e = find_entry(t, blockIdx.x);
     for (int p = blockIdx.x; p < pieces; p += gridDim.x) {
         while (t.first[e + 1] <= p) ++e;
-        const unsigned long long meta = t.meta[e];
-        const long long at = (long long)(p - t.first[e]) * kPiece, n = (long long)(meta >> 8);
-        const int len = (int)(n - at < kPiece ? n - at : kPiece), dt = (int)(meta & 15);
-        const double w = p < stream_pieces ? piece_norm_of<INF, true>(t.src[e], dt, at, len) : piece_norm_of<INF, false>(t.src[e], dt, at, len);
+        const PieceOf q = piece_of(t, e, p);
+        const double w = p < stream_pieces ? piece_norm_of<INF, true>(q.src, q.st, q.at, q.len) : piece_norm_of<INF, false>(q.src, q.st, q.at, q.len);
         v = INF ? max_nan(v, w) : v + w;
     }
     v = block_join(v, INF, sh);
@@ -186,14 +196,11 @@ template <bool OUT> __global__ __launch_bounds__(kThreads) void grad_scale_kerne
     int e = t.count - 1;
     for (int p = t.first[t.count] - 1 - (int)blockIdx.x; p >= 0; p -= gridDim.x) {
         while (t.first[e] > p) --e;
-        const unsigned long long meta = t.meta[e];
-        const long long at = (long long)(p - t.first[e]) * kPiece, n = (long long)(meta >> 8);
-        const int len = (int)(n - at < kPiece ? n - at : kPiece);
-        const int st = (int)(meta & 15), dt = (int)((meta >> 4) & 15);
-        void* dst = OUT ? t.dst[e] : (void*)t.src[e];
-        if (st == DMN_DT_F32) piece_scale_to<float>(t.src[e], dst, OUT ? dt : DMN_DT_F32, at, len, f);
-        else if (st == DMN_DT_BF16) piece_scale_to<__bf16>(t.src[e], dst, OUT ? dt : DMN_DT_BF16, at, len, f);
-        else piece_scale_to<f16>(t.src[e], dst, OUT ? dt : DMN_DT_F16, at, len, f);
+        const PieceOf q = piece_of(t, e, p);
+        void* dst = OUT ? t.dst[e] : (void*)q.src;
+        if (q.st == DMN_DT_F32) piece_scale_to<float>(q.src, dst, OUT ? q.dt : DMN_DT_F32, q.at, q.len, f);
+        else if (q.st == DMN_DT_BF16) piece_scale_to<__bf16>(q.src, dst, OUT ? q.dt : DMN_DT_BF16, q.at, q.len, f);
+        else piece_scale_to<f16>(q.src, dst, OUT ? q.dt : DMN_DT_F16, q.at, q.len, f);
     }
 }
 
@@ -247,6 +254,7 @@ int blocks_per_launch(int n) {
 }
 
 // Hands `emit` one launch's table after the other with its workgroups; the partials' indices run on over the launches.
+// The third argument is the index of the last tensor in the table.
 template <bool OUT, typename F> int for_tables(const DmnGradTensor* t, int n, F emit) {
     ClipTable<OUT> tab;
     tab.count = 0;
@@ -257,14 +265,15 @@ template <bool OUT, typename F> int for_tables(const DmnGradTensor* t, int n, F 
     for (int i = 0; i < n && !rc; ++i) {
         if (t[i].numel > 0) {
             const int k = tab.count++;
-            tab.src[k] = t[i].src;
+            const int64_t pieces = (t[i].numel + kPiece - 1) / kPiece;
+            tab.where[k] = (unsigned long long)(uintptr_t)t[i].src | (unsigned long long)(t[i].src_dtype + 3 * t[i].dst_dtype) << 47 |
+                           (unsigned long long)(t[i].numel - (pieces - 1) * kPiece - 1) << 51;
             if (OUT) tab.dst[OUT ? k : 0] = t[i].dst;
-            tab.meta[k] = (unsigned long long)t[i].numel << 8 | (unsigned)t[i].dst_dtype << 4 | (unsigned)t[i].src_dtype;
-            tab.first[k + 1] = tab.first[k] + (int)((t[i].numel + kPiece - 1) / kPiece);
+            tab.first[k + 1] = tab.first[k] + (int)pieces;
         }
         if (tab.count == ClipTable<OUT>::K || (i == n - 1 && tab.count)) {
             const int pieces = tab.first[tab.count], blocks = pieces < most ? pieces : most;
-            rc = emit(tab, blocks);
+            rc = emit(tab, blocks, i);
             tab.part_base += blocks;
             tab.count = 0;
         }
@@ -295,6 +304,7 @@ extern "C" int dmn_clip_grads(const DmnGradTensor* tensors, int n_tensors, int i
         DMN_REQUIRE(t.numel >= 0 && t.numel < ((int64_t)1 << 40) && t.src_dtype >= 0 && t.src_dtype <= 2 && t.dst_dtype >= 0 && t.dst_dtype <= 2,
                     DMN_ERR_INVALID, "dmn_clip_grads: tensor %d has a bad size or type", i);
         if (t.numel == 0) continue;
+        DMN_REQUIRE(((uintptr_t)t.src | (uintptr_t)t.dst) >> 47 == 0, DMN_ERR_INVALID, "dmn_clip_grads: tensor %d has an impossible address", i);
         DMN_REQUIRE(t.src && (uintptr_t)t.src % dt_bytes(t.src_dtype) == 0 && (uintptr_t)t.dst % dt_bytes(t.dst_dtype) == 0, DMN_ERR_INVALID,
                     "dmn_clip_grads: tensor %d has no address, or one that is not aligned to its type", i);
         total += t.numel;
@@ -323,12 +333,18 @@ extern "C" int dmn_clip_grads(const DmnGradTensor* tensors, int n_tensors, int i
     // scaling of 403 M bfloat16 elements (0.8 GB) into float32, us: 125 + 499 with nothing kept, 130 + 490 with 80 MB, 156 +
     // 477 with 160 MB, 176 + 480 with everything through the caches.
     int64_t before = 0;
-    int rc = for_tables<false>(tensors, n_tensors, [&](const ClipTable<false>& t, int blocks) -> int {
+    int next = 0;   // tensor behind the launches so far
+    int rc = for_tables<false>(tensors, n_tensors, [&](const ClipTable<false>& t, int blocks, int last) -> int {
         int stream = 0;
-        for (int i = 0; i < t.count && before < bytes - kKeep; ++i) {
-            before += (int64_t)(t.meta[i] >> 8) * dt_bytes((int)(t.meta[i] & 15));
-            stream = t.first[i + 1];
-            if (before > bytes - kKeep) stream -= (int)((before - (bytes - kKeep)) / dt_bytes((int)(t.meta[i] & 15)) / kPiece);
+        for (int k = 0; next <= last; ++next) {
+            if (tensors[next].numel == 0) continue;
+            const int size = dt_bytes(tensors[next].src_dtype);
+            if (before < bytes - kKeep) {
+                before += tensors[next].numel * size;
+                stream = t.first[k + 1];
+                if (before > bytes - kKeep) stream -= (int)((before - (bytes - kKeep)) / size / kPiece);
+            }
+            ++k;
         }
         if (inf_norm) grad_norm_kernel<true><<<blocks, kThreads, 0, s>>>(t, part, stream);
         else grad_norm_kernel<false><<<blocks, kThreads, 0, s>>>(t, part, stream);
@@ -343,7 +359,7 @@ extern "C" int dmn_clip_grads(const DmnGradTensor* tensors, int n_tensors, int i
         return DMN_OK;
     }
     c.write_norm = 1;
-    auto scale = [&](const auto& t, int blocks) -> int {
+    auto scale = [&](const auto& t, int blocks, int) -> int {
         grad_scale_kernel<<<blocks, kThreads, 0, s>>>(t, c);
         c.write_norm = 0;
         DMN_BLOCK_LAUNCH_CHECK();

@@ -325,7 +325,7 @@ def clip_grad_norm_(parameters: Union[torch.Tensor, Iterable[torch.Tensor]], max
     `grad_scale` multiplies the gradients first (1 / world_size behind a summing all-reduce, or an inverse loss scale); the
     norm is that of the scaled ones. `out`: tensors that receive the result in the parameters' place (entry i for parameter
     i, same shape, contiguous, float32 / bfloat16 / float16), the gradients stay as they are. Gradients may be float32,
-    bfloat16 and float16 side by side and are read and scaled in two launches for up to 192 of them; they must be on one
+    bfloat16 and float16 side by side and are read and scaled in two launches for up to 330 of them (196 with `out`); they must be on one
     device. A gradient that shares memory with another one is refused: it would be scaled more than once.
 
     This is the clip for gradients in tensors of their own (the autograd route of `DDPM.training_step`); `UnetTrainer` clips
