@@ -81,7 +81,7 @@ struct GemmArgs {
     const void *a, *b;           // A(m, k): K: a[m * lda + k], X: a[k * lda + m]; B(n, k) alike
     long long lda, ldb;
     int M, N, K;
-    int splits, tiles_per_split; // the k tiles are shared out over gridDim.y workgroups
+    int splits, tiles_per_split; // the k tiles are shared out over so many workgroups
     float* part;                 // splits > 1: [splits][M][N] partial products; else the epilogue below
     const void* bias;            // [N] or null
     const void* res;             // [M][ldr] or null, added behind the activation
@@ -262,7 +262,7 @@ template <typename T> __device__ __forceinline__ void load_bias(const GemmArgs& 
 // every wave, in turn, 16 rows at a time) it comes to hold 16 bytes of a row, so that rows are read and written in whole
 // pieces. The vector units do this while the matrix cores stand still, so it is kept short: a lane's columns stay the same
 // (its bias is read once), and tiles inside the matrix check nothing.
-template <typename T, int FM, int FN, bool EDGE> __device__ __forceinline__ void store_rows(const GemmArgs& g, f32x4 (&acc)[FM][FN], int m0, int n0, char* lds, int act) {
+template <typename T, int FM, int FN, bool EDGE> __device__ __forceinline__ void store_rows(const GemmArgs& g, f32x4 (&acc)[FM][FN], int m0, int n0, int split, char* lds, int act) {
     constexpr int V = Pack<T>::N, WN = FN * 16, PITCH = WN + 4, LPR = WN / V, ROWS = 64 / LPR;
     const int lane = threadIdx.x & 63;
     const int c = lane % LPR * V, n = n0 + c;
@@ -285,7 +285,7 @@ template <typename T, int FM, int FN, bool EDGE> __device__ __forceinline__ void
             }
             if (EDGE && (m >= g.M || n >= g.N)) continue;
             if (g.part) {
-                float* p = g.part + ((long long)blockIdx.y * g.M + m) * g.N;
+                float* p = g.part + ((long long)split * g.M + m) * g.N;
 #pragma unroll
                 for (int e = 0; e < V; e += 4) {
                     const f32x4 q = {v[e], v[e + 1], v[e + 2], v[e + 3]};
@@ -298,12 +298,12 @@ template <typename T, int FM, int FN, bool EDGE> __device__ __forceinline__ void
         }
     }
 }
-template <typename T, bool FORWARD, int FM, int FN> __device__ __forceinline__ void store_tile(const GemmArgs& g, f32x4 (&acc)[FM][FN], int m0, int n0, char* lds) {
-    if (m0 + FM * 16 > g.M || n0 + FN * 16 > g.N) store_rows<T, FM, FN, true>(g, acc, m0, n0, lds, FORWARD ? g.act : ACT_NONE);
-    else if (FORWARD && g.act == ACT_GELU) store_rows<T, FM, FN, false>(g, acc, m0, n0, lds, ACT_GELU);
-    else if (FORWARD && g.act == ACT_SILU) store_rows<T, FM, FN, false>(g, acc, m0, n0, lds, ACT_SILU);
-    else if (FORWARD && g.act == ACT_RELU) store_rows<T, FM, FN, false>(g, acc, m0, n0, lds, ACT_RELU);
-    else store_rows<T, FM, FN, false>(g, acc, m0, n0, lds, ACT_NONE);
+template <typename T, bool FORWARD, int FM, int FN> __device__ __forceinline__ void store_tile(const GemmArgs& g, f32x4 (&acc)[FM][FN], int m0, int n0, int split, char* lds) {
+    if (m0 + FM * 16 > g.M || n0 + FN * 16 > g.N) store_rows<T, FM, FN, true>(g, acc, m0, n0, split, lds, FORWARD ? g.act : ACT_NONE);
+    else if (FORWARD && g.act == ACT_GELU) store_rows<T, FM, FN, false>(g, acc, m0, n0, split, lds, ACT_GELU);
+    else if (FORWARD && g.act == ACT_SILU) store_rows<T, FM, FN, false>(g, acc, m0, n0, split, lds, ACT_SILU);
+    else if (FORWARD && g.act == ACT_RELU) store_rows<T, FM, FN, false>(g, acc, m0, n0, split, lds, ACT_RELU);
+    else store_rows<T, FM, FN, false>(g, acc, m0, n0, split, lds, ACT_NONE);
 }
 
 // Tile of workgroup `b`: workgroups go round the eight XCDs, each with an L2 of its own, so each XCD gets a run of
@@ -332,7 +332,7 @@ template <int N> struct Int { static constexpr int value = N; };
 // 128-byte rows in LDS (64-byte rows request half cache lines: 262 instead of 238 us) brought is the step from 366 to 238
 // us for 8192 x 2048 into 8192.
 template <typename T, bool XA, bool XB, int BM, int BN, int WM, int WN, int S>
-__global__ __launch_bounds__((BM / WM) * (BN / WN) * 64) void gemm_pipe_kernel(const GemmArgs g) {
+__device__ __forceinline__ void product_tile(const GemmArgs& g, int tile, int split, char* lds) {
     constexpr int NT = (BM / WM) * (BN / WN) * 64, KB = 128;
     typedef Tile<T, XA, BM, KB> TA;
     typedef Tile<T, XB, BN, KB> TB;
@@ -342,13 +342,12 @@ __global__ __launch_bounds__((BM / WM) * (BN / WN) * 64) void gemm_pipe_kernel(c
     constexpr int BK = TA::BK, A_BYTES = BM * KB, STAGE = (BM + BN) * KB, FM = WM / 16, FN = WN / 16;
     constexpr int WAIT = (S - 2) * (SA::PER + SB::PER);
     static_assert(BK == 2 * Frag<T>::KSTEP && S >= 2 && WAIT + SA::PER + SB::PER < 64, "pipeline");
-    extern __shared__ __attribute__((aligned(16))) char lds[];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int wm = wave % (BM / WM) * WM, wn = wave / (BM / WM) * WN;
     int im, in;
-    tile_of(blockIdx.x, (g.M + BM - 1) / BM, (g.N + BN - 1) / BN, im, in);
+    tile_of(tile, (g.M + BM - 1) / BM, (g.N + BN - 1) / BN, im, in);
     const int m0 = im * BM, n0 = in * BN;
-    const int k_tiles = (g.K + BK - 1) / BK, t0 = blockIdx.y * g.tiles_per_split;
+    const int k_tiles = (g.K + BK - 1) / BK, t0 = split * g.tiles_per_split;
     const int t1 = t0 + g.tiles_per_split < k_tiles ? t0 + g.tiles_per_split : k_tiles;
     int left = (t1 * BK < g.K ? t1 * BK : g.K) - t0 * BK;   // k rows that the next requests may still take
     SA sa;
@@ -411,7 +410,34 @@ __global__ __launch_bounds__((BM / WM) * (BN / WN) * 64) void gemm_pipe_kernel(c
     }
     asm volatile("s_waitcnt vmcnt(0)" : : : "memory");
     __syncthreads();   // the requests behind the end have landed, the tiles' memory is free
-    store_tile<T, !XB, FM, FN>(g, acc, m0 + wm, n0 + wn, lds);
+    store_tile<T, !XB, FM, FN>(g, acc, m0 + wm, n0 + wn, split, lds);
+}
+template <typename T, bool XA, bool XB, int BM, int BN, int WM, int WN, int S>
+__global__ __launch_bounds__((BM / WM) * (BN / WN) * 64) void gemm_pipe_kernel(const GemmArgs g) {
+    extern __shared__ __attribute__((aligned(16))) char lds[];
+    product_tile<T, XA, XB, BM, BN, WM, WN, S>(g, blockIdx.x, blockIdx.y, lds);
+}
+// Both of the backward's products in one launch: they read the same dz, and neither's tiles alone fill the chip evenly (one after
+// the other each has its own first requests, last tiles and launch). The product with the longer tiles goes in front. Both
+// products, one after the other and so (us): 4096 x 1024 into 4096 bf16 85 : 71, 2048 x 1024 into 1024 27 : 19, 4096 x 320 into
+// 1280 29 : 19.5, 256 x 320 into 320 8.0 : 5.0, 16384 x 256 into 1024 float32 149 : 139; 4096^3 bf16, whose 256 x 256 tiles come
+// out even, 214 : 265.
+struct PairArgs {
+    GemmArgs dx, dw;
+    int dx_tiles, dw_tiles;   // of one split
+    int dx_at, dw_at;         // first workgroup of each: one of them 0
+};
+template <typename T, int BM, int BN, int WM, int WN, int S>
+__global__ __launch_bounds__((BM / WM) * (BN / WN) * 64) void gemm_pair_kernel(const PairArgs p) {
+    extern __shared__ __attribute__((aligned(16))) char lds[];
+    const int b = blockIdx.x;
+    if (p.dx_at ? b >= p.dx_at : b < p.dw_at) {
+        const int i = b - p.dx_at, split = i / p.dx_tiles;
+        product_tile<T, false, true, BM, BN, WM, WN, S>(p.dx, i - split * p.dx_tiles, split, lds);
+    } else {
+        const int i = b - p.dw_at, split = i / p.dw_tiles;
+        product_tile<T, true, true, BM, BN, WM, WN, S>(p.dw, i - split * p.dw_tiles, split, lds);
+    }
 }
 
 // The forward product for few rows (M <= 16 MF): bound by reading the weight once. A workgroup takes 16 NF columns; its waves
@@ -664,6 +690,7 @@ inline long long ceil_div(long long a, long long b) { return (a + b - 1) / b; }
 // one more launch.
 struct GemmPlan {
     int tile, splits, per;   // index into kTiles; k tiles are counted in 128 bytes of k
+    double us;
 };
 struct TileShape {
     int bm, bn, together;
@@ -674,33 +701,59 @@ const TileShape kTiles[4] = {{256, 256, 1, 1.60, 1.12, 8.0, 7.4, 7.2, 22.0},
                              {128, 128, 2, 0.50, 0.68, 4.0, 1.9, 2.0, 9.0},
                              {64, 64, 4, 0.22, 0.28, 3.0, 0.55, 0.70, 6.0}};
 
+double join_us(int splits, int M, int N) { return splits > 1 ? 3.0 + (double)splits * M * N * 8 / 4e6 : 0.0; }
 GemmPlan gemm_plan(int M, int N, int K, int dtype) {
-    const int bk = 128 / elem(dtype);
-    const long long kt = ceil_div(K, bk);
-    GemmPlan best{3, 1, (int)kt};
-    double best_us = 1e30;
+    const bool f32 = dtype == DMN_DT_F32;
+    const long long kt = ceil_div(K, 128 / elem(dtype));
+    GemmPlan best{3, 1, (int)kt, 1e30};
     for (int i = 0; i < 4; ++i) {
         const TileShape& t = kTiles[i];
-        const bool f32 = dtype == DMN_DT_F32;
         const double step = f32 ? t.step32 : t.step16, least = f32 ? t.least32 : t.least16, ends = f32 ? t.ends32 : t.ends16;
         const long long tiles = ceil_div(M, t.bm) * ceil_div(N, t.bn);
-        for (int splits = 1; splits <= 64; splits *= 2) {
-            if (splits > 1 && kt / splits < 4) break;
+        for (int splits = 1; splits <= 64 && (splits == 1 || kt / splits >= 4); splits *= 2) {
             const long long per = ceil_div(kt, splits), on_cu = ceil_div(tiles * splits, 256);
             const double all = tiles * splits > 128 ? on_cu * per * step : 0, one = per * least;
-            double us = (all > one ? all : one) + ends * ceil_div(on_cu, t.together);
-            if (splits > 1) us += 3.0 + (double)splits * M * N * 8 / 4e6;
-            if (us < best_us) {
-                best_us = us;
-                best = {i, (int)ceil_div(kt, per), (int)per};
-            }
+            const double us = (all > one ? all : one) + ends * ceil_div(on_cu, t.together) + join_us(splits, M, N);
+            if (us < best.us) best = {i, (int)ceil_div(kt, per), (int)per, us};
         }
     }
     return best;
 }
+// dx and dw in one launch, where that is faster than one after the other: the CUs that one product's tiles leave without work
+// take the other's, and tiles of both share a CU. The sum of their k tiles counts, and the longest one among its neighbours;
+// the ends of all but the last lie beside other tiles' steps.
+struct PairPlan {
+    bool together;
+    GemmPlan dx, dw;
+};
+PairPlan pair_plan(int rows, int in, int out, int dtype) {
+    const bool f32 = dtype == DMN_DT_F32;
+    const int bk = 128 / elem(dtype);
+    const long long kx = ceil_div(out, bk), kw = ceil_div(rows, bk);
+    PairPlan best{false, gemm_plan(rows, in, out, dtype), gemm_plan(out, in, rows, dtype)};
+    double best_us = best.dx.us + best.dw.us;
+    for (int i = 2; i < 4; ++i) {
+        const TileShape& t = kTiles[i];
+        const double step = f32 ? t.step32 : t.step16, least = f32 ? t.least32 : t.least16, ends = f32 ? t.ends32 : t.ends16;
+        const long long tx = ceil_div(rows, t.bm) * ceil_div(in, t.bn), tw = ceil_div(out, t.bm) * ceil_div(in, t.bn);
+        for (int sx = 1; sx <= 64 && (sx == 1 || kx / sx >= 4); sx *= 2)
+            for (int sw = 1; sw <= 64 && (sw == 1 || kw / sw >= 4); sw *= 2) {
+                const long long px = ceil_div(kx, sx), pw = ceil_div(kw, sw), longest = px > pw ? px : pw;
+                const long long tiles = tx * sx + tw * sw, on_cu = ceil_div(tiles, 256);
+                const double all = tiles > 128 ? step * on_cu * (tx * sx * px + tw * sw * pw) / tiles : 0;
+                const double one = longest * (on_cu > 1 ? 2 * step : least);
+                const double us = (all > one ? all : one) + ends + join_us(sx, rows, in) + join_us(sw, out, in);
+                if (us < best_us) {
+                    best_us = us;
+                    best = {true, {i, (int)ceil_div(kx, px), (int)px, us}, {i, (int)ceil_div(kw, pw), (int)pw, us}};
+                }
+            }
+    }
+    return best;
+}
+size_t part_bytes(const GemmPlan& p, int M, int N) { return p.splits > 1 ? block_align256((size_t)p.splits * M * N * sizeof(float)) : 0; }
 size_t gemm_workspace(int M, int N, int K, int dtype) {
-    const GemmPlan p = gemm_plan(M, N, K, dtype);
-    return p.splits > 1 ? block_align256((size_t)p.splits * M * N * sizeof(float)) : 0;
+    return part_bytes(gemm_plan(M, N, K, dtype), M, N);
 }
 
 // An operand in memory: rows of `width` elements, `ld` apart.
@@ -781,20 +834,45 @@ template <typename T> int few_rows_run(const GemmArgs& g, hipStream_t s) {
     return cols >= 1024 ? few_rows_launch<T, 4, 4, 4>(g, s) : cols >= 512 ? few_rows_launch<T, 4, 2, 8>(g, s) : few_rows_launch<T, 4, 1, 16>(g, s);
 }
 
-// C = sum_k A B with the operands on 16-byte boundaries (copy_operands).
-template <typename T, bool XA, bool XB> int gemm_run(GemmArgs& g, int dtype, void* ws, hipStream_t s) {
-    const GemmPlan p = gemm_plan(g.M, g.N, g.K, dtype);
+void set_plan(GemmArgs& g, const GemmPlan& p, void* ws) {
     g.splits = p.splits;
     g.tiles_per_split = p.per;
     g.part = p.splits > 1 ? (float*)ws : nullptr;
+}
+template <typename T> int join_run(const GemmArgs& g, hipStream_t s) {
+    if (g.splits == 1) return DMN_OK;
+    // eight threads per piece where there are few of them
+    return g.splits >= 8 && (long long)g.M * g.N < (1 << 20) ? join_launch<T, 8>(g, s) : join_launch<T, 1>(g, s);
+}
+// C = sum_k A B with the operands on 16-byte boundaries (copy_operands).
+template <typename T, bool XA, bool XB> int gemm_run(GemmArgs& g, int dtype, void* ws, hipStream_t s) {
+    const GemmPlan p = gemm_plan(g.M, g.N, g.K, dtype);
+    set_plan(g, p, ws);
     int rc;
     if (p.tile == 0) rc = pipe_launch<T, XA, XB, 256, 256, 128, 64, 2>(g, s);
     else if (p.tile == 1) rc = pipe_launch<T, XA, XB, 128, 128, 64, 32, 4>(g, s);
     else if (p.tile == 2) rc = pipe_launch<T, XA, XB, 128, 128, 64, 32, 2>(g, s);
     else rc = pipe_launch<T, XA, XB, 64, 64, 32, 32, 2>(g, s);
-    if (rc || p.splits == 1) return rc;
-    // eight threads per piece where there are few of them
-    return p.splits >= 8 && (long long)g.M * g.N < (1 << 20) ? join_launch<T, 8>(g, s) : join_launch<T, 1>(g, s);
+    return rc ? rc : join_run<T>(g, s);
+}
+template <typename T, int BM, int BN, int WM, int WN, int S> int pair_launch(const PairArgs& a, hipStream_t s) {
+    constexpr int NT = (BM / WM) * (BN / WN) * 64, LDS = S * (BM + BN) * 128;
+    static_assert(LDS <= 65536, "LDS without an attribute");
+    gemm_pair_kernel<T, BM, BN, WM, WN, S><<<(unsigned)(a.dx_tiles * a.dx.splits + a.dw_tiles * a.dw.splits), NT, LDS, s>>>(a);
+    DMN_BLOCK_LAUNCH_CHECK();
+    return DMN_OK;
+}
+// dx and dw, each with its epilogue or join; their partial products lie one behind the other in the workspace.
+template <typename T> int pair_run(GemmArgs& dx, GemmArgs& dw, const PairPlan& p, char* ws, hipStream_t s) {
+    set_plan(dx, p.dx, ws);
+    set_plan(dw, p.dw, ws + part_bytes(p.dx, dx.M, dx.N));
+    const TileShape& t = kTiles[p.dx.tile];
+    PairArgs a{dx, dw, (int)(ceil_div(dx.M, t.bm) * ceil_div(dx.N, t.bn)), (int)(ceil_div(dw.M, t.bm) * ceil_div(dw.N, t.bn)), 0, 0};
+    if (p.dx.per >= p.dw.per) a.dw_at = a.dx_tiles * dx.splits;
+    else a.dx_at = a.dw_tiles * dw.splits;
+    int rc = p.dx.tile == 2 ? pair_launch<T, 128, 128, 64, 32, 2>(a, s) : pair_launch<T, 64, 64, 32, 32, 2>(a, s);
+    if (!rc) rc = join_run<T>(dx, s);
+    return rc ? rc : join_run<T>(dw, s);
 }
 
 template <typename T> int forward_run(GemmArgs& g, int dtype, char* ws, hipStream_t s) {
@@ -868,30 +946,27 @@ int backward_run(const void* dy, long long lddy, const void* x, long long ldx, c
     if (dx) list[n++] = &w_;
     if (dw) list[n++] = &x_;
     int rc = copy_operands<T>(list, n, dtype, ws, s);
-    if (dx && !rc) {
-        GemmArgs g{};
-        g.a = z_.p;
-        g.lda = z_.ld;
-        g.b = w_.p;
-        g.ldb = w_.ld;
-        g.M = rows;
-        g.N = in;
-        g.K = out;
-        g.y = dx;
-        rc = gemm_run<T, false, true>(g, dtype, ws, s);
+    if (rc || (!dx && !dw)) return rc;
+    GemmArgs gx{}, gw{};
+    gx.a = gw.a = z_.p;
+    gx.lda = gw.lda = z_.ld;
+    gx.b = w_.p;
+    gx.ldb = w_.ld;
+    gx.M = rows;
+    gx.K = out;
+    gx.y = dx;
+    gw.b = x_.p;
+    gw.ldb = x_.ld;
+    gw.M = out;
+    gw.K = rows;
+    gw.y = dw;
+    gx.N = gw.N = in;
+    if (dx && dw) {
+        const PairPlan p = pair_plan(rows, in, out, dtype);
+        if (p.together) return pair_run<T>(gx, gw, p, ws, s);
     }
-    if (dw && !rc) {
-        GemmArgs g{};
-        g.a = z_.p;
-        g.lda = z_.ld;
-        g.b = x_.p;
-        g.ldb = x_.ld;
-        g.M = out;
-        g.N = in;
-        g.K = rows;
-        g.y = dw;
-        rc = gemm_run<T, true, true>(g, dtype, ws, s);
-    }
+    if (dx) rc = gemm_run<T, false, true>(gx, dtype, ws, s);
+    if (dw && !rc) rc = gemm_run<T, true, true>(gw, dtype, ws, s);
     return rc;
 }
 
@@ -937,9 +1012,11 @@ extern "C" size_t dmn_linear_backward_workspace_bytes(const void* dy, int64_t ld
                                                       int in, int out, int activation, int dtype) {
     if (rows <= 0 || rows >= (1 << 27) || in <= 0 || out <= 0 || dtype < 0 || dtype > 2) return 0;
     const size_t dx = gemm_workspace((int)rows, in, out, dtype), dw = gemm_workspace(out, in, (int)rows, dtype);
+    const PairPlan p = pair_plan((int)rows, in, out, dtype);
+    const size_t pair = p.together ? part_bytes(p.dx, (int)rows, in) + part_bytes(p.dw, out, in) : 0, one = dx > dw ? dx : dw;
     const size_t dz = activation != ACT_NONE ? block_align256((size_t)rows * padded(out, dtype) * elem(dtype)) : copy_bytes({dy, lddy, (int)rows, out}, dtype);
     return block_align256((size_t)dz_runs((int)rows) * out * sizeof(float)) + dz + copy_bytes({x, ldx, (int)rows, in}, dtype) +
-           copy_bytes({weight, in, out, in}, dtype) + (dx > dw ? dx : dw);
+           copy_bytes({weight, in, out, in}, dtype) + (pair > one ? pair : one);
 }
 
 extern "C" int dmn_linear_backward(const void* dy, int64_t lddy, const void* x, int64_t ldx, const void* weight, const void* z, void* dx,

@@ -320,6 +320,13 @@ def test_linear_large_and_split_products(m, k, n):
     linear_case(m, k, n, HF, None, True, False, seed=30)
 
 
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("m,k,n", [(4096, 320, 1280), (64, 1024, 1024), (2047, 1021, 1030), (6000, 1024, 1000), (8192, 128, 512), (256, 320, 320)])
+def test_linear_backward_products_beside_each_other(dtype, m, k, n):
+    """dx and dW from one launch: either's k split, odd sizes, either's tiles in front."""
+    linear_case(m, k, n, dtype, "silu", True, False, seed=60)
+
+
 def test_linear_float32_large():
     linear_case(1555, 1032, 520, F32, "silu", True, True)
     linear_case(4096, 64, 256, F32, "gelu", True, False)
