@@ -417,6 +417,29 @@ __global__ __launch_bounds__((BM / WM) * (BN / WN) * 64) void gemm_pipe_kernel(c
     extern __shared__ __attribute__((aligned(16))) char lds[];
     product_tile<T, XA, XB, BM, BN, WM, WN, S>(g, blockIdx.x, blockIdx.y, lds);
 }
+// out[col] = sum over `parts` partial rows, in a fixed order: 32 columns per workgroup of NT threads, NT / 32 threads per column
+struct ColumnJoin {
+    const float* part;   // [parts][n]
+    int parts, n;
+    void* out;           // null: nothing to do
+};
+template <typename T, int NT> __device__ __forceinline__ void column_join(const ColumnJoin& j, int block, float* sh) {
+    constexpr int G = NT / 32;
+    const int c = threadIdx.x & 31, g = threadIdx.x >> 5, col = block * 32 + c;
+    float s = 0.f;
+    if (col < j.n) {
+#pragma unroll 8
+        for (int i = g; i < j.parts; i += G) s += j.part[(long long)i * j.n + col];
+    }
+    sh[g * 32 + c] = s;
+    __syncthreads();
+    if (g == 0 && col < j.n) {
+        float t = 0.f;
+#pragma unroll
+        for (int i = 0; i < G; ++i) t += sh[i * 32 + c];
+        ((T*)j.out)[col] = (T)t;
+    }
+}
 // Both of the backward's products in one launch: they read the same dz, and neither's tiles alone fill the chip evenly (one after
 // the other each has its own first requests, last tiles and launch). The product with the longer tiles goes in front. Both
 // products, one after the other and so (us): 4096 x 1024 into 4096 bf16 85 : 71, 2048 x 1024 into 1024 27 : 19, 4096 x 320 into
@@ -426,12 +449,16 @@ struct PairArgs {
     GemmArgs dx, dw;
     int dx_tiles, dw_tiles;   // of one split
     int dx_at, dw_at;         // first workgroup of each: one of them 0
+    int db_at;                // the workgroups from here on join the column sums: a launch less
+    ColumnJoin db;
 };
 template <typename T, int BM, int BN, int WM, int WN, int S>
 __global__ __launch_bounds__((BM / WM) * (BN / WN) * 64) void gemm_pair_kernel(const PairArgs p) {
     extern __shared__ __attribute__((aligned(16))) char lds[];
     const int b = blockIdx.x;
-    if (p.dx_at ? b >= p.dx_at : b < p.dw_at) {
+    if (b >= p.db_at) {
+        column_join<T, (BM / WM) * (BN / WN) * 64>(p.db, b - p.db_at, (float*)lds);
+    } else if (p.dx_at ? b >= p.dx_at : b < p.dw_at) {
         const int i = b - p.dx_at, split = i / p.dx_tiles;
         product_tile<T, false, true, BM, BN, WM, WN, S>(p.dx, i - split * p.dx_tiles, split, lds);
     } else {
@@ -629,23 +656,9 @@ template <typename T> __global__ __launch_bounds__(256) void dz_kernel(const DzA
         if (col < a.N) a.part[(long long)blockIdx.y * a.N + col] = t;
     }
 }
-// out[col] = sum over `parts` partial rows, in a fixed order: 32 columns per workgroup, 8 threads per column
-template <typename T> __global__ __launch_bounds__(256) void column_join_kernel(const float* part, int parts, int n, T* out) {
-    __shared__ float sh[8][33];
-    const int c = threadIdx.x & 31, g = threadIdx.x >> 5, col = blockIdx.x * 32 + c;
-    float s = 0.f;
-    if (col < n) {
-#pragma unroll 8
-        for (int i = g; i < parts; i += 8) s += part[(long long)i * n + col];
-    }
-    sh[g][c] = s;
-    __syncthreads();
-    if (g == 0 && col < n) {
-        float t = 0.f;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) t += sh[i][c];
-        out[col] = (T)t;
-    }
+template <typename T> __global__ __launch_bounds__(256) void column_join_kernel(const ColumnJoin j) {
+    __shared__ float sh[256];
+    column_join<T, 256>(j, blockIdx.x, sh);
 }
 
 template <typename T> __global__ __launch_bounds__(256) void zero_kernel(T* p, long long n) {
@@ -858,16 +871,17 @@ template <typename T, bool XA, bool XB> int gemm_run(GemmArgs& g, int dtype, voi
 template <typename T, int BM, int BN, int WM, int WN, int S> int pair_launch(const PairArgs& a, hipStream_t s) {
     constexpr int NT = (BM / WM) * (BN / WN) * 64, LDS = S * (BM + BN) * 128;
     static_assert(LDS <= 65536, "LDS without an attribute");
-    gemm_pair_kernel<T, BM, BN, WM, WN, S><<<(unsigned)(a.dx_tiles * a.dx.splits + a.dw_tiles * a.dw.splits), NT, LDS, s>>>(a);
+    gemm_pair_kernel<T, BM, BN, WM, WN, S><<<(unsigned)(a.db_at + (a.db.out ? ceil_div(a.db.n, 32) : 0)), NT, LDS, s>>>(a);
     DMN_BLOCK_LAUNCH_CHECK();
     return DMN_OK;
 }
-// dx and dw, each with its epilogue or join; their partial products lie one behind the other in the workspace.
-template <typename T> int pair_run(GemmArgs& dx, GemmArgs& dw, const PairPlan& p, char* ws, hipStream_t s) {
+// dx, dw and the join of db's partial sums; their partial products lie one behind the other in the workspace.
+template <typename T> int pair_run(GemmArgs& dx, GemmArgs& dw, const ColumnJoin& db, const PairPlan& p, char* ws, hipStream_t s) {
     set_plan(dx, p.dx, ws);
     set_plan(dw, p.dw, ws + part_bytes(p.dx, dx.M, dx.N));
     const TileShape& t = kTiles[p.dx.tile];
-    PairArgs a{dx, dw, (int)(ceil_div(dx.M, t.bm) * ceil_div(dx.N, t.bn)), (int)(ceil_div(dw.M, t.bm) * ceil_div(dw.N, t.bn)), 0, 0};
+    PairArgs a{dx, dw, (int)(ceil_div(dx.M, t.bm) * ceil_div(dx.N, t.bn)), (int)(ceil_div(dw.M, t.bm) * ceil_div(dw.N, t.bn)), 0, 0, 0, db};
+    a.db_at = a.dx_tiles * dx.splits + a.dw_tiles * dw.splits;
     if (p.dx.per >= p.dw.per) a.dw_at = a.dx_tiles * dx.splits;
     else a.dx_at = a.dw_tiles * dw.splits;
     int rc = p.dx.tile == 2 ? pair_launch<T, 128, 128, 64, 32, 2>(a, s) : pair_launch<T, 64, 64, 32, 32, 2>(a, s);
@@ -915,6 +929,7 @@ int backward_run(const void* dy, long long lddy, const void* x, long long ldx, c
     float* part = (float*)ws;
     const int runs = dz_runs(rows);
     ws += block_align256((size_t)runs * out * sizeof(float));
+    ColumnJoin join{part, runs, out, nullptr};
     Operand z_{dy, lddy, rows, out}, w_{w, in, out, in}, x_{x, ldx, rows, in};
     if (act != ACT_NONE || db) {
         DzArgs a{};
@@ -929,10 +944,7 @@ int backward_run(const void* dy, long long lddy, const void* x, long long ldx, c
         a.act = act;
         dz_kernel<T><<<dim3((unsigned)ceil_div(out, 16 * Pack<T>::N), runs), 256, 0, s>>>(a);
         DMN_BLOCK_LAUNCH_CHECK();
-        if (db) {
-            column_join_kernel<T><<<(unsigned)ceil_div(out, 32), 256, 0, s>>>(part, runs, out, (T*)db);
-            DMN_BLOCK_LAUNCH_CHECK();
-        }
+        join.out = db;
         if (act != ACT_NONE) {
             z_.p = ws;
             z_.ld = a.lddz;
@@ -946,7 +958,7 @@ int backward_run(const void* dy, long long lddy, const void* x, long long ldx, c
     if (dx) list[n++] = &w_;
     if (dw) list[n++] = &x_;
     int rc = copy_operands<T>(list, n, dtype, ws, s);
-    if (rc || (!dx && !dw)) return rc;
+    if (rc) return rc;
     GemmArgs gx{}, gw{};
     gx.a = gw.a = z_.p;
     gx.lda = gw.lda = z_.ld;
@@ -963,7 +975,11 @@ int backward_run(const void* dy, long long lddy, const void* x, long long ldx, c
     gx.N = gw.N = in;
     if (dx && dw) {
         const PairPlan p = pair_plan(rows, in, out, dtype);
-        if (p.together) return pair_run<T>(gx, gw, p, ws, s);
+        if (p.together) return pair_run<T>(gx, gw, join, p, ws, s);
+    }
+    if (join.out) {
+        column_join_kernel<T><<<(unsigned)ceil_div(out, 32), 256, 0, s>>>(join);
+        DMN_BLOCK_LAUNCH_CHECK();
     }
     if (dx) rc = gemm_run<T, false, true>(gx, dtype, ws, s);
     if (dw && !rc) rc = gemm_run<T, true, true>(gw, dtype, ws, s);
