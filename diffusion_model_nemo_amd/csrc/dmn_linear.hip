@@ -449,7 +449,8 @@ struct PairArgs {
     GemmArgs dx, dw;
     int dx_tiles, dw_tiles;   // of one split
     int dx_at, dw_at;         // first workgroup of each: one of them 0
-    int db_at;                // the workgroups from here on join the column sums: a launch less
+    int db_at;                // the workgroups from here on join the column sums: a launch less, beside the last tiles (4096 x 1024
+                              // into 4096, whole step: own launch 139 us, in front of the tiles 136, behind them 129)
     ColumnJoin db;
 };
 template <typename T, int BM, int BN, int WM, int WN, int S>
