@@ -79,12 +79,13 @@ struct Rows {
     Tensor t;
     int64_t ld;
 };
-Rows rows_of(const Tensor& t) {
+Rows rows_of(const Tensor& t, int64_t limit = INT64_MAX) {   // strides from `limit` on are copied too
     const int64_t width = t.size(-1);
     if (t.is_contiguous()) return {t, width};
-    if (t.dim() == 2 && (t.stride(1) == 1 || width == 1) && t.stride(0) >= width) return {t, t.stride(0)};
+    if (t.dim() == 2 && (t.stride(1) == 1 || width == 1) && t.stride(0) >= width && t.stride(0) < limit) return {t, t.stride(0)};
     return {t.contiguous(), width};
 }
+constexpr int64_t kLinearStride = 1 << 20;   // dmn_linear_*: strides below it
 std::optional<Tensor> given(const Tensor& t) { return t.defined() ? std::optional<Tensor>(t) : std::nullopt; }
 Tensor or_none(const std::optional<Tensor>& t) { return t.has_value() ? *t : Tensor(); }
 Tensor new_like(const Tensor& t) { return at::empty(t.sizes(), t.options()); }
@@ -210,7 +211,7 @@ struct LinearNode : torch::autograd::Function<LinearNode> {
     static Tensor forward(AutogradContext* ctx, const Tensor& x, const Tensor& weight, const std::optional<Tensor>& bias_,
                           const std::optional<Tensor>& residual, int64_t act, int64_t stream) {
         const Tensor bias = or_none(bias_);
-        const Rows r = rows_of(x);
+        const Rows r = rows_of(x, kLinearStride);
         // the value in front of the activation is all that the backward needs of the forward's results
         const bool want_z = act != 0 && (x.requires_grad() || weight.requires_grad() || (bias.defined() && bias.requires_grad()));
         Tensor z;
@@ -230,7 +231,7 @@ struct LinearNode : torch::autograd::Function<LinearNode> {
             const Tensor &weight = saved[1], &bias = saved[2], &z = saved[3];
             const bool need_x = ctx->needs_input_grad(0), need_w = ctx->needs_input_grad(1), need_b = bias.defined() && ctx->needs_input_grad(2);
             if (need_x || need_w || need_b) {
-                const Rows x = rows_of(saved[0]), dy = rows_of(grads[0]);
+                const Rows x = rows_of(saved[0], kLinearStride), dy = rows_of(grads[0], kLinearStride);
                 c10::DeviceGuard guard(x.t.device());
                 const int64_t n = weight.size(0), width = weight.size(1), rows = x.t.numel() / width, act = ctx->saved_data["act"].toInt();
                 const int code = code_of(x.t.scalar_type());
@@ -270,7 +271,7 @@ Tensor linear(const Tensor& x, const Tensor& weight_, const std::optional<Tensor
         check_capture(capturing, x, {&x, &weight, &bias, &residual});
         return LinearNode::apply(x, weight, given(bias), given(residual), act, stream);
     }
-    return linear_run(rows_of(x), weight, bias, residual, act, stream, nullptr);
+    return linear_run(rows_of(x, kLinearStride), weight, bias, residual, act, stream, nullptr);
 }
 
 // ---- gradient clipping -------------------------------------------------------------------------------------------------

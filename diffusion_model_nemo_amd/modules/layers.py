@@ -32,7 +32,8 @@ def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Opt
                eps: float = 1e-5) -> torch.Tensor:
     """(x - mean) / sqrt(var + eps) * weight + bias over the last axis of `x` [..., width] (float32, bfloat16 or float16).
     `weight` and `bias` [width] (either may be None) are of x's type or float32, both alike; their gradients come in
-    that type. Rows with any stride are read in place for a 2-D `x`; other layouts are copied first."""
+    that type. Rows with any stride are read in place for a 2-D `x`; other layouts are copied first. The statistics are
+    float32: a row whose squared deviations add up to more than 3.4e38 comes out as zeros times weight plus bias."""
     return N.ops().layer_norm(x, weight, bias, eps, *_stream(x, "layer_norm"))
 
 
@@ -41,8 +42,8 @@ def linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] =
     """act(x weight^T + bias) + residual in one pass: `x` [..., in], `weight` [out, in], `bias` [out], `residual` [..., out],
     all of one type (float32, bfloat16 or float16); `activation` None, 'relu', 'silu' or 'gelu' (the exact one). The sum in
     front of the activation, the activation and the residual are formed in float32 and rounded once. For the backward with
-    an activation the value in front of it is kept, rounded to the type; rows with any stride are read in place for 2-D
-    tensors, other layouts are copied first."""
+    an activation the value in front of it is kept, rounded to the type; rows with any stride below 2^20 are read in
+    place for 2-D tensors, other layouts are copied first. `in` and `out` are below 2^20."""
     code = ACTIVATIONS.get(activation)
     if code is None:
         raise ValueError(f"activation must be one of {list(ACTIVATIONS)}, got {activation!r}")

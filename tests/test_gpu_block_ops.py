@@ -385,6 +385,66 @@ def test_linear_gradients_asked_for_one_by_one(kind, dtype):
             assert torch.equal(got, want[i]), (shape, i)
 
 
+@pytest.mark.parametrize("kind", [None, "gelu"])
+def test_linear_rows_a_million_elements_apart(kind):
+    """Views of a tensor with very long rows: x, the residual and the incoming gradient."""
+    from diffusion_model_nemo_amd.modules import linear
+    wide = randn((3, (1 << 20) + 72), 1, BF)
+    w, b = randn((48, 64), 2, BF, 0.125), randn((48,), 3, BF)
+    x, r, dy = wide[:, 8:72], wide[:, 100:148], wide[:, 1000:1048]
+    got = []
+    for at, rt, dt in ((x, r, dy), (x.contiguous(), r.contiguous(), dy.contiguous())):
+        leaves = [t.detach().requires_grad_(True) for t in (at, w, b, rt)]
+        y = linear(leaves[0], leaves[1], leaves[2], kind, leaves[3])
+        got.append((y,) + torch.autograd.grad(y, leaves, dt))
+    assert all(torch.equal(p, q) for p, q in zip(*got))
+
+
+def test_elements_behind_the_two_thousand_millionth():
+    """More than 2^31 elements in a tensor: the rows at its end, and sums that only rows at both ends feed."""
+    from diffusion_model_nemo_amd.modules import layer_norm, linear
+    from diffusion_model_nemo_amd.training import clip_grad_norm_
+    rows, n, k, ends = (1 << 20) + 3, 2056, 64, 40
+    at = torch.cat([torch.arange(ends, device="cuda"), torch.arange(rows - ends, rows, device="cuda")])
+    big = torch.zeros(rows, n, dtype=BF, device="cuda")
+    big[at] = randn((2 * ends, n), 1, BF)
+    dy = torch.zeros_like(big)
+    dy[at] = randn((2 * ends, n), 2, BF)
+    w, b = randn((n,), 3, BF, 0.1, 1.0), randn((n,), 4, BF)
+    leaves = [t.requires_grad_(True) for t in (big, w, b)]
+    y = layer_norm(*leaves)
+    grads = torch.autograd.grad(y, leaves, dy)
+    f = ln_formula(big[at].detach(), w.detach(), b.detach(), 1e-5, dy[at])
+    tol = ln_bounds(f, big[at].detach(), dy[at], BF, BF)
+    for name, got in (("y", y[at]), ("dx", grads[0][at]), ("dw", grads[1]), ("db", grads[2])):
+        close(got, f[name], tol[name], name)
+    assert not bool(grads[0][ends:rows - ends].any())
+    del y, grads, leaves
+    big = big.detach()
+
+    x, weight = randn((rows, k), 5, BF), randn((n, k), 6, BF, 0.125)
+    leaves = [x.requires_grad_(True), weight.requires_grad_(True)]
+    y = linear(*leaves, None, None, big)
+    xs, ds, wd = x.detach()[at], dy[at], weight.detach()
+    want, size = product(xs, wd.t())
+    want = want + big[at].double()
+    close(y[at], want, half_step(BF) * want.abs() + (k + 64) * U * (size + want.abs()) + floor_of(BF), "y")
+    dx, dw = torch.autograd.grad(y, leaves, dy)
+    del y
+    for got, (want, size), depth in ((dx[at], product(ds, wd), n), (dw, product(ds.t(), xs), 2 * ends)):
+        close(got, want, half_step(BF) * want.abs() + (depth + 64) * U * size + floor_of(BF), "dx, dw")
+    assert not bool(dx[ends:rows - ends].any())
+    del dx, dw, big
+
+    p = torch.nn.Parameter(torch.zeros(rows, n, dtype=BF, device="cuda"))
+    p.grad = dy
+    before = dy[at].clone()
+    norm = clip_grad_norm_(p, 1.0)
+    want = before.double().square().sum().sqrt()
+    assert abs(float(norm) - float(want)) <= 4 * U * float(want)
+    close(dy[at], before.double() / (want + 1e-6), (half_step(BF) + 4 * U) * (before.double() / want).abs() + floor_of(BF), "clipped")
+
+
 def test_linear_empty_batch():
     from diffusion_model_nemo_amd.modules import linear
     for kind in (None, "gelu"):
