@@ -445,6 +445,64 @@ def test_elements_behind_the_two_thousand_millionth():
     close(dy[at], before.double() / (want + 1e-6), (half_step(BF) + 4 * U) * (before.double() / want).abs() + floor_of(BF), "clipped")
 
 
+def test_linear_and_layer_norm_shared_repeated_and_interleaved_uses():
+    """One tensor as input and residual, one weight twice, a graph walked twice, recomputation, an input changed behind the
+    forward's back, two streams at once: all in bits, against the calls one by one."""
+    from torch.utils.checkpoint import checkpoint
+    from diffusion_model_nemo_amd.modules import layer_norm, linear
+    x, w, b = randn((777, 320), 1, BF), randn((320, 320), 2, BF, 0.05), randn((320,), 3, BF)
+    dy = randn((777, 320), 4, BF)
+
+    def step(x, w, b, r):
+        leaves = [t.detach().clone().requires_grad_(True) for t in (x, w, b, r)]
+        y = linear(layer_norm(leaves[0], None, leaves[2]), leaves[1], leaves[2], "gelu", leaves[3])
+        return (y.detach(),) + torch.autograd.grad(y, leaves, dy)
+
+    def plain(x, w, b, r):
+        leaves = [t.detach().clone().requires_grad_(True) for t in (x, w, b, r)]
+        y = linear(*leaves[:3], "gelu", leaves[3])
+        return (y.detach(),) + torch.autograd.grad(y, leaves, dy)
+
+    one = plain(x, w, b, x)
+    xs, ws, bs = (t.detach().clone().requires_grad_(True) for t in (x, w, b))
+    y = linear(xs, ws, bs, "gelu", xs)
+    assert torch.equal(y, one[0])
+    for _ in range(2):   # the same graph twice, the same bits
+        gx, gw, gb = torch.autograd.grad(y, (xs, ws, bs), dy, retain_graph=True)
+        assert torch.equal(gx, one[1] + one[4]) and torch.equal(gw, one[2]) and torch.equal(gb, one[3])
+
+    first = linear(xs, ws)                      # one weight in two layers: the sum of both layers' gradients
+    gx, gw = torch.autograd.grad(linear(first, ws), (xs, ws), dy)
+    f1, w1, x1, w2 = (t.detach().requires_grad_(True) for t in (first, w, x, w))
+    gf, gw2 = torch.autograd.grad(linear(f1, w2), (f1, w2), dy)
+    gx1, gw1 = torch.autograd.grad(linear(x1, w1), (x1, w1), gf)
+    assert torch.equal(gx, gx1) and torch.equal(gw, gw2 + gw1)
+
+    xc = x.detach().requires_grad_(True)
+    yc = checkpoint(lambda t: linear(t, w, b, "gelu", t), xc, use_reentrant=False)
+    assert torch.equal(yc, one[0])
+    xr = x.detach().requires_grad_(True)
+    assert torch.equal(torch.autograd.grad(yc, xc, dy)[0], torch.autograd.grad(linear(xr, w, b, "gelu", xr), xr, dy)[0])
+
+    h = x.detach().clone()
+    y = linear(h, ws, bs, "relu")
+    h.add_(1)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        torch.autograd.grad(y, ws, dy)
+
+    want = step(x, w, b, x)
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    got = []
+    for s in streams:
+        s.wait_stream(torch.cuda.current_stream())
+    for _ in range(6):
+        for s in streams:
+            with torch.cuda.stream(s):
+                got.append(step(x, w, b, x))
+    torch.cuda.synchronize()
+    assert all(torch.equal(p, q) for r in got for p, q in zip(r, want))
+
+
 def test_linear_empty_batch():
     from diffusion_model_nemo_amd.modules import linear
     for kind in (None, "gelu"):
