@@ -846,8 +846,15 @@ template <typename T, int G> int join_launch(const GemmArgs& g, hipStream_t s) {
 // against tiles, weights not in the caches: 64 x 2048 into 8192 bf16 19 : 25, 32 x 1000 into 1531 7 : 14, but 32 x 8192 into
 // 2048 28 : 19 and 64 x 8192 44 : 19); and few columns of a long k leave it CUs without work (16 x 8192 into 2048 19 : 15,
 // 16 x 4096 into 512 11 : 9; one row 14 : 14).
-bool few_rows(int M, int N, int K, int dtype) {
+// Where the weight's rows are off 16-byte boundaries the tiles would need a copy of it, and this kernel's loads are slow, the
+// more so the more of x's rows there are; both sides are estimated in us from these times (this kernel : copy and tiles):
+// bf16, k = 4095 into 4095, 1 row 17 : 27, 16 rows 28 : 28, 40 rows 52 : 31; 4095 into 1023, 1 row 17 : 16, 16 rows 28 : 17; 8191
+// into 8191, 4 rows 74 : 82, 16 rows 100 : 83; float32, 4095 into 4095, 16 rows 25 : 50, 40 rows 41 : 50; 8191 into 2047, 8 rows
+// 40 : 50, 40 rows 77 : 52.
+bool few_rows(const Operand& w, int M, int dtype) {
+    const int N = w.rows, K = w.width;
     const long long bytes = (long long)K * elem(dtype);
+    if (M <= 64 && copy_bytes(w, dtype)) return 2.5 + K * 3.2e-3 * (1 + 0.055 * M) * (N > 4096 ? N / 4096. : 1.) < 11 + 0.55e-6 * bytes * N;
     return M <= 64 && M * bytes <= 256 * 1024 && (M < 8 || N >= 4096 || bytes < 8192);
 }
 template <typename T, int MF, int NF, int WAVES> int few_rows_launch(const GemmArgs& g, hipStream_t s) {
@@ -908,8 +915,8 @@ template <typename T> int pair_run(GemmArgs& dx, GemmArgs& dw, const ColumnJoin&
 }
 
 template <typename T> int forward_run(GemmArgs& g, int dtype, char* ws, hipStream_t s) {
-    if (few_rows(g.M, g.N, g.K, dtype)) return few_rows_run<T>(g, s);
     Operand x{g.a, g.lda, g.M, g.K}, w{g.b, g.ldb, g.N, g.K};
+    if (few_rows(w, g.M, dtype)) return few_rows_run<T>(g, s);
     Operand* list[2] = {&x, &w};
     const int rc = copy_operands<T>(list, 2, dtype, ws, s);
     if (rc) return rc;
@@ -1007,7 +1014,8 @@ int backward_run(const void* dy, long long lddy, const void* x, long long ldx, c
 }  // namespace
 
 extern "C" size_t dmn_linear_forward_workspace_bytes(const void* x, int64_t ldx, const void* weight, int64_t rows, int in, int out, int dtype) {
-    if (rows <= 0 || rows >= (1 << 27) || in <= 0 || out <= 0 || dtype < 0 || dtype > 2 || few_rows((int)rows, out, in, dtype)) return 0;
+    if (rows <= 0 || rows >= (1 << 27) || in <= 0 || out <= 0 || dtype < 0 || dtype > 2) return 0;
+    if (few_rows({weight, in, out, in}, (int)rows, dtype)) return 0;
     return gemm_workspace((int)rows, out, in, dtype) + copy_bytes({x, ldx, (int)rows, in}, dtype) + copy_bytes({weight, in, out, in}, dtype);
 }
 

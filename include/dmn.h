@@ -273,7 +273,8 @@ int dmn_adamw_step(float* params, const float* grads, float* exp_avg, float* exp
  * apart; addresses need the alignment of the element type only. Nothing is allocated, nothing waits for the device, and a
  * call can be recorded into a graph; the device that owns the tensors must be the current one. Two calls that may overlap
  * in time need workspaces of their own. Sums and statistics are float32 or wider; results are rounded once to the output's
- * type. The order of every sum is fixed by the sizes and the outputs asked for: the same call gives the same bits. */
+ * type. The order of every sum is fixed by the sizes, the operands' alignment and the outputs asked for: the same call gives
+ * the same bits. */
 #define DMN_DT_F32 0
 #define DMN_DT_BF16 1
 #define DMN_DT_F16 2
