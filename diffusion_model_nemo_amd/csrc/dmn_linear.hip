@@ -63,8 +63,11 @@ template <typename T> __device__ __forceinline__ float activate(float z, int act
     if (act == ACT_GELU) return gelu<T>(z);
     return z;
 }
+// z is held within +-100, where the slopes have long been 0 and 1: an infinite z (a finite sum beyond the range of the type that
+// kept it) would turn into 0 * inf. A NaN stays.
 template <typename T> __device__ __forceinline__ float act_backward(float dy, float z, int act) {
     if (act == ACT_RELU) return z <= 0.f ? 0.f : dy;
+    z = z < -100.f ? -100.f : z > 100.f ? 100.f : z;
     if (act == ACT_SILU) {
         const float s = __builtin_amdgcn_rcpf(1.0f + __expf(-z));
         return dy * (s * __builtin_fmaf(z, 1.0f - s, 1.0f));
