@@ -82,6 +82,7 @@ template <typename T> __device__ __forceinline__ float act_backward(float dy, fl
 // ---- the product -----------------------------------------------------------------------------------------------------
 struct GemmArgs {
     const void *a, *b;           // A(m, k): K: a[m * lda + k], X: a[k * lda + m]; B(n, k) alike
+    const void* a2;              // null, or A's low part, laid out as a: A = (a + a2 / Parts::LOW) / Parts::PRE
     long long lda, ldb;
     int M, N, K;
     int splits, tiles_per_split; // the k tiles are shared out over so many workgroups
@@ -91,8 +92,26 @@ struct GemmArgs {
     long long ldr;
     void* y;                     // [M][N]
     void* z;                     // [M][N] or null: receives the value in front of the activation
+    int z_rounded;               // z is of the operands' type, else float32
     int act;
 };
+
+// dz = dy act'(z) rounded to 16 bits is off by as much as dx and dW, rounded once, are themselves: their errors grow by sqrt 2
+// (512 x 256 into 1024 GELU, relative, bf16 2.4e-3 instead of 1.7e-3), and far more in float16 where gradients are small (dy about
+// 1e-6, of which the type keeps four bits: dW 2.5e-2 instead of 1.1e-3). So the products take dz as the sum of two numbers of the
+// type, 16 bits of it (bf16) or 22 (float16): k is gone through twice, the low part first. float16's low part is stored 2^11
+// times larger, or it would fall below the type's smallest step; both parts are halved, because a slope of up to 1.13 takes a
+// large dy out of the type's range. The backward's matrix work doubles (training step of 4096 x 1024 into 4096 bf16 GELU: 131
+// -> 217 us, of it dz 16 -> 31, the products 74 -> 148, the forward that keeps a float32 z 46 -> 48); a caller who does not want
+// that asks for a rounded z and dz (DMN_LINEAR_ROUNDED).
+template <typename T> struct Parts { static constexpr float PRE = 1.f, LOW = 1.f; };
+template <> struct Parts<f16> { static constexpr float PRE = 0.5f, LOW = 2048.f; };
+template <typename T> __device__ __forceinline__ void in_two(float d, T& high, T& low) {
+    d *= Parts<T>::PRE;
+    high = (T)d;
+    const float rest = d - (float)high;   // exact
+    low = (T)(fabsf((float)high) < INFINITY ? rest * Parts<T>::LOW : 0.f);   // an infinity or NaN stays what it is
+}
 
 // v_mfma on fragments of 16 bytes per lane: lane l holds row l & 15 of its operand; 16-bit types the eight k from 8 (l >> 4)
 // of a step of 32, float32 the four k from 4 (l >> 4) of a step of 16 (four instructions, both operands in the same k
@@ -195,8 +214,11 @@ template <typename T, bool X, int R, int NT, int KB> struct Stager {
     long long step;
     unsigned off[PER];
 
-    __device__ __forceinline__ void init(const void* p, long long ld, int r0, int extent, int k0) {
+    __device__ __forceinline__ void start(const void* p, long long ld, int r0, int k0) {
         next = (const T*)p + (X ? (long long)k0 * ld + r0 : (long long)r0 * ld + k0);
+    }
+    __device__ __forceinline__ void init(const void* p, long long ld, int r0, int extent, int k0) {
+        start(p, ld, r0, k0);
         step = X ? Tl::BK * ld : Tl::BK;
 #pragma unroll
         for (int i = 0; i < PER; ++i) {
@@ -236,12 +258,20 @@ __device__ __forceinline__ void epilogue(const GemmArgs& g, int m, int n, const 
     typename Pack<T>::vec v;
 #pragma unroll
     for (int i = 0; i < V; ++i) z[i] = acc[i] + bias[i];
-    if (g.z) {   // kept for the backward in the operands' type: half the traffic of float32, one rounding of the slope's argument
+    if (g.z && sizeof(T) == 2 && g.z_rounded) {
 #pragma unroll
         for (int i = 0; i < V; ++i) v[i] = (T)z[i];
         T* p = (T*)g.z + (long long)m * g.N;
         if (EDGE) store16_tail(p, n, g.N, v);
         else store16(p + n, v);
+    } else if (g.z) {
+        float* p = (float*)g.z + (long long)m * g.N;
+#pragma unroll
+        for (int e = 0; e < V; e += 4) {
+            const f32x4 q = {z[e], z[e + 1], z[e + 2], z[e + 3]};
+            if (!EDGE) store16(p + n + e, q);
+            else if (n + e < g.N) store16_tail(p, n + e, g.N, q);
+        }
     }
 #pragma unroll
     for (int i = 0; i < V; ++i) z[i] = activate<T>(z[i], act);
@@ -342,7 +372,9 @@ template <int N> struct Int { static constexpr int value = N; };
 // of LDS while the matrix cores work on the present one's, which are in registers. One barrier per tile, in front of its
 // second step: behind it the tile's fragments of every wave are in registers, so that the request for the tile S further on
 // may take its place, and the next tile has arrived (each wave has waited for its own part of it). Requests go on behind the
-// last tile (they read nothing and give zeros), so that the count of outstanding ones is the same for every tile.
+// last tile (they read nothing and give zeros), so that the count of outstanding ones is the same for every tile. With A in
+// two parts (TWO; a kernel of its own, because the others would pay 3 % for the choice: 4001 x 4096 into 1024 training 118 : 121 us)
+// the k tiles count twice, and at `turn` the requests go back to the first one, with the high part.
 //
 // Bound by the matrix cores where the large tile fills the chip: 8192^3 bf16 820 us forward, 814 dx, 837 dw (1340, 1350, 1314
 // TFLOP/s; the card's own product library 797, 905, 1030 us), float32 4096^3 960 us (143 TFLOP/s of 154). Per step of 128
@@ -351,7 +383,7 @@ template <int N> struct Int { static constexpr int value = N; };
 // TFLOP/s (4096 x 1024 out of k = 4096: 37 us). What reading the next fragments beside the products, counted waits and
 // 128-byte rows in LDS (64-byte rows request half cache lines: 262 instead of 238 us) brought is the step from 366 to 238
 // us for 8192 x 2048 into 8192.
-template <typename T, bool XA, bool XB, int BM, int BN, int WM, int WN, int S>
+template <typename T, bool XA, bool XB, bool TWO, int BM, int BN, int WM, int WN, int S>
 __device__ __forceinline__ void product_tile(const GemmArgs& g, int tile, int split, char* lds) {
     constexpr int NT = (BM / WM) * (BN / WN) * 64, KB = 128;
     typedef Tile<T, XA, BM, KB> TA;
@@ -367,20 +399,38 @@ __device__ __forceinline__ void product_tile(const GemmArgs& g, int tile, int sp
     int im, in;
     tile_of(tile, (g.M + BM - 1) / BM, (g.N + BN - 1) / BN, im, in);
     const int m0 = im * BM, n0 = in * BN;
-    const int k_tiles = (g.K + BK - 1) / BK, t0 = split * g.tiles_per_split;
-    const int t1 = t0 + g.tiles_per_split < k_tiles ? t0 + g.tiles_per_split : k_tiles;
-    int left = (t1 * BK < g.K ? t1 * BK : g.K) - t0 * BK;   // k rows that the next requests may still take
+    const int k_tiles = (g.K + BK - 1) / BK, all = TWO ? 2 * k_tiles : k_tiles, turn = TWO ? k_tiles : 0;
+    const int t0 = split * g.tiles_per_split, t1 = t0 + g.tiles_per_split < all ? t0 + g.tiles_per_split : all;
+    auto rows_to = [&](int tile) { return tile * BK < g.K ? tile * BK : g.K; };
+    const bool high = !TWO || t0 >= turn;   // of the first request
+    const int first = high ? t0 - turn : t0;
+    int left = rows_to(high ? t1 - turn : t1 < turn ? t1 : turn) - first * BK;   // k rows that the next requests may still take
+    int next = t0;                                                               // TWO: tile of the next request
     SA sa;
     SB sb;
-    sa.init(g.a, g.lda, m0, g.M, t0 * BK);
-    sb.init(g.b, g.ldb, n0, g.N, t0 * BK);
+    sa.init(high ? g.a : g.a2, g.lda, m0, g.M, first * BK);
+    sb.init(g.b, g.ldb, n0, g.N, first * BK);
     const unsigned lds0 = __builtin_amdgcn_readfirstlane(lds_address(lds) + (threadIdx.x & ~63) * 16);
     f32x4 acc[FM][FN];
 #pragma unroll
     for (int i = 0; i < FM; ++i)
 #pragma unroll
         for (int j = 0; j < FN; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+    auto scale = [&](float f) {
+#pragma unroll
+        for (int i = 0; i < FM; ++i)
+#pragma unroll
+            for (int j = 0; j < FN; ++j) acc[i][j] *= f;
+    };
     auto fetch = [&](int stage) {
+        if constexpr (TWO) {
+            if (next == turn) {
+                sa.start(g.a, g.lda, m0, 0);
+                sb.start(g.b, g.ldb, n0, 0);
+                left = rows_to(t1 - turn);   // none where the split ends here
+            }
+            ++next;
+        }
         sa.fetch(left, lds0 + stage * STAGE);
         sb.fetch(left, lds0 + stage * STAGE + A_BYTES);
         left -= BK;
@@ -416,6 +466,9 @@ __device__ __forceinline__ void product_tile(const GemmArgs& g, int tile, int sp
     read(Int<0>{}, 0);
     int stage = 0;
     for (int t = t0; t < t1; ++t) {
+        if constexpr (TWO && Parts<T>::LOW != 1.f) {
+            if (t == turn) scale(1.f / Parts<T>::LOW);
+        }
         read(Int<1>{}, stage);
         multiply(Int<0>{});
         __builtin_amdgcn_sched_barrier(0);
@@ -430,12 +483,15 @@ __device__ __forceinline__ void product_tile(const GemmArgs& g, int tile, int sp
     }
     asm volatile("s_waitcnt vmcnt(0)" : : : "memory");
     __syncthreads();   // the requests behind the end have landed, the tiles' memory is free
+    if constexpr (TWO && Parts<T>::LOW != 1.f) {
+        scale(t1 <= turn ? 1.f / (Parts<T>::LOW * Parts<T>::PRE) : 1.f / Parts<T>::PRE);
+    }
     store_tile<T, !XB, FM, FN>(g, acc, m0 + wm, n0 + wn, split, lds);
 }
-template <typename T, bool XA, bool XB, int BM, int BN, int WM, int WN, int S>
+template <typename T, bool XA, bool XB, bool TWO, int BM, int BN, int WM, int WN, int S>
 __global__ __launch_bounds__((BM / WM) * (BN / WN) * 64) void gemm_pipe_kernel(const GemmArgs g) {
     extern __shared__ __attribute__((aligned(16))) char lds[];
-    product_tile<T, XA, XB, BM, BN, WM, WN, S>(g, blockIdx.x, blockIdx.y, lds);
+    product_tile<T, XA, XB, TWO, BM, BN, WM, WN, S>(g, blockIdx.x, blockIdx.y, lds);
 }
 // out[col] = sum over `parts` partial rows, in a fixed order: 32 columns per workgroup of NT threads, NT / 32 threads per column
 struct ColumnJoin {
@@ -473,7 +529,7 @@ struct PairArgs {
                               // into 4096, whole step: own launch 139 us, in front of the tiles 136, behind them 129)
     ColumnJoin db;
 };
-template <typename T, int BM, int BN, int WM, int WN, int S>
+template <typename T, bool TWO, int BM, int BN, int WM, int WN, int S>
 __global__ __launch_bounds__((BM / WM) * (BN / WN) * 64) void gemm_pair_kernel(const PairArgs p) {
     extern __shared__ __attribute__((aligned(16))) char lds[];
     const int b = blockIdx.x;
@@ -481,10 +537,10 @@ __global__ __launch_bounds__((BM / WM) * (BN / WN) * 64) void gemm_pair_kernel(c
         column_join<T, (BM / WM) * (BN / WN) * 64>(p.db, b - p.db_at, (float*)lds);
     } else if (p.dx_at ? b >= p.dx_at : b < p.dw_at) {
         const int i = b - p.dx_at, split = i / p.dx_tiles;
-        product_tile<T, false, true, BM, BN, WM, WN, S>(p.dx, i - split * p.dx_tiles, split, lds);
+        product_tile<T, false, true, TWO, BM, BN, WM, WN, S>(p.dx, i - split * p.dx_tiles, split, lds);
     } else {
         const int i = b - p.dw_at, split = i / p.dw_tiles;
-        product_tile<T, true, true, BM, BN, WM, WN, S>(p.dw, i - split * p.dw_tiles, split, lds);
+        product_tile<T, true, true, TWO, BM, BN, WM, WN, S>(p.dw, i - split * p.dw_tiles, split, lds);
     }
 }
 
@@ -578,7 +634,8 @@ template <typename T, int MF, int NF, int WAVES> __global__ __launch_bounds__(WA
             if (n + e >= g.N) break;
             float z = v[e] + (g.bias ? (float)((const T*)g.bias)[n + e] : 0.f);
             const long long at = (long long)m * g.N + n + e;
-            if (g.z) ((T*)g.z)[at] = (T)z;
+            if (g.z && sizeof(T) == 2 && g.z_rounded) ((T*)g.z)[at] = (T)z;
+            else if (g.z) ((float*)g.z)[at] = z;
             z = activate<T>(z, g.act);
             if (g.res) z += (float)((const T*)g.res)[(long long)m * g.ldr + n + e];
             ((T*)g.y)[at] = (T)z;
@@ -629,17 +686,19 @@ template <typename T, int G> __global__ __launch_bounds__(256) void gemm_join_ke
 
 // ---- what stands in front of the backward's products ------------------------------------------------------------------
 // dz = dy act'(z), and partial column sums of dz: 16 threads of 16 bytes side by side, 16 rows at a time; workgroup
-// (x, y) takes the y-th of gridDim.y runs of rows. dz is rounded to the operands' type: the matrix cores read it so. Bound by
-// memory: 4096 x 4096 bf16 18 us (5.5 TB/s), 16384 x 1024 float32 40 us (5.0 TB/s).
+// (x, y) takes the y-th of gridDim.y runs of rows. EXACT (16-bit types): z is float32, dz leaves in two parts (`in_two`); else z is
+// of the operands' type and dz is rounded to it. Bound by memory: 4096 x 4096 bf16 16 us (6.0 TB/s), EXACT 31 us (5.4 TB/s), 16384 x
+// 1024 float32 40 us (5.0 TB/s).
 struct DzArgs {
     const void *dy, *z;
     long long lddy;
     void* dz;             // [M][lddz], the rows' padding zero; null: only the column sums
+    void* low;            // EXACT: the low part, alike
     long long lddz;
     float* part;          // [gridDim.y][N] or null
     int M, N, act;
 };
-template <typename T> __global__ __launch_bounds__(256) void dz_kernel(const DzArgs a) {
+template <typename T, bool EXACT> __global__ __launch_bounds__(256) void dz_kernel(const DzArgs a) {
     constexpr int V = Pack<T>::N;
     __shared__ float sh[16][16 * V + 1];
     const int c = threadIdx.x & 15, r = threadIdx.x >> 4, n = (blockIdx.x * 16 + c) * V;
@@ -651,14 +710,32 @@ template <typename T> __global__ __launch_bounds__(256) void dz_kernel(const DzA
         for (int m = m0 + r; m < m1; m += 16) {
             auto v = load16_tail((const T*)a.dy + (long long)m * a.lddy, n, a.N);
             if (a.act != ACT_NONE) {
-                const auto z = load16_tail((const T*)a.z + (long long)m * a.N, n, a.N);
+                float z[V];
+                typename Pack<T>::vec low;
+                if constexpr (EXACT) {
+                    load_params<T, float>((const float*)a.z + (long long)m * a.N, n, a.N, z);
+                } else {
+                    const auto q = load16_tail((const T*)a.z + (long long)m * a.N, n, a.N);
+#pragma unroll
+                    for (int i = 0; i < V; ++i) z[i] = (float)q[i];
+                }
 #pragma unroll
                 for (int i = 0; i < V; ++i) {
-                    const float d = act_backward<T>((float)v[i], (float)z[i], a.act);
+                    const float d = act_backward<T>((float)v[i], z[i], a.act);
                     sum[i] += d;
-                    v[i] = (T)d;
+                    if constexpr (EXACT) {
+                        T h, l;
+                        in_two(d, h, l);
+                        v[i] = h;
+                        low[i] = l;
+                    } else {
+                        v[i] = (T)d;
+                    }
                 }
-                if (a.dz) store16((T*)a.dz + (long long)m * a.lddz + n, v);   // behind the row's end dy and z read as zero, dz is
+                if (a.dz) {   // behind the row's end dy and z read as zero, dz is
+                    store16((T*)a.dz + (long long)m * a.lddz + n, v);
+                    if constexpr (EXACT) store16((T*)a.low + (long long)m * a.lddz + n, low);
+                }
             } else {
 #pragma unroll
                 for (int i = 0; i < V; ++i) sum[i] += (float)v[i];
@@ -736,9 +813,9 @@ const TileShape kTiles[4] = {{256, 256, 1, 1.60, 1.12, 8.0, 7.4, 7.2, 22.0},
                              {64, 64, 4, 0.22, 0.28, 3.0, 0.55, 0.70, 6.0}};
 
 double join_us(int splits, int M, int N) { return splits > 1 ? 3.0 + (double)splits * M * N * 8 / 4e6 : 0.0; }
-GemmPlan gemm_plan(int M, int N, int K, int dtype) {
+GemmPlan gemm_plan(int M, int N, int K, int dtype, int parts) {   // parts of A: k is gone through so often
     const bool f32 = dtype == DMN_DT_F32;
-    const long long kt = ceil_div(K, 128 / elem(dtype));
+    const long long kt = parts * ceil_div(K, 128 / elem(dtype));
     GemmPlan best{3, 1, (int)kt, 1e30};
     for (int i = 0; i < 4; ++i) {
         const TileShape& t = kTiles[i];
@@ -760,11 +837,11 @@ struct PairPlan {
     bool together;
     GemmPlan dx, dw;
 };
-PairPlan pair_plan(int rows, int in, int out, int dtype) {
+PairPlan pair_plan(int rows, int in, int out, int dtype, int parts) {
     const bool f32 = dtype == DMN_DT_F32;
     const int bk = 128 / elem(dtype);
-    const long long kx = ceil_div(out, bk), kw = ceil_div(rows, bk);
-    PairPlan best{false, gemm_plan(rows, in, out, dtype), gemm_plan(out, in, rows, dtype)};
+    const long long kx = parts * ceil_div(out, bk), kw = parts * ceil_div(rows, bk);
+    PairPlan best{false, gemm_plan(rows, in, out, dtype, parts), gemm_plan(out, in, rows, dtype, parts)};
     double best_us = best.dx.us + best.dw.us;
     for (int i = 2; i < 4; ++i) {
         const TileShape& t = kTiles[i];
@@ -786,9 +863,12 @@ PairPlan pair_plan(int rows, int in, int out, int dtype) {
     return best;
 }
 size_t part_bytes(const GemmPlan& p, int M, int N) { return p.splits > 1 ? block_align256((size_t)p.splits * M * N * sizeof(float)) : 0; }
-size_t gemm_workspace(int M, int N, int K, int dtype) {
-    return part_bytes(gemm_plan(M, N, K, dtype), M, N);
+size_t gemm_workspace(int M, int N, int K, int dtype, int parts) {
+    return part_bytes(gemm_plan(M, N, K, dtype, parts), M, N);
 }
+int activation_of(int flags) { return flags & ~DMN_LINEAR_ROUNDED; }
+// Parts of dz, of which z is a float32 argument: see Parts.
+int dz_parts(int flags, int dtype) { return dtype != DMN_DT_F32 && activation_of(flags) != ACT_NONE && !(flags & DMN_LINEAR_ROUNDED) ? 2 : 1; }
 
 // An operand in memory: rows of `width` elements, `ld` apart.
 struct Operand {
@@ -830,10 +910,10 @@ template <typename F> int allow_lds(F* kernel, int bytes) {
     if (bytes > 65536) DMN_HIP_CHECK(hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, bytes));
     return DMN_OK;
 }
-template <typename T, bool XA, bool XB, int BM, int BN, int WM, int WN, int S> int pipe_launch(const GemmArgs& g, hipStream_t s) {
+template <typename T, bool XA, bool XB, bool TWO, int BM, int BN, int WM, int WN, int S> int pipe_launch(const GemmArgs& g, hipStream_t s) {
     constexpr int NT = (BM / WM) * (BN / WN) * 64, LDS = S * (BM + BN) * 128;
     static_assert((NT / 64) * 2 * 16 * (WN + 4) * 4 <= LDS, "the epilogue's pieces fit the tiles' memory");
-    auto* kernel = gemm_pipe_kernel<T, XA, XB, BM, BN, WM, WN, S>;
+    auto* kernel = gemm_pipe_kernel<T, XA, XB, TWO, BM, BN, WM, WN, S>;
     const int rc = allow_lds(kernel, LDS);
     if (rc) return rc;
     kernel<<<dim3((unsigned)(ceil_div(g.M, BM) * ceil_div(g.N, BN)), g.splits), NT, LDS, s>>>(g);
@@ -885,23 +965,30 @@ template <typename T> int join_run(const GemmArgs& g, hipStream_t s) {
     // eight threads per piece where there are few of them
     return g.splits >= 8 && (long long)g.M * g.N < (1 << 20) ? join_launch<T, 8>(g, s) : join_launch<T, 1>(g, s);
 }
+template <typename T, bool XA, bool XB, bool TWO> int tile_run(const GemmArgs& g, int tile, hipStream_t s) {
+    if (tile == 0) return pipe_launch<T, XA, XB, TWO, 256, 256, 128, 64, 2>(g, s);
+    if (tile == 1) return pipe_launch<T, XA, XB, TWO, 128, 128, 64, 32, 4>(g, s);
+    if (tile == 2) return pipe_launch<T, XA, XB, TWO, 128, 128, 64, 32, 2>(g, s);
+    return pipe_launch<T, XA, XB, TWO, 64, 64, 32, 32, 2>(g, s);
+}
 // C = sum_k A B with the operands on 16-byte boundaries (copy_operands).
 template <typename T, bool XA, bool XB> int gemm_run(GemmArgs& g, int dtype, void* ws, hipStream_t s) {
-    const GemmPlan p = gemm_plan(g.M, g.N, g.K, dtype);
+    const GemmPlan p = gemm_plan(g.M, g.N, g.K, dtype, g.a2 ? 2 : 1);
     set_plan(g, p, ws);
-    int rc;
-    if (p.tile == 0) rc = pipe_launch<T, XA, XB, 256, 256, 128, 64, 2>(g, s);
-    else if (p.tile == 1) rc = pipe_launch<T, XA, XB, 128, 128, 64, 32, 4>(g, s);
-    else if (p.tile == 2) rc = pipe_launch<T, XA, XB, 128, 128, 64, 32, 2>(g, s);
-    else rc = pipe_launch<T, XA, XB, 64, 64, 32, 32, 2>(g, s);
+    int rc = DMN_ERR_INVALID;
+    if (!g.a2) rc = tile_run<T, XA, XB, false>(g, p.tile, s);
+    else if constexpr (XB && sizeof(T) == 2) rc = tile_run<T, XA, XB, true>(g, p.tile, s);
     return rc ? rc : join_run<T>(g, s);
 }
-template <typename T, int BM, int BN, int WM, int WN, int S> int pair_launch(const PairArgs& a, hipStream_t s) {
+template <typename T, bool TWO, int BM, int BN, int WM, int WN, int S> int pair_launch(const PairArgs& a, hipStream_t s) {
     constexpr int NT = (BM / WM) * (BN / WN) * 64, LDS = S * (BM + BN) * 128;
     static_assert(LDS <= 65536, "LDS without an attribute");
-    gemm_pair_kernel<T, BM, BN, WM, WN, S><<<(unsigned)(a.db_at + (a.db.out ? ceil_div(a.db.n, 32) : 0)), NT, LDS, s>>>(a);
+    gemm_pair_kernel<T, TWO, BM, BN, WM, WN, S><<<(unsigned)(a.db_at + (a.db.out ? ceil_div(a.db.n, 32) : 0)), NT, LDS, s>>>(a);
     DMN_BLOCK_LAUNCH_CHECK();
     return DMN_OK;
+}
+template <typename T, bool TWO> int pair_tile_run(const PairArgs& a, int tile, hipStream_t s) {
+    return tile == 2 ? pair_launch<T, TWO, 128, 128, 64, 32, 2>(a, s) : pair_launch<T, TWO, 64, 64, 32, 32, 2>(a, s);
 }
 // dx, dw and the join of db's partial sums; their partial products lie one behind the other in the workspace.
 template <typename T> int pair_run(GemmArgs& dx, GemmArgs& dw, const ColumnJoin& db, const PairPlan& p, char* ws, hipStream_t s) {
@@ -912,7 +999,9 @@ template <typename T> int pair_run(GemmArgs& dx, GemmArgs& dw, const ColumnJoin&
     a.db_at = a.dx_tiles * dx.splits + a.dw_tiles * dw.splits;
     if (p.dx.per >= p.dw.per) a.dw_at = a.dx_tiles * dx.splits;
     else a.dx_at = a.dw_tiles * dw.splits;
-    int rc = p.dx.tile == 2 ? pair_launch<T, 128, 128, 64, 32, 2>(a, s) : pair_launch<T, 64, 64, 32, 32, 2>(a, s);
+    int rc = DMN_ERR_INVALID;
+    if (!dx.a2) rc = pair_tile_run<T, false>(a, p.dx.tile, s);
+    else if constexpr (sizeof(T) == 2) rc = pair_tile_run<T, true>(a, p.dx.tile, s);
     if (!rc) rc = join_run<T>(dx, s);
     return rc ? rc : join_run<T>(dw, s);
 }
@@ -935,7 +1024,7 @@ int dz_runs(int M) { return (int)(ceil_div(M, 64) < kMaxDzRuns ? ceil_div(M, 64)
 
 int linear_check(const char* who, int64_t rows, int in, int out, int act, int dtype, int64_t ldx) {
     DMN_REQUIRE(dtype >= 0 && dtype <= 2, DMN_ERR_INVALID, "%s: dtype must be DMN_DT_F32, _BF16 or _F16", who);
-    DMN_REQUIRE(act >= ACT_NONE && act <= ACT_GELU, DMN_ERR_INVALID, "%s: unknown activation %d", who, act);
+    DMN_REQUIRE(activation_of(act) >= ACT_NONE && activation_of(act) <= ACT_GELU, DMN_ERR_INVALID, "%s: unknown activation %d", who, act);
     DMN_REQUIRE(rows >= 0 && in > 0 && out > 0, DMN_ERR_INVALID, "%s: rows must be >= 0, in and out > 0", who);
     DMN_REQUIRE(rows < (1 << 27) && in < (1 << 20) && out < (1 << 20) && rows * (in > out ? in : out) < ((int64_t)1 << 40), DMN_ERR_LIMIT,
                 "%s: rows must be below 2^27, in and out below 2^20", who);
@@ -946,7 +1035,7 @@ int linear_check(const char* who, int64_t rows, int in, int out, int act, int dt
 
 template <typename T>
 int backward_run(const void* dy, long long lddy, const void* x, long long ldx, const void* w, const void* z, void* dx, void* dw, void* db,
-                 int rows, int in, int out, int act, int dtype, char* ws, hipStream_t s) {
+                 int rows, int in, int out, int flags, int dtype, char* ws, hipStream_t s) {
     if (rows == 0) {
         if (dw) zero_kernel<T><<<1024, 256, 0, s>>>((T*)dw, (long long)in * out);
         DMN_BLOCK_LAUNCH_CHECK();
@@ -954,11 +1043,13 @@ int backward_run(const void* dy, long long lddy, const void* x, long long ldx, c
         DMN_BLOCK_LAUNCH_CHECK();
         return DMN_OK;
     }
+    const int act = activation_of(flags), parts = dz_parts(flags, dtype);
     float* part = (float*)ws;
     const int runs = dz_runs(rows);
     ws += block_align256((size_t)runs * out * sizeof(float));
     ColumnJoin join{part, runs, out, nullptr};
     Operand z_{dy, lddy, rows, out}, w_{w, in, out, in}, x_{x, ldx, rows, in};
+    const void* low = nullptr;
     if (act != ACT_NONE || db) {
         DzArgs a{};
         a.dy = dy;
@@ -966,18 +1057,23 @@ int backward_run(const void* dy, long long lddy, const void* x, long long ldx, c
         a.lddy = lddy;
         a.dz = act != ACT_NONE && (dx || dw) ? ws : nullptr;
         a.lddz = padded(out, dtype);
+        const size_t dz_bytes = block_align256((size_t)rows * a.lddz * sizeof(T));
+        a.low = parts == 2 ? ws + dz_bytes : nullptr;
         a.part = db ? part : nullptr;
         a.M = rows;
         a.N = out;
         a.act = act;
-        dz_kernel<T><<<dim3((unsigned)ceil_div(out, 16 * Pack<T>::N), runs), 256, 0, s>>>(a);
+        const dim3 grid((unsigned)ceil_div(out, 16 * Pack<T>::N), runs);
+        if (parts == 2) dz_kernel<T, sizeof(T) == 2><<<grid, 256, 0, s>>>(a);
+        else dz_kernel<T, false><<<grid, 256, 0, s>>>(a);
         DMN_BLOCK_LAUNCH_CHECK();
         join.out = db;
         if (act != ACT_NONE) {
             z_.p = ws;
             z_.ld = a.lddz;
             z_.width = (int)a.lddz;
-            ws += block_align256((size_t)rows * a.lddz * sizeof(T));
+            low = a.low;
+            ws += parts * dz_bytes;
         }
     }
     Operand* list[3];
@@ -989,6 +1085,7 @@ int backward_run(const void* dy, long long lddy, const void* x, long long ldx, c
     if (rc) return rc;
     GemmArgs gx{}, gw{};
     gx.a = gw.a = z_.p;
+    gx.a2 = gw.a2 = low;
     gx.lda = gw.lda = z_.ld;
     gx.b = w_.p;
     gx.ldb = w_.ld;
@@ -1002,7 +1099,7 @@ int backward_run(const void* dy, long long lddy, const void* x, long long ldx, c
     gw.y = dw;
     gx.N = gw.N = in;
     if (dx && dw) {
-        const PairPlan p = pair_plan(rows, in, out, dtype);
+        const PairPlan p = pair_plan(rows, in, out, dtype, parts);
         if (p.together) return pair_run<T>(gx, gw, join, p, ws, s);
     }
     if (join.out) {
@@ -1019,7 +1116,7 @@ int backward_run(const void* dy, long long lddy, const void* x, long long ldx, c
 extern "C" size_t dmn_linear_forward_workspace_bytes(const void* x, int64_t ldx, const void* weight, int64_t rows, int in, int out, int dtype) {
     if (rows <= 0 || rows >= (1 << 27) || in <= 0 || out <= 0 || dtype < 0 || dtype > 2) return 0;
     if (few_rows({weight, in, out, in}, (int)rows, dtype)) return 0;
-    return gemm_workspace((int)rows, out, in, dtype) + copy_bytes({x, ldx, (int)rows, in}, dtype) + copy_bytes({weight, in, out, in}, dtype);
+    return gemm_workspace((int)rows, out, in, dtype, 1) + copy_bytes({x, ldx, (int)rows, in}, dtype) + copy_bytes({weight, in, out, in}, dtype);
 }
 
 extern "C" int dmn_linear_forward(const void* x, int64_t ldx, const void* weight, const void* bias, const void* residual, int64_t ldr,
@@ -1045,7 +1142,8 @@ extern "C" int dmn_linear_forward(const void* x, int64_t ldx, const void* weight
     g.ldr = ldr;
     g.y = y;
     g.z = z;
-    g.act = activation;
+    g.z_rounded = (activation & DMN_LINEAR_ROUNDED) != 0;
+    g.act = activation_of(activation);
     hipStream_t s = (hipStream_t)stream;
     char* ws = (char*)workspace;
     if (dtype == DMN_DT_F32) return forward_run<float>(g, dtype, ws, s);
@@ -1056,10 +1154,11 @@ extern "C" int dmn_linear_forward(const void* x, int64_t ldx, const void* weight
 extern "C" size_t dmn_linear_backward_workspace_bytes(const void* dy, int64_t lddy, const void* x, int64_t ldx, const void* weight, int64_t rows,
                                                       int in, int out, int activation, int dtype) {
     if (rows <= 0 || rows >= (1 << 27) || in <= 0 || out <= 0 || dtype < 0 || dtype > 2) return 0;
-    const size_t dx = gemm_workspace((int)rows, in, out, dtype), dw = gemm_workspace(out, in, (int)rows, dtype);
-    const PairPlan p = pair_plan((int)rows, in, out, dtype);
+    const int parts = dz_parts(activation, dtype);
+    const size_t dx = gemm_workspace((int)rows, in, out, dtype, parts), dw = gemm_workspace(out, in, (int)rows, dtype, parts);
+    const PairPlan p = pair_plan((int)rows, in, out, dtype, parts);
     const size_t pair = p.together ? part_bytes(p.dx, (int)rows, in) + part_bytes(p.dw, out, in) : 0, one = dx > dw ? dx : dw;
-    const size_t dz = activation != ACT_NONE ? block_align256((size_t)rows * padded(out, dtype) * elem(dtype)) : copy_bytes({dy, lddy, (int)rows, out}, dtype);
+    const size_t dz = activation_of(activation) != ACT_NONE ? parts * block_align256((size_t)rows * padded(out, dtype) * elem(dtype)) : copy_bytes({dy, lddy, (int)rows, out}, dtype);
     return block_align256((size_t)dz_runs((int)rows) * out * sizeof(float)) + dz + copy_bytes({x, ldx, (int)rows, in}, dtype) +
            copy_bytes({weight, in, out, in}, dtype) + (pair > one ? pair : one);
 }
@@ -1070,7 +1169,7 @@ extern "C" int dmn_linear_backward(const void* dy, int64_t lddy, const void* x, 
     int rc = linear_check("dmn_linear_backward", rows, in, out, activation, dtype, ldx);
     if (rc) return rc;
     if (!dx && !dweight && !dbias) return DMN_OK;
-    DMN_REQUIRE(rows == 0 || (dy && (!dx || weight) && (!dweight || x) && (activation == ACT_NONE || z)), DMN_ERR_INVALID,
+    DMN_REQUIRE(rows == 0 || (dy && (!dx || weight) && (!dweight || x) && (activation_of(activation) == ACT_NONE || z)), DMN_ERR_INVALID,
                 "dmn_linear_backward: null argument");
     DMN_REQUIRE(rows <= 1 || lddy >= out, DMN_ERR_INVALID, "dmn_linear_backward: row stride of dy below its width");
     DMN_REQUIRE(lddy < (1 << 20), DMN_ERR_LIMIT, "dmn_linear_backward: row stride of dy must be below 2^20 elements");

@@ -19,6 +19,7 @@ import torch.nn as nn
 from .. import _native as N
 
 ACTIVATIONS = {None: 0, "relu": 1, "silu": 2, "gelu": 3}
+ROUNDED = 16   # DMN_LINEAR_ROUNDED of include/dmn.h
 
 
 def _stream(x: torch.Tensor, what: str):
@@ -38,16 +39,20 @@ def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Opt
 
 
 def linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] = None, activation: Optional[str] = None,
-           residual: Optional[torch.Tensor] = None) -> torch.Tensor:
+           residual: Optional[torch.Tensor] = None, rounded_backward: bool = False) -> torch.Tensor:
     """act(x weight^T + bias) + residual in one pass: `x` [..., in], `weight` [out, in], `bias` [out], `residual` [..., out],
     all of one type (float32, bfloat16 or float16); `activation` None, 'relu', 'silu' or 'gelu' (the exact one). The sum in
-    front of the activation, the activation and the residual are formed in float32 and rounded once. For the backward with
-    an activation the value in front of it is kept, rounded to the type; rows with any stride below 2^20 are read in
-    place for 2-D tensors, other layouts are copied first. `in` and `out` are below 2^20."""
+    front of the activation, the activation and the residual are formed in float32 and rounded once. Rows with any stride
+    below 2^20 are read in place for 2-D tensors, other layouts are copied first. `in` and `out` are below 2^20.
+
+    For the backward with an activation the value z in front of it is kept in float32, and dz = dy act'(z) enters the products
+    of a 16-bit type in two parts, so the gradients too are rounded once. `rounded_backward=True` keeps z and dz in the type, as
+    a composition of 16-bit layers does: a 16-bit z, half of the backward's matrix work, errors of dx and dweight sqrt 2
+    larger. It changes nothing for float32 or without an activation."""
     code = ACTIVATIONS.get(activation)
     if code is None:
         raise ValueError(f"activation must be one of {list(ACTIVATIONS)}, got {activation!r}")
-    return N.ops().linear(x, weight, bias, code, residual, *_stream(x, "linear"))
+    return N.ops().linear(x, weight, bias, code | ROUNDED if rounded_backward else code, residual, *_stream(x, "linear"))
 
 
 class LayerNorm(nn.Module):
@@ -70,14 +75,14 @@ class LayerNorm(nn.Module):
 
 class Linear(nn.Linear):
     """torch.nn.Linear (its parameters, initialisation and state_dict) with an activation and a residual in its epilogue:
-    `Linear(in, out, activation='gelu')(x)`, `Linear(in, out)(x, residual=x0)`."""
+    `Linear(in, out, activation='gelu')(x)`, `Linear(in, out)(x, residual=x0)`. `rounded_backward` as in `linear`."""
 
     def __init__(self, in_features: int, out_features: int, bias: bool = True, activation: Optional[str] = None, device=None,
-                 dtype=None):
+                 dtype=None, rounded_backward: bool = False):
         if activation not in ACTIVATIONS:
             raise ValueError(f"activation must be one of {list(ACTIVATIONS)}, got {activation!r}")
         super().__init__(in_features, out_features, bias, device=device, dtype=dtype)
-        self.activation = activation
+        self.activation, self.rounded_backward = activation, bool(rounded_backward)
 
     def forward(self, x: torch.Tensor, residual: Optional[torch.Tensor] = None) -> torch.Tensor:
-        return linear(x, self.weight, self.bias, self.activation, residual)
+        return linear(x, self.weight, self.bias, self.activation, residual, self.rounded_backward)

@@ -142,3 +142,14 @@ def test_gradient_clipping_hook_takes_the_configured_value(monkeypatch):
     assert DDPM(cfg).configure_gradient_clipping(opt) is None and len(seen) == 2   # no trainer section: no clipping
     with pytest.raises(NotImplementedError):
         m.configure_gradient_clipping(opt, gradient_clip_algorithm="value")
+
+
+def test_linear_entry_points_take_the_rounded_flag_with_an_activation_only():
+    lib = _N().lib()
+    need = lambda act, dt: lib.dmn_linear_backward_workspace_bytes(X, 4096, X, 1024, X, 4096, 1024, 4096, act, dt)  # noqa: E731
+    dz = 4096 * 4096 * 2
+    assert need(3, 1) - need(3 + 16, 1) >= dz and need(3, 2) - need(3 + 16, 2) >= dz     # dz in two parts, or one
+    assert need(0, 1) == need(16, 1) and need(3, 0) == need(3 + 16, 0)
+    for act in (20, 31, 32, 8, -16):
+        assert lib.dmn_linear_backward(X, 8, X, 8, X, X, X, X, X, 4, 8, 8, act, 1, None, 0, None) == -1
+        assert lib.dmn_linear_forward(X, 8, X, None, None, 0, X, None, 4, 8, 8, act, 1, None, 0, None) == -1

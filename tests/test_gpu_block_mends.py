@@ -3,7 +3,7 @@ with the bounds of `check_linear` (tests/test_gpu_block_ops.py), or as refusals.
 import pytest
 import torch
 
-from test_gpu_block_ops import HF, TYPES, U, act_formula, close, floor_of, half_step, product, randn
+from test_gpu_block_ops import BF, HF, TYPES, U, act_formula, close, floor_of, half_step, product, randn
 
 pytestmark = pytest.mark.gpu
 
@@ -56,3 +56,86 @@ def test_slopes_at_infinite_sums_are_their_limits(dtype, kind):
     db = grads_of(x, w, b, kind, dy)[3]
     assert float(db[3]) == 70 and float(db[4]) == 0 and bool(torch.isnan(db[5]))
     assert bool((db[6:] == 35).all()) and bool((db[:3] == 35).all())
+
+
+def check_gradients(m, k, n, dtype, kind, rounded=False, scale=1.0, one_by_one=False):
+    """dx, dweight and dbias with ONE rounding (the result's) and float32 work in front of it; `rounded` adds half a step of z and
+    of dz. Two numbers of the type hold dz to half_step squared of it (float16: down to 2^-35, as its low part is kept 2^11
+    times larger and both are halved)."""
+    from diffusion_model_nemo_amd.modules import linear
+    x, w, b = randn((m, k), 1, dtype), randn((n, k), 2, dtype, k ** -0.5), randn((n,), 3, dtype, 0.3)
+    dy = randn((m, n), 4, dtype, scale)
+    got = grads_of(x, w, b, kind, dy, rounded_backward=rounded)
+    if one_by_one:   # each product in a launch of its own
+        for i in range(2):
+            leaves = [t.detach().requires_grad_(i == j) for j, t in enumerate((x, w, b))]
+            (g,) = torch.autograd.grad(linear(*leaves, kind, rounded_backward=rounded), leaves[i], dy)
+            got = got[:1 + i] + (g,) + got[2 + i:]
+    z, za = product(x, w.t())
+    ez = (k + 64) * U * za + 4 * U * (z.abs() + 2 * b.double().abs())
+    z = z + b.double()
+    a, slope = act_formula(z, kind)
+    close(got[0], a, half_step(dtype) * a.abs() + 1.13 * ez + 6e-6 * a.abs() + floor_of(dtype), "y")
+    d = dy.double()
+    dz, h = d * slope, half_step(dtype)
+    edz = d.abs() * (1.2 * ez + 4e-6 + 4 * U)
+    if rounded:
+        edz = edz + d.abs() * 1.2 * (h * z.abs() + floor_of(dtype))
+    if kind == "relu":   # the slope jumps at 0: only where the sign is in doubt, and there by all of dy
+        edz = torch.where(z.abs() <= ez + (floor_of(dtype) if rounded else 0), d.abs(), torch.zeros_like(dz))
+    part = h * dz.abs() + floor_of(dtype) if rounded else h * h * dz.abs() + (2.0 ** -35 if dtype == HF else 2.0 ** -140)
+    for at, (p, q), depth in ((1, (dz, w), n), (2, (dz.t(), x), m)):
+        want, size = product(p, q)
+        err = product((edz + part) if at == 1 else (edz + part).t(), q)[1]
+        close(got[at], want, h * want.abs() + err + (2 * depth + 64) * U * (1.01 * size + err) + floor_of(dtype), "dx" if at == 1 else "dw")
+        if not rounded and kind != "relu" and scale == 1.0:
+            # all errors together, against those of the exact result rounded once
+            once = (want.to(dtype).double() - want).norm()
+            assert float((got[at].double() - want).norm()) <= 1.02 * float(once), at
+    want = dz.sum(0)
+    close(got[3], want, h * want.abs() + edz.sum(0) + (m + 64) * U * (dz.abs() + edz).sum(0) + floor_of(dtype), "db")
+
+
+@pytest.mark.parametrize("dtype", [BF, HF], ids=str)
+@pytest.mark.parametrize("kind", ["silu", "gelu"])
+@pytest.mark.parametrize("m,k,n", [(1, 8, 8), (17, 40, 24), (130, 127, 131), (70, 96, 104), (2048, 512, 1024), (64, 72, 8200), (8200, 72, 64)])
+def test_gradients_of_16_bit_layers_are_rounded_once(dtype, kind, m, k, n):
+    check_gradients(m, k, n, dtype, kind)
+
+
+@pytest.mark.parametrize("dtype", [BF, HF], ids=str)
+@pytest.mark.parametrize("m,k,n", [(130, 127, 131), (64, 72, 8200), (8200, 72, 64), (1030, 1032, 1040)])
+def test_gradients_of_16_bit_layers_one_by_one(dtype, m, k, n):
+    check_gradients(m, k, n, dtype, "gelu", one_by_one=True)
+    check_gradients(m, k, n, dtype, "relu", one_by_one=True)
+
+
+@pytest.mark.parametrize("scale", [1e-6, 2e-4])
+def test_small_float16_gradients_keep_their_digits(scale):
+    check_gradients(300, 136, 520, HF, "gelu", scale=scale)
+
+
+def test_large_float16_gradients_stay_in_range():
+    """A slope of up to 1.13 takes dz out of float16's range where dx is well within it."""
+    x, w, b = torch.full((80, 8), 0.25, dtype=HF, device="cuda"), torch.full((16, 8), 0.5, dtype=HF, device="cuda"), torch.full((16,), 0.5, dtype=HF, device="cuda")
+    w[8:] = -0.5
+    dy = torch.full((80, 16), 65000.0, dtype=HF, device="cuda")
+    b[8:] = 2.5                                                         # sums of 1.5: gelu's slope is 1.1275 there
+    y, dx, dw, db = grads_of(x, w, b, "gelu", dy)
+    assert bool((dx == 0).all())                                        # 8 times 0.5 dz - 8 times 0.5 dz
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("kind", ["relu", "gelu"])
+def test_rounded_backward_is_the_callers_choice(dtype, kind):
+    from diffusion_model_nemo_amd.modules import Linear, linear
+    for m, k, n in ((1, 8, 8), (130, 127, 131), (2048, 512, 1024), (64, 72, 8200)):
+        check_gradients(m, k, n, dtype, kind, rounded=True)
+    layer = Linear(96, 104, activation=kind, dtype=dtype, device="cuda", rounded_backward=True)
+    x, dy = randn((70, 96), 1, dtype).requires_grad_(True), randn((70, 104), 2, dtype)
+    want = grads_of(x, layer.weight, layer.bias, kind, dy, rounded_backward=True)
+    y = layer(x)
+    assert torch.equal(y, want[0]) and all(torch.equal(p, q) for p, q in zip(torch.autograd.grad(y, (x, layer.weight, layer.bias), dy), want[1:]))
+    if dtype == TYPES[0]:   # float32: there is nothing to choose
+        assert all(torch.equal(p, q) for p, q in zip(grads_of(x, layer.weight, layer.bias, kind, dy), want))
+    assert torch.equal(linear(x, layer.weight, layer.bias, None, rounded_backward=True), linear(x, layer.weight, layer.bias))
