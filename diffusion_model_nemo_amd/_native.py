@@ -91,6 +91,7 @@ SIGNATURES = {
     "dmn_linear_backward": (_i, [_vp, _i64, _vp, _i64, _vp, _vp, _vp, _vp, _vp, _i64, _i, _i, _i, _i, _vp, _sz, _vp]),
     "dmn_clip_grads_workspace_bytes": (_sz, [_i]),
     "dmn_clip_grads": (_i, [_vp, _i, _i, _f, _f, _vp, _vp, _sz, _vp]),
+    "dmn_stream_is_capturing": (_i, [_vp]),
     "dmn_fill_normal": (_i, [_vp, _i, _i, _u64, C.c_uint32, _i64, _f, _vp]),
     "dmn_unet_set_sample_chains": (_i, [_vp, _i, _i]),
     "dmn_ddpm_loop_chains": (_i, [_vp, _i]),
@@ -162,7 +163,7 @@ _ops = None
 # entry points that the compiled binding calls, in the order of its `Api`
 BOUND = ("dmn_last_error", "dmn_layer_norm_forward", "dmn_layer_norm_workspace_bytes", "dmn_layer_norm_backward",
          "dmn_linear_forward_workspace_bytes", "dmn_linear_forward", "dmn_linear_backward_workspace_bytes", "dmn_linear_backward",
-         "dmn_clip_grads_workspace_bytes", "dmn_clip_grads")
+         "dmn_clip_grads_workspace_bytes", "dmn_clip_grads", "dmn_stream_is_capturing")
 
 
 def ops():

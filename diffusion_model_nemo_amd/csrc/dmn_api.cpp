@@ -78,6 +78,16 @@ extern "C" int dmn_sde_corrector_step(const float* table, int row, const float* 
     return launch_langevin(a, (hipStream_t)stream);
 }
 
+extern "C" int dmn_stream_is_capturing(void* stream) {
+    hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
+    if (!stream) return 0;   // asking the default stream beside a capture is an error of its own
+    if (hipStreamIsCapturing((hipStream_t)stream, &status) != hipSuccess) {
+        (void)hipGetLastError();
+        return 0;
+    }
+    return status != hipStreamCaptureStatusNone;
+}
+
 extern "C" int dmn_fill_normal(float* x, int B, int per, uint64_t seed, uint32_t step, int64_t img_offset, float scale,
                                void* stream) {
     DMN_REQUIRE(x && B > 0 && per > 0, DMN_ERR_INVALID, "dmn_fill_normal: bad argument");

@@ -4,6 +4,7 @@
 // 105 us in Python's side of autograd and 25 us on the GPU. Host code only; streams arrive as handles.
 #include <ATen/ATen.h>
 #include <c10/core/DeviceGuard.h>
+#include <c10/core/StreamGuard.h>
 #include <c10/core/impl/DeviceGuardImplInterface.h>
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
@@ -11,6 +12,7 @@
 #include <torch/csrc/utils/pybind.h>
 
 #include <cstring>
+#include <unordered_set>
 #include <vector>
 
 #include "../../include/dmn.h"
@@ -33,6 +35,7 @@ struct Api {
     decltype(&dmn_linear_backward) linear_backward;
     decltype(&dmn_clip_grads_workspace_bytes) clip_workspace;
     decltype(&dmn_clip_grads) clip;
+    decltype(&dmn_stream_is_capturing) is_capturing;
 } api;
 PyObject* error_class = nullptr;     // DmnError
 PyObject* current_stream = nullptr;  // device index -> stream handle
@@ -107,17 +110,39 @@ variable_list once_differentiable(variable_list grads) {
     return grads;
 }
 
+int64_t stream_handle(c10::DeviceIndex device) {   // of its current stream; with the GIL held
+    const py::object h = py::reinterpret_steal<py::object>(PyObject_CallFunction(current_stream, "i", (int)device));
+    if (!h) throw py::error_already_set();
+    return h.cast<int64_t>();
+}
+bool is_capturing(const c10::Stream& s) {
+    c10::StreamGuard guard(s);
+    py::gil_scoped_acquire gil;
+    return api.is_capturing(handle(stream_handle(s.device_index()))) != 0;
+}
+
 // Under capture the gradients of a leaf would be accumulated on the stream on which an eager graph that still lives first
-// used the leaf; torch then touches that stream in the middle of the capture, and the process ends. Such a call is refused.
-void check_capture(bool capturing, const Tensor& x, std::initializer_list<const Tensor*> inputs) {
-    if (!capturing) return;
+// used the leaf; torch then touches that stream in the middle of the capture, and the process ends. The same holds for any node of
+// an eager graph that the backward would pass through. Such a call is refused, however far behind the inputs (views, transposes,
+// copies) the node lies; a stream that was forked into the same capture is none of these.
+void check_capture(int64_t stream, const Tensor& x, std::initializer_list<const Tensor*> inputs) {
+    if (!api.is_capturing(handle(stream))) return;
     const c10::Stream now = c10::impl::getDeviceGuardImpl(c10::DeviceType::CUDA)->getStream(x.device());
-    for (const Tensor* t : inputs) {
-        if (!t->defined() || !t->requires_grad() || !t->is_leaf()) continue;
-        const auto accumulator = torch::autograd::impl::try_get_grad_accumulator(*t);
-        if (accumulator && accumulator->stream().has_value() && *accumulator->stream() != now)
+    std::vector<std::shared_ptr<torch::autograd::Node>> todo;
+    std::unordered_set<torch::autograd::Node*> seen;
+    auto add = [&](const std::shared_ptr<torch::autograd::Node>& node) {
+        if (node && seen.insert(node.get()).second) todo.push_back(node);
+    };
+    for (const Tensor* t : inputs)
+        if (t->defined() && t->requires_grad()) add(t->is_leaf() ? torch::autograd::impl::try_get_grad_accumulator(*t) : t->grad_fn());
+    while (!todo.empty()) {
+        const auto node = todo.back();
+        todo.pop_back();
+        const auto stream = node->stream();
+        if (stream.has_value() && *stream != now && !is_capturing(*stream))
             throw std::runtime_error("a graph is being captured while an eager graph over the same parameters or inputs, made on another stream, "
                                      "still lives: drop its results first (del loss, outputs), or warm up on the capturing stream");
+        for (const auto& edge : node->next_edges()) add(edge.function);
     }
 }
 
@@ -171,7 +196,7 @@ struct LayerNormNode : torch::autograd::Function<LayerNormNode> {
     }
 };
 
-Tensor layer_norm(const Tensor& x, const std::optional<Tensor>& weight_, const std::optional<Tensor>& bias_, double eps, int64_t stream, bool capturing) {
+Tensor layer_norm(const Tensor& x, const std::optional<Tensor>& weight_, const std::optional<Tensor>& bias_, double eps, int64_t stream) {
     check_input(x, "layer_norm");
     if (x.dim() == 0 || x.size(-1) == 0) throw py::value_error("layer_norm needs a last axis of at least one element");
     if (x.size(-1) > INT32_MAX) throw py::value_error("layer_norm: the last axis is too long");
@@ -184,7 +209,7 @@ Tensor layer_norm(const Tensor& x, const std::optional<Tensor>& weight_, const s
     if (bias.defined()) bias = bias.contiguous();
     c10::DeviceGuard guard(x.device());
     if (at::GradMode::is_enabled() && (x.requires_grad() || (weight.defined() && weight.requires_grad()) || (bias.defined() && bias.requires_grad()))) {
-        check_capture(capturing, x, {&x, &weight, &bias});
+        check_capture(stream, x, {&x, &weight, &bias});
         return LayerNormNode::apply(x, given(weight), given(bias), eps, stream);
     }
     return layer_norm_run(rows_of(x), weight, bias, eps, stream, nullptr);
@@ -254,7 +279,7 @@ struct LinearNode : torch::autograd::Function<LinearNode> {
 };
 
 Tensor linear(const Tensor& x, const Tensor& weight_, const std::optional<Tensor>& bias_, int64_t act, const std::optional<Tensor>& residual_,
-              int64_t stream, bool capturing) {
+              int64_t stream) {
     check_input(x, "linear");
     if (weight_.dim() != 2 || weight_.size(0) == 0 || weight_.size(1) == 0 || weight_.size(0) > INT32_MAX || weight_.size(1) > INT32_MAX)
         throw py::value_error(c10::str("weight must be [out, in], got ", weight_.sizes()));
@@ -268,7 +293,7 @@ Tensor linear(const Tensor& x, const Tensor& weight_, const std::optional<Tensor
     c10::DeviceGuard guard(x.device());
     if (at::GradMode::is_enabled() && (x.requires_grad() || weight.requires_grad() || (bias.defined() && bias.requires_grad()) ||
                                        (residual.defined() && residual.requires_grad()))) {
-        check_capture(capturing, x, {&x, &weight, &bias, &residual});
+        check_capture(stream, x, {&x, &weight, &bias, &residual});
         return LinearNode::apply(x, weight, given(bias), given(residual), act, stream);
     }
     return linear_run(rows_of(x, kLinearStride), weight, bias, residual, act, stream, nullptr);
@@ -308,14 +333,12 @@ py::object clip_grads(const py::list& params, const py::object& out, bool inf_no
     }
     if (table.empty()) return py::none();
     c10::DeviceGuard guard(device);
-    const py::object stream = py::reinterpret_steal<py::object>(PyObject_CallFunction(current_stream, "i", (int)device.index()));
-    if (!stream) throw py::error_already_set();
     const at::TensorOptions on = at::TensorOptions().device(device);
     Tensor norm = at::empty({}, on.dtype(at::kFloat));
     const size_t bytes = api.clip_workspace((int)table.size());
     const Tensor ws = at::empty({(int64_t)bytes}, on.dtype(at::kByte));
     check(api.clip(table.data(), (int)table.size(), inf_norm, (float)max_norm, (float)grad_scale, (float*)norm.data_ptr(), ws.data_ptr(), bytes,
-                   handle(stream.cast<int64_t>())));
+                   handle(stream_handle(device.index()))));
     for (const Tensor& t : written) t.unsafeGetTensorImpl()->bump_version();
     return py::reinterpret_steal<py::object>(THPVariable_Wrap(norm));
 }

@@ -9,7 +9,8 @@ What the reference builds its blocks from outside the convolutions -- `Residual(
 Results are rounded once, to the input's type; sums, statistics and parameter gradients are formed in float32. The backward
 passes are not differentiable themselves. Calls and their backward passes can be captured into a graph; a call that would be
 captured while an eager graph over the same leaves, made on another stream, still lives is refused (its backward would end
-the process inside torch).
+the process inside torch, `autograd.grad` as well as `backward`). Whether a backward follows cannot be seen from the call: a
+forward alone is captured beside such a graph under `torch.no_grad()`.
 """
 from typing import Optional
 
@@ -23,10 +24,10 @@ ROUNDED = 16   # DMN_LINEAR_ROUNDED of include/dmn.h
 
 
 def _stream(x: torch.Tensor, what: str):
-    """(torch's current stream of x's device, whether a graph is being captured); the other checks are in csrc/dmn_torch.cpp."""
+    """Torch's current stream of x's device; the other checks are in csrc/dmn_torch.cpp."""
     if not x.is_cuda:
         raise RuntimeError(f"{what} runs only on MI355X device tensors (no CPU implementation)")
-    return torch._C._cuda_getCurrentRawStream(x.get_device()), torch._C._cuda_isCurrentStreamCapturing()
+    return torch._C._cuda_getCurrentRawStream(x.get_device())
 
 
 def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Optional[torch.Tensor] = None,
@@ -35,7 +36,7 @@ def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Opt
     `weight` and `bias` [width] (either may be None) are of x's type or float32, both alike; their gradients come in
     that type. Rows with any stride are read in place for a 2-D `x`; other layouts are copied first. The statistics are
     float32: a row whose squared deviations add up to more than 3.4e38 comes out as zeros times weight plus bias."""
-    return N.ops().layer_norm(x, weight, bias, eps, *_stream(x, "layer_norm"))
+    return N.ops().layer_norm(x, weight, bias, eps, _stream(x, "layer_norm"))
 
 
 def linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] = None, activation: Optional[str] = None,
@@ -52,7 +53,7 @@ def linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] =
     code = ACTIVATIONS.get(activation)
     if code is None:
         raise ValueError(f"activation must be one of {list(ACTIVATIONS)}, got {activation!r}")
-    return N.ops().linear(x, weight, bias, code | ROUNDED if rounded_backward else code, residual, *_stream(x, "linear"))
+    return N.ops().linear(x, weight, bias, code | ROUNDED if rounded_backward else code, residual, _stream(x, "linear"))
 
 
 class LayerNorm(nn.Module):

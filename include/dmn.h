@@ -330,6 +330,9 @@ size_t dmn_clip_grads_workspace_bytes(int n_tensors);
 int dmn_clip_grads(const DmnGradTensor* tensors, int n_tensors, int inf_norm, float max_norm, float grad_scale, float* norm,
                    void* workspace, size_t workspace_bytes, void* stream);
 
+/* 1 while work on `stream` is being recorded into a graph, else 0 (always 0 for NULL, the default stream, which cannot be). */
+int dmn_stream_is_capturing(void* stream);
+
 /* N(0,1) * scale into x[B][per] with the library's generator (prior draws; tests). */
 int dmn_fill_normal(float* x, int B, int per, uint64_t seed, uint32_t step, int64_t img_offset, float scale, void* stream);
 

@@ -153,3 +153,7 @@ def test_linear_entry_points_take_the_rounded_flag_with_an_activation_only():
     for act in (20, 31, 32, 8, -16):
         assert lib.dmn_linear_backward(X, 8, X, 8, X, X, X, X, X, 4, 8, 8, act, 1, None, 0, None) == -1
         assert lib.dmn_linear_forward(X, 8, X, None, None, 0, X, None, 4, 8, 8, act, 1, None, 0, None) == -1
+
+
+def test_default_stream_is_never_recorded():
+    assert _N().lib().dmn_stream_is_capturing(None) == 0

@@ -139,3 +139,71 @@ def test_rounded_backward_is_the_callers_choice(dtype, kind):
     if dtype == TYPES[0]:   # float32: there is nothing to choose
         assert all(torch.equal(p, q) for p, q in zip(grads_of(x, layer.weight, layer.bias, kind, dy), want))
     assert torch.equal(linear(x, layer.weight, layer.bias, None, rounded_backward=True), linear(x, layer.weight, layer.bias))
+
+
+def test_capture_guard_sees_leaves_behind_views_and_copies():
+    """A transposed weight, a view of an input and a strided bias are no leaves themselves; their gradients end in leaves all the same."""
+    from diffusion_model_nemo_amd.modules import layer_norm, linear
+    x, w, b = randn((130, 72), 1).requires_grad_(True), randn((72, 40), 2, scale=0.1).requires_grad_(True), randn((80,), 3).requires_grad_(True)
+    plain, fixed = randn((130, 72), 4), randn((40, 72), 5)
+    dy = randn((130, 40), 6)
+    calls = {"transposed weight": (lambda: linear(plain, w.t(), None, "gelu"), w), "strided bias": (lambda: linear(plain, fixed, b[::2]), b),
+             "view of x": (lambda: linear(x.view(13, 10, 72).reshape(130, 72) * 2, fixed), x),
+             "rows of x": (lambda: layer_norm(x[3:]), x), "strided scale": (lambda: layer_norm(randn_40, b[::2]), b)}
+    randn_40 = randn((9, 40), 7)
+    for name, (call, leaf) in calls.items():
+        alive = call()
+        with pytest.raises(RuntimeError, match="still lives"):
+            with torch.cuda.graph(torch.cuda.CUDAGraph()):
+                call()
+        del alive
+    # with the eager graphs gone: captured, replayed, and as the eager call
+    def step():
+        y = linear(x * 1.0, w.t(), b[::2], "gelu")
+        return (y.detach(),) + torch.autograd.grad(y, (x, w, b), dy)
+    graph = torch.cuda.CUDAGraph()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    with torch.cuda.graph(graph):
+        got = step()
+    for turn in range(3):
+        with torch.no_grad():
+            x.copy_(randn((130, 72), 20 + turn))
+        graph.replay()
+        kept = [g.clone() for g in got]
+        want = step()
+        torch.cuda.synchronize()
+        assert all(torch.equal(p, q) for p, q in zip(kept, want)), turn
+
+
+def test_forward_alone_is_captured_beside_an_eager_graph_and_on_a_forked_stream():
+    from diffusion_model_nemo_amd.modules import layer_norm, linear
+    x, w = randn((70, 72), 1).requires_grad_(True), randn((40, 72), 2, scale=0.1).requires_grad_(True)
+    alive = linear(layer_norm(x), w)
+    graph = torch.cuda.CUDAGraph()
+    with torch.no_grad(), torch.cuda.graph(graph):
+        y = linear(layer_norm(x), w)
+    for turn in range(3):
+        with torch.no_grad():
+            x.copy_(randn((70, 72), 10 + turn))
+        graph.replay()
+        kept = y.clone()
+        with torch.no_grad():
+            assert torch.equal(kept, linear(layer_norm(x), w)), turn
+    del alive
+    # a leaf whose first use lies on a stream that was forked into the capture itself
+    graph, fork = torch.cuda.CUDAGraph(), torch.cuda.Stream()
+    with torch.cuda.graph(graph):
+        fork.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(fork):
+            a = linear(x, w)
+        torch.cuda.current_stream().wait_stream(fork)
+        b = linear(x, w, activation="relu")
+        kept = (a.detach(), b.detach())
+        del a, b
+    graph.replay()
+    with torch.no_grad():
+        assert torch.equal(kept[0], linear(x, w)) and torch.equal(kept[1], linear(x, w, activation="relu"))
