@@ -8,6 +8,7 @@
 #include <c10/core/impl/DeviceGuardImplInterface.h>
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
+#include <torch/csrc/autograd/graph_task.h>
 #include <torch/csrc/autograd/python_variable.h>
 #include <torch/csrc/utils/pybind.h>
 
@@ -124,26 +125,43 @@ bool is_capturing(const c10::Stream& s) {
 // Under capture the gradients of a leaf would be accumulated on the stream on which an eager graph that still lives first
 // used the leaf; torch then touches that stream in the middle of the capture, and the process ends. The same holds for any node of
 // an eager graph that the backward would pass through. Such a call is refused, however far behind the inputs (views, transposes,
-// copies) the node lies; a stream that was forked into the same capture is none of these.
-void check_capture(int64_t stream, const Tensor& x, std::initializer_list<const Tensor*> inputs) {
-    if (!api.is_capturing(handle(stream))) return;
-    const c10::Stream now = c10::impl::getDeviceGuardImpl(c10::DeviceType::CUDA)->getStream(x.device());
-    std::vector<std::shared_ptr<torch::autograd::Node>> todo;
+// copies) the node lies; a stream that was forked into the same capture is none of these. `pass`: the nodes that the
+// backward will run (null: all).
+using ExecInfo = std::unordered_map<torch::autograd::Node*, torch::autograd::GraphTask::ExecInfo>;
+void check_nodes(std::vector<std::shared_ptr<torch::autograd::Node>> todo, const c10::Device& device, const ExecInfo* pass) {
+    const c10::Stream now = c10::impl::getDeviceGuardImpl(c10::DeviceType::CUDA)->getStream(device);
     std::unordered_set<torch::autograd::Node*> seen;
-    auto add = [&](const std::shared_ptr<torch::autograd::Node>& node) {
-        if (node && seen.insert(node.get()).second) todo.push_back(node);
-    };
-    for (const Tensor* t : inputs)
-        if (t->defined() && t->requires_grad()) add(t->is_leaf() ? torch::autograd::impl::try_get_grad_accumulator(*t) : t->grad_fn());
     while (!todo.empty()) {
         const auto node = todo.back();
         todo.pop_back();
+        if (!node || !seen.insert(node.get()).second) continue;
+        if (pass && !pass->empty()) {
+            const auto it = pass->find(node.get());
+            if (it == pass->end() || !it->second.should_execute()) continue;
+        }
         const auto stream = node->stream();
         if (stream.has_value() && *stream != now && !is_capturing(*stream))
             throw std::runtime_error("a graph is being captured while an eager graph over the same parameters or inputs, made on another stream, "
                                      "still lives: drop its results first (del loss, outputs), or warm up on the capturing stream");
-        for (const auto& edge : node->next_edges()) add(edge.function);
+        for (const auto& edge : node->next_edges()) todo.push_back(edge.function);
     }
+}
+void check_capture(int64_t stream, const Tensor& x, std::initializer_list<const Tensor*> inputs) {
+    if (!api.is_capturing(handle(stream))) return;
+    std::vector<std::shared_ptr<torch::autograd::Node>> nodes;
+    for (const Tensor* t : inputs)
+        if (t->defined() && t->requires_grad()) nodes.push_back(t->is_leaf() ? torch::autograd::impl::try_get_grad_accumulator(*t) : t->grad_fn());
+    check_nodes(std::move(nodes), x.device(), nullptr);
+}
+// The same for a backward pass that is captured while its forward was not (made eagerly on the capturing stream): asked before
+// the gradients are handed on.
+void check_captured_backward(int64_t stream, const c10::Device& device) {
+    if (!api.is_capturing(handle(stream))) return;
+    const auto self = torch::autograd::get_current_node();
+    if (!self) return;
+    std::vector<std::shared_ptr<torch::autograd::Node>> nodes;
+    for (const auto& edge : self->next_edges()) nodes.push_back(edge.function);
+    check_nodes(std::move(nodes), device, torch::autograd::get_current_graph_task_exec_info());
 }
 
 // ---- layer norm --------------------------------------------------------------------------------------------------------
@@ -180,6 +198,7 @@ struct LayerNormNode : torch::autograd::Function<LayerNormNode> {
             const Rows x = rows_of(saved[0]), dy = rows_of(grads[0]);
             const Tensor &weight = saved[1], &bias = saved[2], &stats = saved[3];
             c10::DeviceGuard guard(x.t.device());
+            check_captured_backward(ctx->saved_data["stream"].toInt(), x.t.device());
             const int64_t width = x.t.size(-1), rows = stats.size(0);
             const int code = code_of(x.t.scalar_type());
             size_t edge = 0;   // the node has an edge for every tensor that was given
@@ -254,6 +273,7 @@ struct LinearNode : torch::autograd::Function<LinearNode> {
             at::AutoGradMode off(false);
             const auto saved = ctx->get_saved_variables();
             const Tensor &weight = saved[1], &bias = saved[2], &z = saved[3];
+            check_captured_backward(ctx->saved_data["stream"].toInt(), weight.device());
             const bool need_x = ctx->needs_input_grad(0), need_w = ctx->needs_input_grad(1), need_b = bias.defined() && ctx->needs_input_grad(2);
             if (need_x || need_w || need_b) {
                 const Rows x = rows_of(saved[0], kLinearStride), dy = rows_of(grads[0], kLinearStride);

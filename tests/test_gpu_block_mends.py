@@ -207,3 +207,47 @@ def test_forward_alone_is_captured_beside_an_eager_graph_and_on_a_forked_stream(
     graph.replay()
     with torch.no_grad():
         assert torch.equal(kept[0], linear(x, w)) and torch.equal(kept[1], linear(x, w, activation="relu"))
+
+
+@pytest.mark.parametrize("op", ["linear", "layer_norm"])
+def test_captured_backward_of_an_eager_forward(op):
+    """Forward made eagerly on a stream, its backward captured there: refused while a leaf it ends in was first used on the default
+    stream by a graph that still lives, unless the gradients asked for do not pass that leaf."""
+    from diffusion_model_nemo_amd.modules import layer_norm, linear
+    x = randn((70, 72), 1).requires_grad_(True)
+    w = randn((72, 72), 2, scale=0.1).requires_grad_(True) if op == "linear" else randn((72,), 2).requires_grad_(True)
+    dy = randn((70, 72), 3)
+    call = (lambda h: linear(h, w)) if op == "linear" else (lambda h: layer_norm(h, w))
+    side = torch.cuda.Stream()
+    alive = call(x)
+    want = torch.autograd.grad(alive, (x, w), dy, retain_graph=True)
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        y = call(x)
+    with pytest.raises(RuntimeError, match="still lives"):
+        with torch.cuda.graph(torch.cuda.CUDAGraph(), stream=side):
+            torch.autograd.grad(y, (x, w), dy, retain_graph=True)
+    del y
+    with torch.cuda.stream(side):
+        h = x.detach().clone().requires_grad_(True)
+        y = call(h)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side):
+        (dx,) = torch.autograd.grad(y, (h,), dy, retain_graph=True)   # w's gradient is not asked for
+    for turn in range(3):
+        dx.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(dx, want[0]), turn
+    del y, alive
+    with torch.cuda.stream(side):
+        y = call(x)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side):
+        got = torch.autograd.grad(y, (x, w), dy, retain_graph=True)
+    for turn in range(3):
+        for g in got:
+            g.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(p, q) for p, q in zip(got, want)), turn
