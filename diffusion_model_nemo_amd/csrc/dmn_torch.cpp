@@ -10,6 +10,7 @@
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/autograd/graph_task.h>
 #include <torch/csrc/autograd/python_variable.h>
+#include <torch/csrc/jit/frontend/tracer.h>
 #include <torch/csrc/utils/pybind.h>
 
 #include <cstring>
@@ -67,6 +68,14 @@ void check_input(const Tensor& x, const char* what) {
     if (!x.is_cuda()) throw std::runtime_error(c10::str(what, " runs only on MI355X device tensors (no CPU implementation)"));
     if (code_of(x.scalar_type()) < 0 || x.layout() != at::kStrided)
         throw py::value_error(c10::str(what, ": dtype must be float32, bfloat16 or float16, got ", x.scalar_type(), " (", x.layout(), ")"));
+}
+// Only the reverse-mode nodes below know what the kernels compute. A dual tensor would come out without its tangent, which
+// reads as a derivative of zero, and a trace would hold the allocation of the output and nothing else: both are refused.
+void check_recorded(const char* what, std::initializer_list<const std::optional<Tensor>*> inputs) {
+    if (torch::jit::tracer::isTracing()) throw std::runtime_error(c10::str(what, " cannot be traced: its kernels are not torch operators"));
+    for (const auto* t : inputs)
+        if (t->has_value() && (*t)->_fw_grad(0).defined())
+            throw std::runtime_error(c10::str(what, " has no forward-mode derivative: an input is a dual tensor"));
 }
 // p on x's device, of `shape` and of x's type (or float32 where `or_float`); comes back contiguous
 Tensor checked_param(const std::optional<Tensor>& p, const char* name, at::IntArrayRef shape, const Tensor& x, bool or_float) {
@@ -216,6 +225,8 @@ struct LayerNormNode : torch::autograd::Function<LayerNormNode> {
 };
 
 Tensor layer_norm(const Tensor& x, const std::optional<Tensor>& weight_, const std::optional<Tensor>& bias_, double eps, int64_t stream) {
+    const std::optional<Tensor> x_(x);
+    check_recorded("layer_norm", {&x_, &weight_, &bias_});
     check_input(x, "layer_norm");
     if (x.dim() == 0 || x.size(-1) == 0) throw py::value_error("layer_norm needs a last axis of at least one element");
     if (x.size(-1) > INT32_MAX) throw py::value_error("layer_norm: the last axis is too long");
@@ -300,6 +311,8 @@ struct LinearNode : torch::autograd::Function<LinearNode> {
 
 Tensor linear(const Tensor& x, const Tensor& weight_, const std::optional<Tensor>& bias_, int64_t act, const std::optional<Tensor>& residual_,
               int64_t stream) {
+    const std::optional<Tensor> x_(x), w_(weight_);
+    check_recorded("linear", {&x_, &w_, &bias_, &residual_});
     check_input(x, "linear");
     if (weight_.dim() != 2 || weight_.size(0) == 0 || weight_.size(1) == 0 || weight_.size(0) > INT32_MAX || weight_.size(1) > INT32_MAX)
         throw py::value_error(c10::str("weight must be [out, in], got ", weight_.sizes()));
@@ -324,6 +337,7 @@ Tensor linear(const Tensor& x, const Tensor& weight_, const std::optional<Tensor
 // The ordinary case of training.clip_grad_norm_: every gradient (and every tensor of `out`) dense, contiguous, of the three
 // types and on one device. Anything else comes back as None, and Python takes it apart with its own words.
 py::object clip_grads(const py::list& params, const py::object& out, bool inf_norm, double max_norm, double grad_scale) {
+    if (torch::jit::tracer::isTracing()) throw std::runtime_error("clip_grad_norm_ cannot be traced: its kernels are not torch operators");
     const size_t n = params.size();
     const bool to_out = !out.is_none();
     py::list outs = to_out ? py::reinterpret_borrow<py::list>(out) : py::list();

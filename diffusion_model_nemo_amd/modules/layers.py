@@ -4,7 +4,8 @@ What the reference builds its blocks from outside the convolutions -- `Residual(
 (diffusion_model_nemo/utils.py:68-93) and the `nn.Linear` / `nn.GELU` pairs of its embedding networks
 (diffusion_model_nemo/modules/unet.py:59-66) -- as calls on device tensors with their backward passes. `layer_norm` and
 `linear` are differentiable torch functions; `LayerNorm` and `Linear` hold the parameters under torch's names, so
-`state_dict`s interchange with `torch.nn`. There is no CPU implementation: a CPU tensor raises.
+`state_dict`s interchange with `torch.nn`. There is no CPU implementation: a CPU tensor raises. So do dual tensors (forward-mode
+derivatives) and `torch.jit.trace`, which see nothing of what the kernels compute.
 
 Results are rounded once, to the input's type; sums, statistics and parameter gradients are formed in float32. The backward
 passes are not differentiable themselves. Calls and their backward passes can be captured into a graph; a call that would be

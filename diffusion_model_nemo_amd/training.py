@@ -258,6 +258,8 @@ def _dense(t: torch.Tensor) -> bool:
 def _clip_one_by_one(params, norm_type, max_norm, error_if_nonfinite, grad_scale, out):
     """`clip_grad_norm_` where it has to wait for the norm, and for gradients out of the ordinary: none at all, scattered or
     permuted ones, and those it refuses."""
+    if torch.jit.is_tracing():
+        raise RuntimeError("clip_grad_norm_ cannot be traced: its kernels are not torch operators")
     grads = [p.grad for p in params]
     if out is not None:
         out = [o for o, g in zip(out, grads) if g is not None]

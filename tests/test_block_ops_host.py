@@ -157,3 +157,34 @@ def test_linear_entry_points_take_the_rounded_flag_with_an_activation_only():
 
 def test_default_stream_is_never_recorded():
     assert _N().lib().dmn_stream_is_capturing(None) == 0
+
+
+def _unrecorded_calls(device):
+    """name -> (the call on one tensor, that tensor): every input of layer_norm and linear in turn."""
+    ops = _N().ops()
+    x, w, v, r = (torch.ones(s, device=device) for s in ((4, 8), (8, 8), (8,), (4, 8)))
+    s = 0 if device == "cpu" else torch._C._cuda_getCurrentRawStream(0)
+    return {"layer_norm x": (lambda t: ops.layer_norm(t, v, v, 1e-5, s), x), "layer_norm weight": (lambda t: ops.layer_norm(x, t, None, 1e-5, s), v),
+            "layer_norm bias": (lambda t: ops.layer_norm(x, None, t, 1e-5, s), v), "linear x": (lambda t: ops.linear(t, w, v, 3, r, s), x),
+            "linear weight": (lambda t: ops.linear(x, t, None, 0, None, s), w), "linear bias": (lambda t: ops.linear(x, w, t, 1, None, s), v),
+            "linear residual": (lambda t: ops.linear(x, w, None, 0, t, s), r)}
+
+
+@pytest.mark.parametrize("device", ["cpu", pytest.param("cuda", marks=pytest.mark.gpu)])
+def test_forward_mode_derivatives_and_traces_are_refused(device):
+    """They would come out as a derivative of zero, and as a traced module that returns memory nobody wrote."""
+    from torch.autograd import forward_ad
+    from diffusion_model_nemo_amd.training import clip_grad_norm_
+    for name, (call, t) in _unrecorded_calls(device).items():
+        with forward_ad.dual_level():
+            dual = forward_ad.make_dual(t, torch.ones_like(t))
+            with pytest.raises(RuntimeError, match="forward-mode"):
+                call(dual)
+        with pytest.raises(RuntimeError, match="cannot be traced"):
+            torch.jit.trace(call, (t,), check_trace=False)
+    p = torch.nn.Parameter(torch.ones(4, device=device))
+    p.grad = torch.ones(4, device=device)
+    for finite in (False, True):
+        with pytest.raises(RuntimeError, match="cannot be traced"):
+            torch.jit.trace(lambda t: t + clip_grad_norm_([p], 1.0, error_if_nonfinite=finite), (p.detach(),), check_trace=False)
+    assert bool((p.grad == 1).all())
