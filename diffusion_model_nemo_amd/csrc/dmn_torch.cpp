@@ -271,7 +271,10 @@ struct LinearNode : torch::autograd::Function<LinearNode> {
         const bool want_z = (act & ~DMN_LINEAR_ROUNDED) != 0 && (x.requires_grad() || weight.requires_grad() || (bias.defined() && bias.requires_grad()));
         Tensor z;
         Tensor y = linear_run(r, weight, bias, or_none(residual), act, stream, want_z ? &z : nullptr);
-        ctx->save_for_backward({r.t, weight, bias, z});
+        // x for dW and the weight for dx alone: what is not needed is not kept, and may be overwritten before the backward
+        ctx->save_for_backward({weight.requires_grad() ? r.t : Tensor(), x.requires_grad() ? weight : Tensor(), z});
+        ctx->saved_data["x"] = x.sizes();
+        ctx->saved_data["weight"] = weight.sizes();
         ctx->saved_data["act"] = act;
         ctx->saved_data["stream"] = stream;
         ctx->saved_data["bias"] = bias.defined();
@@ -283,22 +286,24 @@ struct LinearNode : torch::autograd::Function<LinearNode> {
         {
             at::AutoGradMode off(false);
             const auto saved = ctx->get_saved_variables();
-            const Tensor &weight = saved[1], &bias = saved[2], &z = saved[3];
-            check_captured_backward(ctx->saved_data["stream"].toInt(), weight.device());
-            const bool need_x = ctx->needs_input_grad(0), need_w = ctx->needs_input_grad(1), need_b = bias.defined() && ctx->needs_input_grad(2);
+            const Tensor &weight = saved[1], &z = saved[2];
+            const bool need_x = ctx->needs_input_grad(0), need_w = ctx->needs_input_grad(1);
+            const bool need_b = ctx->saved_data["bias"].toBool() && ctx->needs_input_grad(2);
+            check_captured_backward(ctx->saved_data["stream"].toInt(), grads[0].device());
             if (need_x || need_w || need_b) {
-                const Rows x = rows_of(saved[0], kLinearStride), dy = rows_of(grads[0], kLinearStride);
-                c10::DeviceGuard guard(x.t.device());
-                const int64_t n = weight.size(0), width = weight.size(1), rows = x.t.numel() / width, act = ctx->saved_data["act"].toInt();
-                const int code = code_of(x.t.scalar_type());
-                if (need_x) out[0] = new_like(x.t);
-                if (need_w) out[1] = new_like(weight);
-                if (need_b) out[2] = new_like(bias);
-                const size_t bytes = api.linear_backward_workspace(dy.t.data_ptr(), dy.ld, x.t.data_ptr(), x.ld, weight.data_ptr(), rows, (int)width,
-                                                                   (int)n, (int)act, code);
-                const Tensor ws = workspace(bytes, x.t);
-                check_backward(api.linear_backward(dy.t.data_ptr(), dy.ld, x.t.data_ptr(), x.ld, weight.data_ptr(), ptr(z), ptr(out[0]), ptr(out[1]),
-                                                   ptr(out[2]), rows, (int)width, (int)n, (int)act, code, ptr(ws), bytes,
+                const auto w_shape = ctx->saved_data["weight"].toIntVector();
+                const int64_t n = w_shape[0], width = w_shape[1], rows = grads[0].numel() / n, act = ctx->saved_data["act"].toInt();
+                const Rows x = need_w ? rows_of(saved[0], kLinearStride) : Rows{Tensor(), width}, dy = rows_of(grads[0], kLinearStride);
+                c10::DeviceGuard guard(dy.t.device());
+                const int code = code_of(dy.t.scalar_type());
+                if (need_x) out[0] = at::empty(ctx->saved_data["x"].toIntVector(), dy.t.options());
+                if (need_w) out[1] = at::empty(w_shape, dy.t.options());
+                if (need_b) out[2] = at::empty({n}, dy.t.options());
+                const size_t bytes = api.linear_backward_workspace(dy.t.data_ptr(), dy.ld, ptr(x.t), x.ld, ptr(weight), rows, (int)width, (int)n,
+                                                                   (int)act, code);
+                const Tensor ws = workspace(bytes, dy.t);
+                check_backward(api.linear_backward(dy.t.data_ptr(), dy.ld, ptr(x.t), x.ld, ptr(weight), ptr(z), ptr(out[0]), ptr(out[1]), ptr(out[2]),
+                                                   rows, (int)width, (int)n, (int)act, code, ptr(ws), bytes,
                                                    handle(ctx->saved_data["stream"].toInt())));
             }
         }

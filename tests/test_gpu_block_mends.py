@@ -251,3 +251,30 @@ def test_captured_backward_of_an_eager_forward(op):
         graph.replay()
         torch.cuda.synchronize()
         assert all(torch.equal(p, q) for p, q in zip(got, want)), turn
+
+
+@pytest.mark.parametrize("kind", [None, "gelu"])
+def test_linear_keeps_only_what_its_gradients_need(kind):
+    """A frozen layer's input may be overwritten before the backward, and the weight of a layer whose input needs no gradient, as with
+    torch's own linear layer; what a gradient does need is still guarded."""
+    from diffusion_model_nemo_amd.modules import linear
+    x, w, b, r, dy = randn((70, 72), 1), randn((40, 72), 2, scale=0.1), randn((40,), 3), randn((70, 40), 4), randn((70, 40), 5)
+    want = torch.autograd.grad(linear(*(t.requires_grad_(True) for t in (x, w, b)), kind, r.requires_grad_(True)), (x, w, b, r), dy)
+    for i, harmless in enumerate(((0, 2, 3), (1, 2, 3), (0, 1, 2, 3), (0, 1, 2, 3))):
+        args = [t.detach().clone().requires_grad_(i == j) for j, t in enumerate((x, w, b, r))]
+        y = linear(args[0], args[1], args[2], kind, args[3])
+        with torch.no_grad():
+            for j in harmless:
+                args[j].add_(1.0)
+        (got,) = torch.autograd.grad(y, args[i], dy, retain_graph=True)
+        assert torch.equal(got, want[i]), i
+        for j in set(range(2)) - set(harmless):
+            with torch.no_grad():
+                args[j].add_(1.0)
+            with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+                torch.autograd.grad(y, args[i], dy, retain_graph=True)
+    frozen, given = torch.nn.Parameter(w.detach().clone(), requires_grad=False), x.detach().clone().requires_grad_(True)
+    torch.cuda.synchronize()
+    before = torch.cuda.memory_allocated()
+    y = linear(given * 1.0, frozen)
+    assert torch.cuda.memory_allocated() - before <= y.numel() * y.element_size() + 512     # the product's input is gone again
