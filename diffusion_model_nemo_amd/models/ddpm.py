@@ -220,6 +220,21 @@ class DDPM(AbstractDiffusionModel):
             object.__setattr__(self, "_native_trainer", tr)
         return tr
 
+    def _trainer_value(self, key):
+        """A trainer's setting: an object or mapping handed to the constructor wins over the YAML's section."""
+        for src in (self.trainer, getattr(self, 'trainer_cfg', None)):
+            if src is None:
+                continue
+            v = src.get(key, None) if isinstance(src, dict) else getattr(src, key, None)
+            if v is not None:
+                return v
+        return None
+
+    def _clip_value(self) -> float:
+        """`trainer.gradient_clip_val`, 0 where there is none; whatever the optimizer."""
+        clip = self._trainer_value('gradient_clip_val')
+        return 0.0 if clip is None else float(clip)
+
     def _optim_settings(self):
         """AdamW arguments, learning-rate policy and clip value as the reference's trainer would apply them
         (examples/configs/ddpm/unet_small.yaml:65-78,83-84,90)."""
@@ -228,28 +243,18 @@ class DDPM(AbstractDiffusionModel):
         if name != 'adamw':
             raise NotImplementedError(f"optimizer '{name}': only adamw is built")
         sched = optim.get('sched', None) or {}
-        def trainer_value(key):   # a trainer object / mapping handed to the constructor wins over the YAML's section
-            for src in (self.trainer, getattr(self, 'trainer_cfg', None)):
-                if src is None:
-                    continue
-                v = src.get(key, None) if isinstance(src, dict) else getattr(src, key, None)
-                if v is not None:
-                    return v
-            return None
-
         sname = sched.get('name', None)
         if sname not in (None, 'CosineAnnealing'):
             raise NotImplementedError(f"learning-rate policy '{sname}': only CosineAnnealing is built")
-        max_steps = sched.get('max_steps', None) or trainer_value('max_steps')
+        max_steps = sched.get('max_steps', None) or self._trainer_value('max_steps')
         if max_steps is not None and int(max_steps) <= 0:
             max_steps = None
-        clip = trainer_value('gradient_clip_val')
         return {"lr": float(optim.get('lr', 1e-3)), "betas": tuple(optim.get('betas', (0.9, 0.999))),
                 "eps": float(optim.get('eps', 1e-8)), "weight_decay": float(optim.get('weight_decay', 0.01)),
                 "sched": sname, "min_lr": float(sched.get('min_lr', 0.0) or 0.0),
                 "warmup_steps": int(sched.get('warmup_steps', 0) or 0),
                 "max_steps": None if max_steps is None else int(max_steps),
-                "clip": 0.0 if clip is None else float(clip)}
+                "clip": self._clip_value()}
 
     def learning_rate(self, step: int) -> float:
         """Learning rate of optimisation step `step` (0-based) under the config's policy: CosineAnnealing from `lr` to
@@ -298,7 +303,7 @@ class DDPM(AbstractDiffusionModel):
         from ..training import clip_grad_norm_
         if gradient_clip_algorithm not in (None, 'norm'):
             raise NotImplementedError(f"gradient_clip_algorithm '{gradient_clip_algorithm}': only 'norm' is built")
-        value = self._optim_settings()["clip"] if gradient_clip_val is None else float(gradient_clip_val)
+        value = self._clip_value() if gradient_clip_val is None else float(gradient_clip_val)
         if value == 0.0:
             return None
         return clip_grad_norm_([p for group in optimizer.param_groups for p in group["params"]], value)

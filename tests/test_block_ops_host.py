@@ -188,3 +188,20 @@ def test_forward_mode_derivatives_and_traces_are_refused(device):
         with pytest.raises(RuntimeError, match="cannot be traced"):
             torch.jit.trace(lambda t: t + clip_grad_norm_([p], 1.0, error_if_nonfinite=finite), (p.detach(),), check_trace=False)
     assert bool((p.grad == 1).all())
+
+
+def test_gradient_clipping_hook_works_beside_any_optimizer(monkeypatch):
+    """The hook is the autograd route's, with whatever torch optimizer and learning-rate policy the config names."""
+    from diffusion_model_nemo_amd import training
+    from diffusion_model_nemo_amd.models import DDPM
+    seen = []
+    monkeypatch.setattr(training, "clip_grad_norm_", lambda params, value: seen.append(value) or torch.tensor(3.0))
+    cfg = {"image_size": 32, "timesteps": 10, "channels": 3, "optim": {"name": "sgd", "lr": 0.1, "sched": {"name": "StepLR"}},
+           "diffusion_model": {"_target_": "diffusion_model_nemo.modules.Unet", "input_dim": 32, "dim": 32, "use_convnext": False},
+           "sampler": {"_target_": "diffusion_model_nemo.modules.GaussianDiffusion", "timesteps": 10, "schedule_name": "linear"},
+           "loss": {"_target_": "diffusion_model_nemo.loss.DiffusionLoss", "loss_type": "l2"}}
+    m = DDPM(cfg, trainer={"gradient_clip_val": 0.5})
+    assert float(m.configure_gradient_clipping(torch.optim.SGD(m.parameters(), lr=0.1))) == 3.0 and seen == [0.5]
+    assert DDPM(cfg).configure_gradient_clipping(torch.optim.SGD(m.parameters(), lr=0.1)) is None
+    with pytest.raises(NotImplementedError):
+        m._optim_settings()          # the all-device step stays AdamW
