@@ -230,10 +230,16 @@ class DDPM(AbstractDiffusionModel):
                 return v
         return None
 
-    def _clip_value(self) -> float:
-        """`trainer.gradient_clip_val`, 0 where there is none; whatever the optimizer."""
-        clip = self._trainer_value('gradient_clip_val')
-        return 0.0 if clip is None else float(clip)
+    def _clip_value(self, value=None, algorithm: Optional[str] = None) -> float:
+        """The 2-norm to clip to, 0 where nothing is clipped: `value`, or else the config's `trainer.gradient_clip_val`. A way of
+        clipping (given or configured) other than by the norm is refused where there is something to clip."""
+        value = self._trainer_value('gradient_clip_val') if value is None else value
+        value = 0.0 if value is None else float(value)
+        configured = self._trainer_value('gradient_clip_algorithm') if value != 0.0 else None
+        algorithm = configured if algorithm is None else algorithm
+        if algorithm not in (None, 'norm'):
+            raise NotImplementedError(f"gradient_clip_algorithm '{algorithm}': only 'norm' is built")
+        return value
 
     def _optim_settings(self):
         """AdamW arguments, learning-rate policy and clip value as the reference's trainer would apply them
@@ -298,12 +304,11 @@ class DDPM(AbstractDiffusionModel):
                                     gradient_clip_algorithm: Optional[str] = None):
         """What a trainer's loop calls between `loss.backward()` and `optimizer.step()` (Lightning's hook of this name):
         clips the `.grad`s of the optimizer's parameters to the global 2-norm `gradient_clip_val` (default: the config's
-        `trainer.gradient_clip_val`; None or 0: no clipping) with `training.clip_grad_norm_`. Returns the norm as a device
+        `trainer.gradient_clip_val`; None or 0: no clipping) with `training.clip_grad_norm_`. `gradient_clip_algorithm` (default:
+        the config's `trainer.gradient_clip_algorithm`) is 'norm' or nothing; others are refused. Returns the norm as a device
         scalar, or None where nothing is clipped."""
         from ..training import clip_grad_norm_
-        if gradient_clip_algorithm not in (None, 'norm'):
-            raise NotImplementedError(f"gradient_clip_algorithm '{gradient_clip_algorithm}': only 'norm' is built")
-        value = self._clip_value() if gradient_clip_val is None else float(gradient_clip_val)
+        value = self._clip_value(gradient_clip_val, gradient_clip_algorithm)
         if value == 0.0:
             return None
         return clip_grad_norm_([p for group in optimizer.param_groups for p in group["params"]], value)

@@ -205,3 +205,25 @@ def test_gradient_clipping_hook_works_beside_any_optimizer(monkeypatch):
     assert DDPM(cfg).configure_gradient_clipping(torch.optim.SGD(m.parameters(), lr=0.1)) is None
     with pytest.raises(NotImplementedError):
         m._optim_settings()          # the all-device step stays AdamW
+
+
+def test_configured_clipping_by_value_is_refused_instead_of_clipped_by_norm(monkeypatch):
+    from diffusion_model_nemo_amd import training
+    from diffusion_model_nemo_amd.models import DDPM
+    seen = []
+    monkeypatch.setattr(training, "clip_grad_norm_", lambda params, value: seen.append(value) or torch.tensor(3.0))
+    cfg = {"image_size": 32, "timesteps": 10, "channels": 3,
+           "diffusion_model": {"_target_": "diffusion_model_nemo.modules.Unet", "input_dim": 32, "dim": 32, "use_convnext": False},
+           "sampler": {"_target_": "diffusion_model_nemo.modules.GaussianDiffusion", "timesteps": 10, "schedule_name": "linear"},
+           "loss": {"_target_": "diffusion_model_nemo.loss.DiffusionLoss", "loss_type": "l2"}}
+    m = DDPM(cfg, trainer={"gradient_clip_val": 0.5, "gradient_clip_algorithm": "value"})
+    opt = torch.optim.SGD(m.parameters(), lr=0.1)
+    for kw in ({}, {"gradient_clip_val": 2.0}):
+        with pytest.raises(NotImplementedError, match="value"):
+            m.configure_gradient_clipping(opt, **kw)
+    with pytest.raises(NotImplementedError, match="value"):
+        m._optim_settings()
+    assert m.configure_gradient_clipping(opt, gradient_clip_val=0.0) is None and not seen
+    m.configure_gradient_clipping(opt, gradient_clip_algorithm="norm")       # the caller's word is the last
+    assert seen == [0.5]
+    assert DDPM(cfg, trainer={"gradient_clip_algorithm": "value"}).configure_gradient_clipping(opt) is None
