@@ -195,9 +195,11 @@ constexpr unsigned kOutOfRange = 0x80000000u;   // byte offset behind every buff
 
 // 16 bytes per lane from a buffer to LDS, lane l's at dst + 16 l. As assembly, because behind the builtin the compiler
 // waits for ALL outstanding requests in front of every transposing LDS read, which leaves nothing in flight (the
-// narrow dx product took 80 us instead of 41). No register is written; the kernel waits for arrivals itself. The s_nop
-// covers the wait states between a scalar write of m0 (or a vector write of the descriptor) and the request; nothing else in
-// these kernels uses m0.
+// narrow dx product took 80 us instead of 41). The kernel waits for arrivals itself. The s_nop covers the wait states between a
+// scalar write of m0 (or a vector write of the descriptor) and the request. m0 cannot be declared as overwritten (it is reserved);
+// the build checks that nothing else in these kernels uses it (isa_check.py). The write to LDS is not declared either: a memory
+// clobber here costs 1 % (8192 x 2048 into 8192 259 : 262 us). It is not needed, because between two of the kernel's barriers, which
+// do carry one (the waits), requests go to a stage that no read touches: reads may pass requests, but never a barrier.
 __device__ __forceinline__ void load_to_lds(u32x4 rsrc, unsigned offset, unsigned dst) {
     asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" : : "s"(dst), "v"(offset), "s"(rsrc));
 }

@@ -1,4 +1,5 @@
-"""Static check of the device code inside libdmn_hip.so: no packed-FP32 VALU instruction may be present.
+"""Static checks of the device code inside libdmn_hip.so: no packed-FP32 VALU instruction may be present, kernels that wait
+for each other stay small enough, and m0 belongs to the requests to LDS that write it.
 
 Why: with ``v_pk_add_f32 / v_pk_mul_f32 / v_pk_fma_f32`` in the kernels (the SLP vectoriser emits them for the
 epilogues) this library returned wrong GroupNorm partial sums and linear-attention merge rows in lanes 48..63 of a
@@ -115,6 +116,50 @@ def assert_exchanging_kernels_fit_half_a_cu(lib_path: str) -> Dict[str, int]:
     return regs
 
 
+# Kernels that write m0 in inline assembly for their requests to LDS (csrc/dmn_linear.hip, load_to_lds). The register cannot be
+# declared as overwritten (the compiler keeps it for itself and warns), so the result is looked at: every instruction that names
+# it has to be such a request's own write, right in front of the request.
+REQUESTING = re.compile(r"gemm_(pipe|pair)_kernel")
+
+
+def foreign_m0_uses(disassembly: str) -> Dict[str, List[str]]:
+    """kernel symbol -> instructions on m0 that are not `s_mov_b32 m0, sN` with `s_nop 4` and a load to LDS right behind it, for
+    every requesting kernel of a disassembly."""
+    out: Dict[str, List[str]] = {}
+    name, code = None, []
+
+    def close():
+        if name is None or not REQUESTING.search(name):
+            return
+        out[name] = [ln for i, ln in enumerate(code)
+                     if re.search(r"\bm0\b", ln) and not (re.match(r"s_mov_b32 m0, s\d+$", ln) and code[i + 1:i + 2] == ["s_nop 4"] and i + 2 < len(code)
+                                                           and re.match(r"buffer_load_dwordx4 .* offen lds$", code[i + 2]))]
+
+    for ln in disassembly.splitlines():
+        m = re.match(r"[0-9a-f]+ <(.+)>:$", ln)
+        if m:
+            close()
+            name, code = m.group(1), []
+        elif ln.startswith("\t"):
+            code.append(ln.split("//")[0].strip())
+    close()
+    return out
+
+
+def assert_m0_is_the_requests_own(lib_path: str) -> int:
+    """Number of requesting kernels looked at."""
+    found: Dict[str, List[str]] = {}
+    with tempfile.TemporaryDirectory(prefix="dmn_isa_") as tmp:
+        for co in extract_code_objects(lib_path, tmp):
+            found.update(foreign_m0_uses(disassemble(co)))
+    if not found:
+        raise RuntimeError(f"{lib_path}: no requesting kernel found (symbol pattern out of date?)")
+    bad = {k: v for k, v in found.items() if v}
+    if bad:
+        raise RuntimeError(f"{lib_path}: m0 is used beside the requests to LDS: {bad}. Their inline assembly overwrites it.")
+    return len(found)
+
+
 if __name__ == "__main__":
     here = os.path.dirname(os.path.abspath(__file__))
     path = sys.argv[1] if len(sys.argv) > 1 else os.path.join(here, "lib", "libdmn_hip.so")
@@ -125,4 +170,5 @@ if __name__ == "__main__":
             total[k] += c[k]
     print(f"total: {total}")
     regs = assert_exchanging_kernels_fit_half_a_cu(path)
+    print(f"kernels whose requests to LDS own m0: {assert_m0_is_the_requests_own(path)}")
     print(f"exchanging kernels: {len(regs)}, registers per lane {min(regs.values())}..{max(regs.values())} (limit {MAX_EXCHANGING_REGS})")

@@ -227,3 +227,17 @@ def test_configured_clipping_by_value_is_refused_instead_of_clipped_by_norm(monk
     m.configure_gradient_clipping(opt, gradient_clip_algorithm="norm")       # the caller's word is the last
     assert seen == [0.5]
     assert DDPM(cfg, trainer={"gradient_clip_algorithm": "value"}).configure_gradient_clipping(opt) is None
+
+
+def test_m0_belongs_to_the_requests_that_write_it():
+    """Their inline assembly overwrites m0 and cannot declare it: nothing else in those kernels may use it."""
+    from diffusion_model_nemo_amd import isa_check
+    assert isa_check.assert_m0_is_the_requests_own(_N().LIB_PATH) >= 40
+    own = ["s_mov_b32 m0, s4", "s_nop 4", "buffer_load_dwordx4 v3, s[8:11], 0 offen lds"]
+    kernel = lambda *code: "0000000000001000 <_ZN1a16gemm_pipe_kernelIfEEv>:\n" + "".join(f"\t{c} // 000000001000: BF800004\n" for c in code)  # noqa: E731
+    bad = lambda *code: list(isa_check.foreign_m0_uses(kernel(*code)).values())  # noqa: E731
+    assert bad("v_add_f32_e32 v0, v1, v2", *own, *own) == [[]]
+    assert bad(*own, "s_mov_b32 s3, m0") == [["s_mov_b32 s3, m0"]]                     # somebody keeps a value there
+    assert bad("s_mov_b32 m0, -1", *own) == [["s_mov_b32 m0, -1"]]
+    assert bad(own[0], "s_nop 0", own[2]) == [[own[0]]] and bad(own[0], own[1]) == [[own[0]]]
+    assert isa_check.foreign_m0_uses(kernel(*own).replace("gemm_pipe", "other")) == {}
