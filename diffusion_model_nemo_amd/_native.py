@@ -92,6 +92,7 @@ SIGNATURES = {
     "dmn_clip_grads_workspace_bytes": (_sz, [_i]),
     "dmn_clip_grads": (_i, [_vp, _i, _i, _f, _f, _vp, _vp, _sz, _vp]),
     "dmn_stream_is_capturing": (_i, [_vp]),
+    "dmn_test_linear_plan": (_i, [_i64, _i, _i, _i, _i, _i, C.POINTER(_i)]),
     "dmn_fill_normal": (_i, [_vp, _i, _i, _u64, C.c_uint32, _i64, _f, _vp]),
     "dmn_unet_set_sample_chains": (_i, [_vp, _i, _i]),
     "dmn_ddpm_loop_chains": (_i, [_vp, _i]),

@@ -1184,3 +1184,17 @@ extern "C" int dmn_linear_backward(const void* dy, int64_t lddy, const void* x, 
     if (dtype == DMN_DT_BF16) return backward_run<__bf16>(dy, lddy, x, ldx, weight, z, dx, dweight, dbias, (int)rows, in, out, activation, dtype, ws, s);
     return backward_run<f16>(dy, lddy, x, ldx, weight, z, dx, dweight, dbias, (int)rows, in, out, activation, dtype, ws, s);
 }
+
+extern "C" int dmn_test_linear_plan(int64_t rows, int in, int out, int activation, int dtype, int alone, int* plan) {
+    const int rc = linear_check("dmn_test_linear_plan", rows, in, out, activation, dtype, in);
+    if (rc) return rc;
+    DMN_REQUIRE(plan && rows > 0, DMN_ERR_INVALID, "dmn_test_linear_plan: null argument or no rows");
+    const int parts = dz_parts(activation, dtype);
+    const GemmPlan f = gemm_plan((int)rows, out, in, dtype, 1);
+    PairPlan b = pair_plan((int)rows, in, out, dtype, parts);
+    if (alone) b = {false, gemm_plan((int)rows, in, out, dtype, parts), gemm_plan(out, in, (int)rows, dtype, parts)};
+    const bool few = few_rows({nullptr, in, out, in}, (int)rows, dtype);
+    const int all[7] = {few ? -1 : f.tile, few ? 1 : f.splits, b.together, b.dx.tile, b.dx.splits, b.dw.tile, b.dw.splits};
+    for (int i = 0; i < 7; ++i) plan[i] = all[i];
+    return DMN_OK;
+}

@@ -367,6 +367,11 @@ int dmn_test_attention(int dtype, const void* qkv, void* out, int B, int n, int 
 int dmn_test_attn_train(int adt, const void* qkv, const void* dout, void* out, void* dqkv, float* lse, int B, int n, int heads,
                         int bf16_operands, void* stream);
 
+/* Unit-test hook: which kernels dmn_linear_* takes for a layer with its operands on 16-byte boundaries (host only). plan[7]: tile of
+ * the forward (0: 256 x 256, 1: 128 x 128 with four stages, 2: with two, 3: 64 x 64, -1: the kernel for few rows) and its k
+ * splits; whether dx and dweight share a launch; tile and splits of dx, of dweight (with `alone` as when only one is asked for). */
+int dmn_test_linear_plan(int64_t rows, int in, int out, int activation, int dtype, int alone, int* plan);
+
 /* Diagnosis: after every launch of a forward, a checksum of the whole workspace goes to slot k of a device array. */
 int dmn_test_unet_trace(DmnUnet* u, unsigned long long* slots, int max_slots);
 int dmn_test_unet_trace_count(const DmnUnet* u);

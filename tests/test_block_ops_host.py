@@ -241,3 +241,35 @@ def test_m0_belongs_to_the_requests_that_write_it():
     assert bad("s_mov_b32 m0, -1", *own) == [["s_mov_b32 m0, -1"]]
     assert bad(own[0], "s_nop 0", own[2]) == [[own[0]]] and bad(own[0], own[1]) == [[own[0]]]
     assert isa_check.foreign_m0_uses(kernel(*own).replace("gemm_pipe", "other")) == {}
+
+
+def test_every_compiled_tile_has_a_tested_size():
+    """The sizes of test_every_tile_type_and_layout against the planner: a change of its model must not move them off a kernel."""
+    from test_gpu_block_mends import EVERY_TILE
+    lib = _N().lib()
+    seen = set()
+    for m, k, n, kind in EVERY_TILE:
+        act = 0 if kind is None else 3
+        for dt in range(3) if act == 0 else (1, 2):
+            for alone in (0, 1):
+                p = (C.c_int * 7)()
+                assert lib.dmn_test_linear_plan(m, k, n, act, dt, alone, p) == 0
+                two = act > 0
+                seen.add(("forward", dt, p[0]))
+                seen.add(("forward split", dt, p[0] if p[1] > 1 else None))
+                if p[2]:
+                    seen |= {("pair", dt, two, p[3]), ("pair split", dt, two, p[3], p[4] > 1, p[6] > 1)}
+                else:
+                    seen |= {("dx", dt, two, p[3]), ("dw", dt, two, p[5]), ("dx split", dt, two, p[3], p[4] > 1), ("dw split", dt, two, p[5], p[6] > 1)}
+                    if not alone:
+                        seen.add(("one after the other", dt, two))
+    for dt in range(3):
+        want = {("forward", dt, t) for t in (-1, 0, 1, 2, 3)} | {("forward split", dt, t) for t in (0, 1, 2, 3)}
+        for two in (False, True)[:1 if dt == 0 else 2]:
+            want |= {(op, dt, two, t) for op in ("dx", "dw") for t in range(4)} | {("pair", dt, two, t) for t in (2, 3)} | {("one after the other", dt, two)}
+            want |= {(op + " split", dt, two, t, True) for op in ("dx", "dw") for t in range(4) if not (op == "dw" and t == 2 and not two and dt)}
+            want |= {("pair split", dt, two, t, a, b) for t in (2, 3) for a in (False, True) for b in (False, True)}
+        assert want <= seen, sorted(map(str, want - seen))
+    p = (C.c_int * 7)()
+    assert lib.dmn_test_linear_plan(0, 8, 8, 0, 0, 0, p) == -1 and lib.dmn_test_linear_plan(8, 8, 8, 4, 0, 0, p) == -1
+    assert lib.dmn_test_linear_plan(8, 8, 8, 0, 0, 0, None) == -1

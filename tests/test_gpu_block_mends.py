@@ -3,7 +3,7 @@ with the bounds of `check_linear` (tests/test_gpu_block_ops.py), or as refusals.
 import pytest
 import torch
 
-from test_gpu_block_ops import BF, HF, TYPES, U, act_formula, close, floor_of, half_step, product, randn
+from test_gpu_block_ops import BF, F32, HF, TYPES, U, act_formula, close, floor_of, half_step, product, randn
 
 pytestmark = pytest.mark.gpu
 
@@ -58,6 +58,17 @@ def test_slopes_at_infinite_sums_are_their_limits(dtype, kind):
     assert bool((db[6:] == 35).all()) and bool((db[:3] == 35).all())
 
 
+# rows, in, out, activation: together they take every compiled tile in every type and operand layout, with k whole and split, dx and
+# dweight in one launch, one after the other and alone, dz in one part and in two (test_block_ops_host.py asserts it).
+EVERY_TILE = [(1, 33, 33, None), (1, 33, 33, "gelu"), (1, 33, 520, "gelu"), (1, 33, 1016, None), (510, 33, 33, "gelu"), (1020, 33, 33, None),
+              (20, 4104, 33, None), (1, 1016, 16360, "gelu"), (1, 1016, 4104, None), (1, 1016, 4104, "gelu"), (1, 2040, 16360, None),
+              (1020, 33, 520, "gelu"), (321, 136, 16360, "gelu"), (1020, 16360, 250, None), (4090, 1016, 1016, "gelu"), (321, 16360, 136, "gelu"),
+              (8184, 250, 8184, None), (2050, 2040, 33, None), (4090, 33, 2040, None), (8184, 136, 8184, "gelu"), (1020, 16360, 1016, "gelu"),
+              (1030, 2040, 2040, None), (8184, 520, 8184, None), (130, 16360, 8184, "gelu"), (8184, 16360, 136, "gelu"), (250, 1016, 16360, None),
+              (8184, 1016, 16360, None), (8184, 16360, 1016, None), (16368, 504, 16360, None), (321, 8184, 1016, "gelu"),
+              (8184, 136, 8184, None), (120, 8184, 16360, None), (4090, 1016, 1016, None)]
+
+
 def check_gradients(m, k, n, dtype, kind, rounded=False, scale=1.0, one_by_one=False):
     """dx, dweight and dbias with ONE rounding (the result's) and float32 work in front of it; `rounded` adds half a step of z and
     of dz. Two numbers of the type hold dz to half_step squared of it (float16: down to 2^-35, as its low part is kept 2^11
@@ -66,11 +77,11 @@ def check_gradients(m, k, n, dtype, kind, rounded=False, scale=1.0, one_by_one=F
     x, w, b = randn((m, k), 1, dtype), randn((n, k), 2, dtype, k ** -0.5), randn((n,), 3, dtype, 0.3)
     dy = randn((m, n), 4, dtype, scale)
     got = grads_of(x, w, b, kind, dy, rounded_backward=rounded)
-    if one_by_one:   # each product in a launch of its own
+    alone = ()
+    if one_by_one:   # each product in a launch of its own too
         for i in range(2):
             leaves = [t.detach().requires_grad_(i == j) for j, t in enumerate((x, w, b))]
-            (g,) = torch.autograd.grad(linear(*leaves, kind, rounded_backward=rounded), leaves[i], dy)
-            got = got[:1 + i] + (g,) + got[2 + i:]
+            alone += torch.autograd.grad(linear(*leaves, kind, rounded_backward=rounded), leaves[i], dy)
     z, za = product(x, w.t())
     ez = (k + 64) * U * za + 4 * U * (z.abs() + 2 * b.double().abs())
     z = z + b.double()
@@ -83,15 +94,19 @@ def check_gradients(m, k, n, dtype, kind, rounded=False, scale=1.0, one_by_one=F
         edz = edz + d.abs() * 1.2 * (h * z.abs() + floor_of(dtype))
     if kind == "relu":   # the slope jumps at 0: only where the sign is in doubt, and there by all of dy
         edz = torch.where(z.abs() <= ez + (floor_of(dtype) if rounded else 0), d.abs(), torch.zeros_like(dz))
-    part = h * dz.abs() + floor_of(dtype) if rounded else h * h * dz.abs() + (2.0 ** -35 if dtype == HF else 2.0 ** -140)
+    if kind is None:     # dz is dy itself
+        edz = torch.zeros_like(dz)
+    part = edz if kind is None else h * dz.abs() + floor_of(dtype) if rounded else h * h * dz.abs() + (2.0 ** -35 if dtype == HF else 2.0 ** -140)
     for at, (p, q), depth in ((1, (dz, w), n), (2, (dz.t(), x), m)):
         want, size = product(p, q)
         err = product((edz + part) if at == 1 else (edz + part).t(), q)[1]
-        close(got[at], want, h * want.abs() + err + (2 * depth + 64) * U * (1.01 * size + err) + floor_of(dtype), "dx" if at == 1 else "dw")
-        if not rounded and kind != "relu" and scale == 1.0:
-            # all errors together, against those of the exact result rounded once
-            once = (want.to(dtype).double() - want).norm()
-            assert float((got[at].double() - want).norm()) <= 1.02 * float(once), at
+        tol = h * want.abs() + err + (2 * depth + 64) * U * (1.01 * size + err) + floor_of(dtype)
+        once = (want.to(dtype).double() - want).norm()
+        for g in (got[at],) + alone[at - 1:at]:
+            close(g, want, tol, "dx" if at == 1 else "dw")
+            if not rounded and kind != "relu" and scale == 1.0 and dtype != F32:
+                # all errors together, against those of the exact result rounded once
+                assert float((g.double() - want).norm()) <= 1.02 * float(once), at
     want = dz.sum(0)
     close(got[3], want, h * want.abs() + edz.sum(0) + (m + 64) * U * (dz.abs() + edz).sum(0) + floor_of(dtype), "db")
 
@@ -108,6 +123,42 @@ def test_gradients_of_16_bit_layers_are_rounded_once(dtype, kind, m, k, n):
 def test_gradients_of_16_bit_layers_one_by_one(dtype, m, k, n):
     check_gradients(m, k, n, dtype, "gelu", one_by_one=True)
     check_gradients(m, k, n, dtype, "relu", one_by_one=True)
+
+
+@pytest.mark.parametrize("m,k,n,kind", EVERY_TILE)
+def test_every_tile_type_and_layout(m, k, n, kind):
+    for dtype in TYPES if kind is None else (BF, HF):
+        check_gradients(m, k, n, dtype, kind, one_by_one=True)
+
+
+@pytest.mark.parametrize("m,k,n,kind,tiles", [(4096, 1024, 4096, None, (0, None)), (2048, 2048, 2048, None, (1, None)), (4096, 4096, 4096, None, (0, 0)),
+                                              (4096, 4096, 4096, "gelu", (0, 0)), (250, 1016, 16360, None, (1, None))])
+def test_large_tiles_are_captured(m, k, n, kind, tiles):
+    """Tiles of more LDS than a launch may have without an attribute: set inside a capture, forward and backward."""
+    import ctypes as C
+    from diffusion_model_nemo_amd import _native as N
+    from diffusion_model_nemo_amd.modules import linear
+    plan = (C.c_int * 7)()
+    assert N.lib().dmn_test_linear_plan(m, k, n, 0 if kind is None else 3, 1, 0, plan) == 0
+    assert plan[0] == tiles[0] and (tiles[1] is None or (plan[2], plan[3]) == (0, tiles[1])), list(plan)
+    x, w = randn((m, k), 1, BF).requires_grad_(True), randn((n, k), 2, BF, k ** -0.5).requires_grad_(True)
+    dy = randn((m, n), 4, BF)
+
+    def step():
+        y = linear(x, w, None, kind)
+        return (y.detach(),) + torch.autograd.grad(y, (x, w), dy)
+
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = step()
+    for turn in range(3):
+        with torch.no_grad():
+            x.copy_(randn((m, k), 20 + turn, BF))
+        graph.replay()
+        kept = [g.clone() for g in got]
+        want = step()
+        torch.cuda.synchronize()
+        assert all(torch.equal(p, q) for p, q in zip(kept, want)), turn
 
 
 @pytest.mark.parametrize("scale", [1e-6, 2e-4])
