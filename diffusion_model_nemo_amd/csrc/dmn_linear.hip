@@ -378,8 +378,9 @@ template <int N> struct Int { static constexpr int value = N; };
 // two parts (TWO; a kernel of its own, because the others would pay 3 % for the choice: 4001 x 4096 into 1024 training 118 : 121 us)
 // the k tiles count twice, and at `turn` the requests go back to the first one, with the high part.
 //
-// Bound by the matrix cores where the large tile fills the chip: 8192^3 bf16 820 us forward, 814 dx, 837 dw (1340, 1350, 1314
-// TFLOP/s; the card's own product library 797, 905, 1030 us), float32 4096^3 960 us (143 TFLOP/s of 154). Per step of 128
+// Bound by the matrix cores where the large tile fills the chip: 8192^3 bf16 827 us forward, 824 dx, 855 dw (1330, 1335, 1286
+// TFLOP/s; the card's own product library 715, 816, 930 us), float32 4096^3 960, 968, 984 us (143 to 140 TFLOP/s; library 914 to
+// 918). Per step of 128
 // bytes of k a 256 x 256 tile keeps them busy for 2048 cycles and brings 64 KB through the CU's first-level cache, 1024
 // cycles at 64 bytes each; 128 x 128 brings half of that for a quarter of the products, which is why it stays below 1000
 // TFLOP/s (4096 x 1024 out of k = 4096: 37 us). What reading the next fragments beside the products, counted waits and
@@ -796,11 +797,13 @@ inline long long ceil_div(long long a, long long b) { return (a + b - 1) / b; }
 // Tile and k split of a product, from its sizes and type alone, by the times that the tiles were measured to take (MI355X, us):
 // `step` per 128 bytes of k and tile of a CU that works through several, `least` for a tile that is alone on its CU, `ends`
 // for what stands around the steps (first requests, epilogue, launch); `together` tiles share a CU. The large tile moves the
-// fewest bytes per product (8192^3 bf16: 820 us; 128 x 128: 1100, 64 x 64: 1520), the others leave fewer CUs without work:
-// 4096 x 1024 out of k = 4096 takes 94 us in 64 large tiles and 37 us in 256 tiles of 128 x 128 with four stages each, which
-// two stages and two tiles per CU turn into 47 us; with 1024 such tiles it is the other way round (52 against 38 us).
-// Where there are too few tiles for the CUs, k is split: the partial products are written and read again at some 4 TB/s, in
-// one more launch.
+// fewest bytes per product (8192^3 bf16 forward: 827 us; 128 x 128 with four stages 1078, with two 961, 64 x 64 1582), the others
+// leave fewer CUs without work: 4096 x 1024 out of k = 4096 takes 88 us in 64 large tiles and 36 to 41 us in 256 tiles of 128 x
+// 128 with four stages each, 43 with two; with 1024 such tiles it is the other way round (4096 x 4096 out of k = 1024: 46 with
+// four stages, 38 with two, 34 in 256 large tiles). Where there are too few tiles for the CUs, k is split: the partial
+// products are written and read again at some 4 TB/s, in one more launch. `ends` is one figure for every epilogue: a forward that
+// keeps z or reads a residual takes longer than its estimate (4096 x 1024 into 4096 with GELU and z: 34 estimated, 48 measured), in all
+// tiles alike.
 struct GemmPlan {
     int tile, splits, per;   // index into kTiles; k tiles are counted in 128 bytes of k
     double us;
@@ -928,14 +931,15 @@ template <typename T, int G> int join_launch(const GemmArgs& g, hipStream_t s) {
     return DMN_OK;
 }
 // Whether the forward takes the kernel for few rows. Its workgroups read all of x each, so x has to be small (us, this kernel
-// against tiles, weights not in the caches: 64 x 2048 into 8192 bf16 19 : 25, 32 x 1000 into 1531 7 : 14, but 32 x 8192 into
-// 2048 28 : 19 and 64 x 8192 44 : 19); and few columns of a long k leave it CUs without work (16 x 8192 into 2048 19 : 15,
-// 16 x 4096 into 512 11 : 9; one row 14 : 14).
+// against tiles, weights not in the caches: 64 x 2048 into 8192 bf16 17 : 25, 32 x 1000 into 1531 5 : 10, but 32 x 8192 into
+// 2048 27 : 18 and 64 x 8192 42 : 19); and few columns of a long k leave it CUs without work (16 x 8192 into 2048 19 : 14,
+// 16 x 4096 into 512 10 : 10; one row 13 : 14, in float32, where the tiles split k, 30 : 25).
 // Where the weight's rows are off 16-byte boundaries the tiles would need a copy of it, and this kernel's loads are slow, the
 // more so the more of x's rows there are; both sides are estimated in us from these times (this kernel : copy and tiles):
-// bf16, k = 4095 into 4095, 1 row 17 : 27, 16 rows 28 : 28, 40 rows 52 : 31; 4095 into 1023, 1 row 17 : 16, 16 rows 28 : 17; 8191
-// into 8191, 4 rows 74 : 82, 16 rows 100 : 83; float32, 4095 into 4095, 16 rows 25 : 50, 40 rows 41 : 50; 8191 into 2047, 8 rows
-// 40 : 50, 40 rows 77 : 52.
+// bf16, k = 4095 into 4095, 1 row 17 : 27, 16 rows 28 : 28, 40 rows 52 : 31; 4095 into 1023, 1 row 17 : 17, 16 rows 28 : 18; 8191
+// into 8191, 4 rows 76 : 83, 16 rows 100 : 86; float32, 4095 into 4095, 16 rows 25 : 49, 40 rows 42 : 50; 8191 into 2047, 8 rows
+// 41 : 50, 40 rows 77 : 51. One estimate serves all types; it takes the slower side at float32 8191 into 8191 with 40 and 64 rows (131
+// and 138 : 205) and, by less, at float32 4095 into 1023 with 8 (21 : 25).
 bool few_rows(const Operand& w, int M, int dtype) {
     const int N = w.rows, K = w.width;
     const long long bytes = (long long)K * elem(dtype);
@@ -1021,6 +1025,10 @@ template <typename T> int forward_run(GemmArgs& g, int dtype, char* ws, hipStrea
     return gemm_run<T, false, false>(g, dtype, ws, s);
 }
 
+// Runs of rows that dz_kernel's workgroups take: more of them keep more CUs busy, and each leaves a partial row of column sums that
+// the join has to read. dz's sums and their join, 16 : 64 : 256 : 1024 runs at most, us: 4096 x 4096 bf16 28 : 24 : 22 : 22, 4001 x 1024
+// 23 : 10 : 12 : 12, 16384 x 1024 float32 59 : 23 : 25 : 29; narrow outputs, where 64 runs are 64 workgroups, would take more: 65536 x
+// 64 bf16 305 : 80 : 27 : 17.
 constexpr int kMaxDzRuns = 64;
 int dz_runs(int M) { return (int)(ceil_div(M, 64) < kMaxDzRuns ? ceil_div(M, 64) : kMaxDzRuns); }
 
