@@ -92,7 +92,7 @@ struct GemmArgs {
     long long ldr;
     void* y;                     // [M][N]
     void* z;                     // [M][N] or null: receives the value in front of the activation
-    int z_rounded;               // z is of the operands' type, else float32
+    int z_exact;                 // z is float32, else of the operands' type
     int act;
 };
 
@@ -103,7 +103,7 @@ struct GemmArgs {
 // times larger, or it would fall below the type's smallest step; both parts are halved, because a slope of up to 1.13 takes a
 // large dy out of the type's range. The backward's matrix work doubles (training step of 4096 x 1024 into 4096 bf16 GELU: 131
 // -> 217 us, of it dz 16 -> 31, the products 74 -> 148, the forward that keeps a float32 z 46 -> 48); a caller who does not want
-// that asks for a rounded z and dz (DMN_LINEAR_ROUNDED).
+// that leaves out DMN_LINEAR_EXACT: z and dz are rounded to the type.
 template <typename T> struct Parts { static constexpr float PRE = 1.f, LOW = 1.f; };
 template <> struct Parts<f16> { static constexpr float PRE = 0.5f, LOW = 2048.f; };
 template <typename T> __device__ __forceinline__ void in_two(float d, T& high, T& low) {
@@ -260,7 +260,7 @@ __device__ __forceinline__ void epilogue(const GemmArgs& g, int m, int n, const 
     typename Pack<T>::vec v;
 #pragma unroll
     for (int i = 0; i < V; ++i) z[i] = acc[i] + bias[i];
-    if (g.z && sizeof(T) == 2 && g.z_rounded) {
+    if (g.z && sizeof(T) == 2 && !g.z_exact) {
 #pragma unroll
         for (int i = 0; i < V; ++i) v[i] = (T)z[i];
         T* p = (T*)g.z + (long long)m * g.N;
@@ -637,7 +637,7 @@ template <typename T, int MF, int NF, int WAVES> __global__ __launch_bounds__(WA
             if (n + e >= g.N) break;
             float z = v[e] + (g.bias ? (float)((const T*)g.bias)[n + e] : 0.f);
             const long long at = (long long)m * g.N + n + e;
-            if (g.z && sizeof(T) == 2 && g.z_rounded) ((T*)g.z)[at] = (T)z;
+            if (g.z && sizeof(T) == 2 && !g.z_exact) ((T*)g.z)[at] = (T)z;
             else if (g.z) ((float*)g.z)[at] = z;
             z = activate<T>(z, g.act);
             if (g.res) z += (float)((const T*)g.res)[(long long)m * g.ldr + n + e];
@@ -802,8 +802,8 @@ inline long long ceil_div(long long a, long long b) { return (a + b - 1) / b; }
 // 128 with four stages each, 43 with two; with 1024 such tiles it is the other way round (4096 x 4096 out of k = 1024: 46 with
 // four stages, 38 with two, 34 in 256 large tiles). Where there are too few tiles for the CUs, k is split: the partial
 // products are written and read again at some 4 TB/s, in one more launch. `ends` is one figure for every epilogue: a forward that
-// keeps z or reads a residual takes longer than its estimate (4096 x 1024 into 4096 with GELU and z: 34 estimated, 48 measured), in all
-// tiles alike.
+// keeps z or reads a residual takes longer than its estimate (4096 x 1024 into 4096 with GELU and z: 34 estimated, 48 measured);
+// whether another tile would hide that better is not modelled.
 struct GemmPlan {
     int tile, splits, per;   // index into kTiles; k tiles are counted in 128 bytes of k
     double us;
@@ -871,9 +871,9 @@ size_t part_bytes(const GemmPlan& p, int M, int N) { return p.splits > 1 ? block
 size_t gemm_workspace(int M, int N, int K, int dtype, int parts) {
     return part_bytes(gemm_plan(M, N, K, dtype, parts), M, N);
 }
-int activation_of(int flags) { return flags & ~DMN_LINEAR_ROUNDED; }
+int activation_of(int flags) { return flags & ~DMN_LINEAR_EXACT; }
 // Parts of dz, of which z is a float32 argument: see Parts.
-int dz_parts(int flags, int dtype) { return dtype != DMN_DT_F32 && activation_of(flags) != ACT_NONE && !(flags & DMN_LINEAR_ROUNDED) ? 2 : 1; }
+int dz_parts(int flags, int dtype) { return dtype != DMN_DT_F32 && activation_of(flags) != ACT_NONE && (flags & DMN_LINEAR_EXACT) ? 2 : 1; }
 
 // An operand in memory: rows of `width` elements, `ld` apart.
 struct Operand {
@@ -1152,7 +1152,7 @@ extern "C" int dmn_linear_forward(const void* x, int64_t ldx, const void* weight
     g.ldr = ldr;
     g.y = y;
     g.z = z;
-    g.z_rounded = (activation & DMN_LINEAR_ROUNDED) != 0;
+    g.z_exact = (activation & DMN_LINEAR_EXACT) != 0;
     g.act = activation_of(activation);
     hipStream_t s = (hipStream_t)stream;
     char* ws = (char*)workspace;

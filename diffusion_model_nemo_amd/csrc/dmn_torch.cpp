@@ -253,7 +253,7 @@ Tensor linear_run(const Rows& x, const Tensor& weight, const Tensor& bias, const
     auto shape = x.t.sizes().vec();
     shape.back() = out;
     Tensor y = at::empty(shape, x.t.options());
-    if (z) *z = at::empty({rows, out}, act & DMN_LINEAR_ROUNDED ? x.t.options() : x.t.options().dtype(at::kFloat));
+    if (z) *z = at::empty({rows, out}, act & DMN_LINEAR_EXACT ? x.t.options().dtype(at::kFloat) : x.t.options());
     const Rows r = residual.defined() ? rows_of(residual) : Rows{Tensor(), 0};
     const size_t bytes = api.linear_forward_workspace(x.t.data_ptr(), x.ld, weight.data_ptr(), rows, (int)width, (int)out, code);
     const Tensor ws = workspace(bytes, x.t);
@@ -268,7 +268,7 @@ struct LinearNode : torch::autograd::Function<LinearNode> {
         const Tensor bias = or_none(bias_);
         const Rows r = rows_of(x, kLinearStride);
         // the value in front of the activation is all that the backward needs of the forward's results
-        const bool want_z = (act & ~DMN_LINEAR_ROUNDED) != 0 && (x.requires_grad() || weight.requires_grad() || (bias.defined() && bias.requires_grad()));
+        const bool want_z = (act & ~DMN_LINEAR_EXACT) != 0 && (x.requires_grad() || weight.requires_grad() || (bias.defined() && bias.requires_grad()));
         Tensor z;
         Tensor y = linear_run(r, weight, bias, or_none(residual), act, stream, want_z ? &z : nullptr);
         // x for dW and the weight for dx alone: what is not needed is not kept, and may be overwritten before the backward

@@ -21,7 +21,7 @@ import torch.nn as nn
 from .. import _native as N
 
 ACTIVATIONS = {None: 0, "relu": 1, "silu": 2, "gelu": 3}
-ROUNDED = 16   # DMN_LINEAR_ROUNDED of include/dmn.h
+EXACT = 16   # DMN_LINEAR_EXACT of include/dmn.h
 
 
 def _stream(x: torch.Tensor, what: str):
@@ -54,7 +54,7 @@ def linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] =
     code = ACTIVATIONS.get(activation)
     if code is None:
         raise ValueError(f"activation must be one of {list(ACTIVATIONS)}, got {activation!r}")
-    return N.ops().linear(x, weight, bias, code | ROUNDED if rounded_backward else code, residual, _stream(x, "linear"))
+    return N.ops().linear(x, weight, bias, code if rounded_backward else code | EXACT, residual, _stream(x, "linear"))
 
 
 class LayerNorm(nn.Module):

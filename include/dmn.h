@@ -292,22 +292,23 @@ int dmn_layer_norm_backward(const void* dy, int64_t lddy, const void* x, int64_t
                             void* workspace, size_t workspace_bytes, void* stream);
 
 /* y = act(x weight^T + bias) + residual: x [rows][in] (ldx apart), weight [out][in], bias [out] or NULL, residual [rows][out]
- * (ldr apart) or NULL, all of `dtype`; y [rows][out]. activation: 0 none, 1 ReLU, 2 SiLU, 3 GELU (exact), + DMN_LINEAR_ROUNDED.
- * z: optional [rows][out], receives x weight^T + bias for the backward, float32 (rounded to dtype with DMN_LINEAR_ROUNDED). rows may be 0; rows < 2^27, in, out and row
+ * (ldr apart) or NULL, all of `dtype`; y [rows][out]. activation: 0 none, 1 ReLU, 2 SiLU, 3 GELU (exact), and DMN_LINEAR_EXACT
+ * added to it for a backward that rounds once. z: optional [rows][out], receives x weight^T + bias for the backward, rounded to
+ * dtype (float32 with DMN_LINEAR_EXACT). rows may be 0; rows < 2^27, in, out and row
  * strides of x and dy < 2^20. Products run on the matrix cores with float32 accumulation (float32 operands exactly).
  * workspace: 256-byte aligned; 0 bytes needed: may be NULL. What is needed depends on the sizes and on whether the operands'
  * rows lie on 16-byte boundaries (the workspace functions look at the addresses for nothing else): copies of those that do
  * not, partial products where k is split, the backward's dz. */
-#define DMN_LINEAR_ROUNDED 16
+#define DMN_LINEAR_EXACT 16
 size_t dmn_linear_forward_workspace_bytes(const void* x, int64_t ldx, const void* weight, int64_t rows, int in, int out, int dtype);
 int dmn_linear_forward(const void* x, int64_t ldx, const void* weight, const void* bias, const void* residual, int64_t ldr,
                        void* y, void* z, int64_t rows, int in, int out, int activation, int dtype, void* workspace,
                        size_t workspace_bytes, void* stream);
 /* dx [rows][in], dweight [out][in], dbias [out] (each optional, overwritten) from dy [rows][out] (lddy apart) and the
- * forward's x, weight and z (z only with an activation). The residual's gradient is dy. dz = dy act'(z) enters the products as
- * the sum of two numbers of a 16-bit dtype (its leading 16 bits in bfloat16, 22 in float16), so that dx and dweight are
- * rounded once. With DMN_LINEAR_ROUNDED, the same in both calls, z and dz are rounded to dtype: half of the products' matrix work
- * and of z's memory for errors sqrt 2 larger. dbias adds dz up in float32 either way. */
+ * forward's x, weight and z (z only with an activation). The residual's gradient is dy. dz = dy act'(z) is rounded to dtype where
+ * it enters the products, not where dbias adds it up. With DMN_LINEAR_EXACT (the same in both calls) it enters them as the sum of
+ * two numbers of a 16-bit dtype (its leading 16 bits in bfloat16, 22 in float16), so that dx and dweight are rounded once: twice
+ * the products' matrix work for errors sqrt 2 smaller, and for float16 gradients near its smallest step far smaller. */
 size_t dmn_linear_backward_workspace_bytes(const void* dy, int64_t lddy, const void* x, int64_t ldx, const void* weight,
                                            int64_t rows, int in, int out, int activation, int dtype);
 int dmn_linear_backward(const void* dy, int64_t lddy, const void* x, int64_t ldx, const void* weight, const void* z, void* dx,

@@ -144,11 +144,11 @@ def test_gradient_clipping_hook_takes_the_configured_value(monkeypatch):
         m.configure_gradient_clipping(opt, gradient_clip_algorithm="value")
 
 
-def test_linear_entry_points_take_the_rounded_flag_with_an_activation_only():
+def test_linear_entry_points_take_the_exact_flag():
     lib = _N().lib()
     need = lambda act, dt: lib.dmn_linear_backward_workspace_bytes(X, 4096, X, 1024, X, 4096, 1024, 4096, act, dt)  # noqa: E731
     dz = 4096 * 4096 * 2
-    assert need(3, 1) - need(3 + 16, 1) >= dz and need(3, 2) - need(3 + 16, 2) >= dz     # dz in two parts, or one
+    assert need(3 + 16, 1) - need(3, 1) >= dz and need(3 + 16, 2) - need(3, 2) >= dz     # dz in two parts, or one
     assert need(0, 1) == need(16, 1) and need(3, 0) == need(3 + 16, 0)
     for act in (20, 31, 32, 8, -16):
         assert lib.dmn_linear_backward(X, 8, X, 8, X, X, X, X, X, 4, 8, 8, act, 1, None, 0, None) == -1
@@ -249,7 +249,7 @@ def test_every_compiled_tile_has_a_tested_size():
     lib = _N().lib()
     seen = set()
     for m, k, n, kind in EVERY_TILE:
-        act = 0 if kind is None else 3
+        act = 0 if kind is None else 3 + 16
         for dt in range(3) if act == 0 else (1, 2):
             for alone in (0, 1):
                 p = (C.c_int * 7)()

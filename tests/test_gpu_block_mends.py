@@ -139,7 +139,7 @@ def test_large_tiles_are_captured(m, k, n, kind, tiles):
     from diffusion_model_nemo_amd import _native as N
     from diffusion_model_nemo_amd.modules import linear
     plan = (C.c_int * 7)()
-    assert N.lib().dmn_test_linear_plan(m, k, n, 0 if kind is None else 3, 1, 0, plan) == 0
+    assert N.lib().dmn_test_linear_plan(m, k, n, 0 if kind is None else 3 + 16, 1, 0, plan) == 0
     assert plan[0] == tiles[0] and (tiles[1] is None or (plan[2], plan[3]) == (0, tiles[1])), list(plan)
     x, w = randn((m, k), 1, BF).requires_grad_(True), randn((n, k), 2, BF, k ** -0.5).requires_grad_(True)
     dy = randn((m, n), 4, BF)
@@ -329,3 +329,24 @@ def test_linear_keeps_only_what_its_gradients_need(kind):
     before = torch.cuda.memory_allocated()
     y = linear(given * 1.0, frozen)
     assert torch.cuda.memory_allocated() - before <= y.numel() * y.element_size() + 512     # the product's input is gone again
+
+
+def test_c_callers_keep_a_rounded_z_unless_they_ask():
+    """z of the operands' type and a rounded dz without DMN_LINEAR_EXACT, as `rounded_backward=True` computes them."""
+    from diffusion_model_nemo_amd import _native as N
+    lib, s = N.lib(), N.current_stream_handle()
+    m, k, n = 130, 72, 88
+    x, w, b, dy = randn((m, k), 1, BF), randn((n, k), 2, BF, 0.1), randn((n,), 3, BF), randn((m, n), 4, BF)
+    for flag, rounded in ((0, True), (16, False)):
+        z = torch.empty((m + 1, n), dtype=BF if rounded else torch.float32, device="cuda")
+        z[m] = 7.0
+        y, dx, dw, db = (torch.empty_like(t) for t in (dy, x, w, b))
+        nb = max(lib.dmn_linear_forward_workspace_bytes(x.data_ptr(), k, w.data_ptr(), m, k, n, 1),
+                 lib.dmn_linear_backward_workspace_bytes(dy.data_ptr(), n, x.data_ptr(), k, w.data_ptr(), m, k, n, 3 + flag, 1))
+        ws = torch.empty(nb, dtype=torch.uint8, device="cuda")
+        N.check(lib.dmn_linear_forward(x.data_ptr(), k, w.data_ptr(), b.data_ptr(), None, 0, y.data_ptr(), z.data_ptr(), m, k, n, 3 + flag, 1,
+                                       ws.data_ptr(), nb, s))
+        N.check(lib.dmn_linear_backward(dy.data_ptr(), n, x.data_ptr(), k, w.data_ptr(), z.data_ptr(), dx.data_ptr(), dw.data_ptr(), db.data_ptr(),
+                                        m, k, n, 3 + flag, 1, ws.data_ptr(), nb, s))
+        want = grads_of(x, w, b, "gelu", dy, rounded_backward=rounded)
+        assert all(torch.equal(p, q) for p, q in zip((y, dx, dw, db), want)) and bool((z[m] == 7.0).all())
