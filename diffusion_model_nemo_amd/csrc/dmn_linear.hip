@@ -521,7 +521,7 @@ template <typename T, int NT> __device__ __forceinline__ void column_join(const 
 }
 // Both of the backward's products in one launch: they read the same dz, and neither's tiles alone fill the chip evenly (one after
 // the other each has its own first requests, last tiles and launch). The product with the longer tiles goes in front. Both
-// products, one after the other and so (us): 4096 x 1024 into 4096 bf16 85 : 71, 2048 x 1024 into 1024 27 : 19, 4096 x 320 into
+// products, one after the other and so (us, dz in one part): 4096 x 1024 into 4096 bf16 85 : 71, 2048 x 1024 into 1024 27 : 19, 4096 x 320 into
 // 1280 29 : 19.5, 256 x 320 into 320 8.0 : 5.0, 16384 x 256 into 1024 float32 149 : 139; 4096^3 bf16, whose 256 x 256 tiles come
 // out even, 214 : 265.
 struct PairArgs {
