@@ -77,14 +77,16 @@ void check_recorded(const char* what, std::initializer_list<const std::optional<
         if (t->has_value() && (*t)->_fw_grad(0).defined())
             throw std::runtime_error(c10::str(what, " has no forward-mode derivative: an input is a dual tensor"));
 }
+// Contiguous, with the values that are in memory: a view with the negation bit (the imaginary part of a conjugate) is copied.
+Tensor dense(const Tensor& t) { return (t.is_neg() ? t.resolve_neg() : t).contiguous(); }
 // p on x's device, of `shape` and of x's type (or float32 where `or_float`); comes back contiguous
-Tensor checked_param(const std::optional<Tensor>& p, const char* name, at::IntArrayRef shape, const Tensor& x, bool or_float) {
+Tensor checked_param(const std::optional<Tensor>& p, const char* name, at::IntArrayRef shape, const Tensor& x, bool or_float, bool rows = false) {
     if (!p.has_value()) return Tensor();
     if (p->device() != x.device()) throw std::runtime_error(c10::str(name, " on ", p->device(), ", input on ", x.device()));
     if (p->sizes() != shape) throw py::value_error(c10::str(name, " must have shape ", shape, ", got ", p->sizes()));
     if (p->scalar_type() != x.scalar_type() && !(or_float && p->scalar_type() == at::kFloat))
         throw py::value_error(c10::str(name, " must be ", x.scalar_type(), or_float ? " or Float" : "", ", got ", p->scalar_type()));
-    return *p;
+    return rows ? *p : dense(*p);
 }
 
 // `t` as rows of contiguous elements `ld` apart, copied only where its strides do not allow that.
@@ -94,6 +96,7 @@ struct Rows {
 };
 Rows rows_of(const Tensor& t, int64_t limit = INT64_MAX) {   // strides from `limit` on are copied too
     const int64_t width = t.size(-1);
+    if (t.is_neg()) return {dense(t), width};
     if (t.is_contiguous()) return {t, width};
     if (t.dim() == 2 && (t.stride(1) == 1 || width == 1) && t.stride(0) >= width && t.stride(0) < limit) return {t, t.stride(0)};
     return {t.contiguous(), width};
@@ -235,8 +238,6 @@ Tensor layer_norm(const Tensor& x, const std::optional<Tensor>& weight_, const s
     Tensor weight = checked_param(weight_, "weight", shape, x, true), bias = checked_param(bias_, "bias", shape, x, true);
     if (weight.defined() && bias.defined() && weight.scalar_type() != bias.scalar_type())
         throw py::value_error(c10::str("weight and bias must have one type, got ", weight.scalar_type(), " and ", bias.scalar_type()));
-    if (weight.defined()) weight = weight.contiguous();
-    if (bias.defined()) bias = bias.contiguous();
     c10::DeviceGuard guard(x.device());
     if (at::GradMode::is_enabled() && (x.requires_grad() || (weight.defined() && weight.requires_grad()) || (bias.defined() && bias.requires_grad()))) {
         check_capture(stream, x, {&x, &weight, &bias});
@@ -325,9 +326,8 @@ Tensor linear(const Tensor& x, const Tensor& weight_, const std::optional<Tensor
     if (x.dim() == 0 || x.size(-1) != width) throw py::value_error(c10::str("expected a last axis of ", width, ", got ", x.sizes()));
     auto shape = x.sizes().vec();
     shape.back() = out;
-    Tensor weight = checked_param(weight_, "weight", weight_.sizes(), x, false).contiguous();
-    Tensor bias = checked_param(bias_, "bias", {out}, x, false), residual = checked_param(residual_, "residual", shape, x, false);
-    if (bias.defined()) bias = bias.contiguous();
+    Tensor weight = checked_param(weight_, "weight", weight_.sizes(), x, false);
+    Tensor bias = checked_param(bias_, "bias", {out}, x, false), residual = checked_param(residual_, "residual", shape, x, false, true);
     c10::DeviceGuard guard(x.device());
     if (at::GradMode::is_enabled() && (x.requires_grad() || weight.requires_grad() || (bias.defined() && bias.requires_grad()) ||
                                        (residual.defined() && residual.requires_grad()))) {
@@ -358,12 +358,12 @@ py::object clip_grads(const py::list& params, const py::object& out, bool inf_no
         if (!g.defined()) continue;
         const int code = code_of(g.scalar_type());
         if (table.empty()) device = g.device();
-        if (code < 0 || !g.is_cuda() || g.device() != device || g.layout() != at::kStrided || !g.is_contiguous() || g.is_inference()) return py::none();
+        if (code < 0 || !g.is_cuda() || g.device() != device || g.layout() != at::kStrided || !g.is_contiguous() || g.is_neg() || g.is_inference()) return py::none();
         Tensor o = g;
         if (to_out) {
             if (!THPVariable_Check(outs[i].ptr())) return py::none();
             o = THPVariable_Unpack(outs[i].ptr());
-            if (code_of(o.scalar_type()) < 0 || o.device() != device || o.layout() != at::kStrided || !o.is_contiguous() || o.is_inference() ||
+            if (code_of(o.scalar_type()) < 0 || o.device() != device || o.layout() != at::kStrided || !o.is_contiguous() || o.is_neg() || o.is_inference() ||
                 o.sizes() != g.sizes())
                 return py::none();
         }

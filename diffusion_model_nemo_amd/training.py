@@ -275,15 +275,15 @@ def _clip_one_by_one(params, norm_type, max_norm, error_if_nonfinite, grad_scale
             raise RuntimeError(f"gradients on {dev} and {g.device}: all must be on one device")
         if g.layout != torch.strided or g.dtype not in N.DTYPE_CODES:
             raise ValueError(f"gradients must be dense float32, bfloat16 or float16 tensors, got {g.dtype} ({g.layout})")
-        if not g.is_contiguous() and (out is not None or not _dense(g)):
-            copied.append((g, g.contiguous()))
+        if g.is_neg() or (not g.is_contiguous() and (out is not None or not _dense(g))):
+            copied.append((g, g.resolve_neg().contiguous()))
     if out is None and copied:
         _refuse_shared_memory([g for g, _ in copied], grads)
     dense = {id(g): c for g, c in copied}
     srcs = [dense.get(id(g), g) for g in grads]
     if out is not None:
         for o, g in zip(out, grads):
-            if o.device != dev or o.shape != g.shape or o.dtype not in N.DTYPE_CODES or not o.is_contiguous():
+            if o.device != dev or o.shape != g.shape or o.dtype not in N.DTYPE_CODES or not o.is_contiguous() or o.is_neg():
                 raise ValueError("out must hold contiguous float32 / bfloat16 / float16 tensors of the gradients' shapes, on "
                                  "their device")
     dsts = srcs if out is None else out

@@ -350,3 +350,41 @@ def test_c_callers_keep_a_rounded_z_unless_they_ask():
                                         m, k, n, 3 + flag, 1, ws.data_ptr(), nb, s))
         want = grads_of(x, w, b, "gelu", dy, rounded_backward=rounded)
         assert all(torch.equal(p, q) for p, q in zip((y, dx, dw, db), want)) and bool((z[m] == 7.0).all())
+
+
+@pytest.mark.parametrize("width", [1, 24])
+def test_views_with_the_negation_bit_are_read_with_their_sign(width):
+    """What torch.conj(z).imag gives: memory that holds the negative of the values."""
+    from diffusion_model_nemo_amd.modules import layer_norm, linear
+    from diffusion_model_nemo_amd.training import clip_grad_norm_
+    x, w, b, r, dy = randn((9, width), 1), randn((width, width), 2), randn((width,), 3), randn((9, width), 4), randn((9, width), 5)
+    neg = [torch._neg_view(t) for t in (x, w, b, r, dy)]
+    for t in neg:
+        assert t.is_neg() and t.is_contiguous()
+    plain = [t.clone() for t in neg]
+    assert torch.equal(plain[0], -x) and not plain[0].is_neg()
+    strided = torch.complex(x, r).conj().imag                       # rows two elements apart
+    assert strided.is_neg() and torch.equal(linear(strided, w), linear(-r, w)) and torch.equal(layer_norm(strided), layer_norm(-r))
+
+    def both(op, n):
+        out = []
+        for args in (neg, plain):
+            leaves = [t.detach().requires_grad_(True) for t in args[:n]]
+            y = op(*leaves)
+            out.append((y,) + torch.autograd.grad(y, leaves, args[4]))
+        assert all(torch.equal(p, q) for p, q in zip(*out))
+
+    both(lambda x, w, b, r: linear(x, w, b, "gelu", r), 4)
+    both(lambda x, w, b: layer_norm(x, w[0], b), 3)
+    p = [torch.nn.Parameter(torch.zeros_like(t)) for t in (x, r)]
+    p[0].grad, p[1].grad = neg[0], r.clone()
+    norm = clip_grad_norm_(p, 0.5)
+    want = torch.linalg.vector_norm(torch.cat([plain[0], r]).double())
+    assert abs(float(norm) - float(want)) <= 4 * U * float(want)
+    close(p[0].grad.clone(), plain[0].double() * 0.5 / want, 8 * U * plain[0].double().abs(), "clipped")
+    out = [torch.empty_like(t) for t in (x, r)]
+    p[0].grad = torch._neg_view(x.neg())                             # x again
+    clip_grad_norm_(p, 1e9, out=out)
+    assert torch.equal(out[0], p[0].grad) and torch.equal(out[1], p[1].grad)
+    with pytest.raises(ValueError):
+        clip_grad_norm_(p, 1.0, out=[torch._neg_view(out[0]), out[1]])
